@@ -387,7 +387,8 @@ def _plain_sample(state):
     most = x.amax(1, keepdim=True)
     temperature = state["temperature"].unsqueeze(1)
     greedy = temperature <= 0
-    z = torch.where(x == most, 0.0, torch.where(greedy, -math.inf, (x - most) / torch.where(greedy, 1.0, temperature)))
+    z = (x - most) * (1.0 / torch.where(greedy, 1.0, temperature))
+    z = torch.where(x == most, 0.0, torch.where(greedy, -math.inf, z))
     share = z.exp()
     weight = (share * _UNIT).floor().long()
     top_k = state["top_k"].unsqueeze(1)
