@@ -88,6 +88,18 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
          _P, _I64P, _P, _I64P, _I32, _I64, _I32, _I32, _I32, _P, _P],
     ),
     "augur_kv_decode_layer": (ctypes.c_int, [_P, _I32, _P, _P, _P, _P, _P]),
+    "augur_kv_shared_prefix_attention": (ctypes.c_int, [_P, _I32, _P, _P, _P]),
+    "augur_kv_shared_prefix_workspace": (ctypes.c_int, [_I32, _I32, _I32, _I32, _I32, _I32, _I64P, _I64P]),
+    "augur_kv_rope_axes_scatter": (
+        ctypes.c_int,
+        [_P, _I64P, _P, _I64P, _I32, _P, _I64P, _P, _I64P, _I32, _P, _P, _I64P, _I64, _I32, _P, _I64, _P, _I64P,
+         _I32, _P, _P, _I64, _I32, _I32, _P, _P],
+    ),
+    "augur_kv_sample": (
+        ctypes.c_int,
+        [_P, _I64, _I32, _I32, _I32, _P, _P, ctypes.c_float, _P, _I32, _P, ctypes.c_float, _P, ctypes.c_float,
+         _P, _P, _P],
+    ),
     "augur_kv_signal": (ctypes.c_int, [_P, _I32, _P]),
     "augur_kv_wait": (ctypes.c_int, [_P, _I32, _I64, _P, _P]),
 }
@@ -128,6 +140,48 @@ class DecodeArgs(ctypes.Structure):
         ("counters_bytes", ctypes.c_int64),
         ("scratch", ctypes.c_void_p),
         ("scratch_bytes", ctypes.c_int64),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class SharedPrefixArgs(ctypes.Structure):
+    """augur_kv_shared_prefix_args: a shared-prefix attention plan and what its layers share (field for field)."""
+
+    _fields_ = [
+        ("k_pool", ctypes.c_void_p),
+        ("v_pool", ctypes.c_void_p),
+        ("pool_strides", ctypes.c_int64 * 4),
+        ("num_blocks", ctypes.c_int64),
+        ("block_size", ctypes.c_int32),
+        ("n_layers", ctypes.c_int32),
+        ("n_q_heads", ctypes.c_int32),
+        ("n_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("batch", ctypes.c_int32),
+        ("flags", ctypes.c_int32),
+        ("q_strides", ctypes.c_int64 * 2),
+        ("out_strides", ctypes.c_int64 * 2),
+        ("block_tables", ctypes.c_void_p),
+        ("tables_stride", ctypes.c_int64),
+        ("max_blocks", ctypes.c_int64),
+        ("seq_lens", ctypes.c_void_p),
+        ("shared_lens", ctypes.c_void_p),
+        ("max_own_len", ctypes.c_int32),
+        ("n_items", ctypes.c_int32),
+        ("items", ctypes.c_void_p),
+        ("members", ctypes.c_void_p),
+        ("run_blocks", ctypes.c_void_p),
+        ("ref_starts", ctypes.c_void_p),
+        ("refs", ctypes.c_void_p),
+        ("n_members", ctypes.c_int32),
+        ("n_run_blocks", ctypes.c_int32),
+        ("n_refs", ctypes.c_int32),
+        ("n_slabs", ctypes.c_int32),
+        ("scratch", ctypes.c_void_p),
+        ("scratch_bytes", ctypes.c_int64),
+        ("counters", ctypes.c_void_p),
+        ("counters_bytes", ctypes.c_int64),
         ("status", ctypes.c_void_p),
     ]
 

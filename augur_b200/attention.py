@@ -348,3 +348,302 @@ def paged_attention(
     out = paged_prefill_attention(q[0].transpose(0, 1).contiguous(), cache, layer_idx, [block_table], [q.shape[2]],
                                   generic=generic, kernel=kernel)
     return out.transpose(0, 1).unsqueeze(0)
+
+
+# ---------------------------------------------------------------- sequences that share blocks
+
+_ITEM_FIELDS = 12
+_TILE_ROWS = 128
+_TILE_KEYS = 128
+# A run is worth a pass of its own when the sequences would otherwise re-read this many positions
+_MIN_SAVED_TOKENS = 256
+
+
+def _shared_runs(rows: np.ndarray, full: np.ndarray, min_saved: int) -> tuple[list[tuple[np.ndarray, int, int]], np.ndarray]:
+    """The runs of blocks that several sequences hold at the same place: a list of (members,
+    first block, last block + 1), and how many leading blocks of each sequence they cover.
+
+    rows: int32 [batch, width] block ids; full: blocks of each sequence that are filled. The
+    tables form a trie over their block ids; a stretch of it that at least two sequences pass
+    is a run when it spares min_saved blocks of reading, and otherwise joins the stretches
+    that follow it (which then read it once each)."""
+    batch = rows.shape[0]
+    covered = np.zeros(batch, dtype=np.int64)
+    runs: list[tuple[np.ndarray, int, int]] = []
+
+    def split(members: np.ndarray, col: int) -> list[np.ndarray]:
+        """members still filled at column col, grouped by their block there."""
+        members = members[full[members] > col]
+        if members.size < 2:
+            return []
+        ids = rows[members, col]
+        order = np.argsort(ids, kind="stable")
+        cuts = np.flatnonzero(np.diff(ids[order])) + 1
+        return [np.sort(members[g]) for g in np.split(order, cuts) if g.size >= 2]
+
+    stack = [(group, 0, 0) for group in reversed(split(np.arange(batch), 0))]
+    while stack:
+        members, start, col = stack.pop()  # equal in [start, col); [0, start) is covered
+        limit = int(full[members].min())
+        same = (rows[members, col:limit] == rows[members[0], col:limit]).all(axis=0)
+        differ = np.flatnonzero(~same)
+        end = col + int(differ[0]) if differ.size else limit
+        if (members.size - 1) * (end - start) >= min_saved:
+            runs.append((members, start, end))
+            covered[members] = end
+            start = end
+        stack.extend((group, start, end) for group in reversed(split(members, end)))
+    return runs, covered
+
+
+def _ranges(tiles: Sequence[int], units: Sequence[int], ctas: int) -> list[int]:
+    """Into how many key ranges each run's tiles are cut: tiles[i] key tiles, each range an
+    item for each of units[i] (row tiles x KV heads). The ranges are as short as one wave of
+    CTAs (one an SM) allows; where the runs alone exceed a wave, as long as three waves make
+    them, so that the last wave's waste is small."""
+    total = sum(t * u for t, u in zip(tiles, units))
+    waves = 1 if sum(units) <= ctas else 3
+    per = max(2, -(-total // (ctas * waves)))
+    while waves == 1 and sum(-(-t // per) * u for t, u in zip(tiles, units)) > ctas:
+        per += max(1, per // 16)
+    return [-(-t // per) for t in tiles]
+
+
+class SharedPrefixTables:
+    """Device plan of a decode step whose sequences share blocks, reusable across layers.
+
+    Built from the batch's block tables as they stand (each table's seq_len counts the new
+    token, as for DecodeTables): the runs of full blocks that several sequences hold in common
+    (PagedSequences.fork and its prefix cache make them) are found, nested ones included, and
+    cut into work items; the tables, lengths and the plan go to the device in one pinned copy.
+    A batch that shares nothing gets an empty plan and is attended sequence by sequence.
+    """
+
+    def __init__(self, cache: PagedKVCache, tables: Sequence[SequenceBlockTable], n_q_heads: int,
+                 seq_lens: Sequence[int] | None = None, stream: torch.cuda.Stream | None = None) -> None:
+        """stream: the stream the copy is ordered on (the current one by default); launches on
+        another stream wait for it."""
+        L, NB, Hkv, bs, D = cache.keys.shape
+        if n_q_heads <= 0 or n_q_heads % Hkv != 0:
+            raise ValueError("n_q_heads must be a positive multiple of the cache's KV heads")
+        lens = [t.seq_len for t in tables] if seq_lens is None else [int(n) for n in seq_lens]
+        if len(lens) != len(tables):
+            raise ValueError("seq_lens and tables must have the same length")
+        if any(t.block_size != bs for t in tables):
+            raise ValueError("block table block_size must equal the cache block size")
+        device = cache.keys.device
+        B, groups = len(tables), n_q_heads // Hkv
+        packed, width = _table_rows(tables, lens, 0)
+        rows = packed[: B * width].reshape(B, width)
+        lens_np = np.asarray(lens, dtype=np.int64)
+        runs, covered = _shared_runs(rows, lens_np // bs, -(-_MIN_SAVED_TOKENS // bs))
+        self.batch, self.n_q_heads, self.block_size = B, n_q_heads, bs
+        self.max_seq_len = max(lens, default=0)
+        self.shared_lens = covered * bs
+        self.max_own_len = int((lens_np - self.shared_lens).max(initial=0))
+        self.runs = [(members.tolist(), start * bs, end * bs) for members, start, end in runs]
+        ctas = _sm_count(device)
+        row_tiles = [-(-m.size * groups // _TILE_ROWS) for m, _, _ in runs]
+        tiles = [-(-(end - start) * bs // _TILE_KEYS) for _, start, end in runs]
+        ranges = _ranges(tiles, [-(-rt // 2) * Hkv for rt in row_tiles], ctas)
+        items: list[tuple[int, ...]] = []
+        refs: list[list[tuple[int, ...]]] = [[] for _ in range(B)]
+        member0 = block0 = slab = 0
+        for (members, start, end), rt, t, n in zip(runs, row_tiles, tiles, ranges):
+            n_rows, n_blocks = members.size * groups, end - start
+            cuts = [min(n_blocks * bs, (t * c // n) * _TILE_KEYS) for c in range(n)] + [n_blocks * bs]
+            for h in range(Hkv):
+                for tile in range(0, rt, 2):
+                    at = slab + (h * rt + tile) * n
+                    pair = tile + 1 < rt
+                    items.extend((member0, n_rows, block0, n_blocks, h, tile * _TILE_ROWS, cuts[c], cuts[c + 1],
+                                  at + c, at + n + c if pair else -1, 0, 0) for c in range(n))
+            for place, b in enumerate(members.tolist()):
+                refs[b].append((slab, n, place, rt))
+            member0 += members.size
+            block0 += n_blocks
+            slab += Hkv * rt * n
+        # the longest items first: the last wave is made of short ones
+        items.sort(key=lambda i: (i[6] - i[7]) * (2 if i[9] >= 0 else 1))
+        self.n_items, self.n_slabs, self.n_members, self.n_run_blocks = len(items), slab, member0, block0
+        starts = np.zeros(B + 1, dtype=np.int32)
+        np.cumsum([len(r) for r in refs], out=starts[1:])
+        flat = [f for r in refs for f in r]
+        self.n_refs = len(flat)
+        none = np.empty(0, dtype=np.int32)
+        parts = {
+            "refs": np.asarray(flat, dtype=np.int32).reshape(-1),  # first: 16-byte aligned
+            "items": np.asarray(items, dtype=np.int32).reshape(-1),
+            "blocks": packed,
+            "shared": self.shared_lens.astype(np.int32),
+            "starts": starts,
+            "members": np.concatenate([m for m, _, _ in runs]).astype(np.int32) if runs else none,
+            "run_blocks": np.concatenate([rows[m[0], s:e] for m, s, e in runs]) if runs else none,
+        }
+        dev = upload_int32(np.concatenate(list(parts.values())), device, stream)
+        self._dev, at = {}, 0
+        for name, part in parts.items():
+            self._dev[name] = dev[at: at + part.size]
+            at += part.size
+        self.blocks = self._dev["blocks"][: B * width].view(B, width)
+        self.lens = self._dev["blocks"][B * width:]
+        self._device = device
+        self.uploaded: torch.cuda.Event | None = None
+        if device.type == "cuda":
+            self.uploaded = torch.cuda.Event()
+            self.uploaded.record(stream if stream is not None else torch.cuda.current_stream(device))
+        self._fast: tuple | None = None
+
+    def _prepare(self, q: Tensor, out: Tensor, cache: PagedKVCache, st: torch.cuda.Stream, flags: int) -> _lib.SharedPrefixArgs:
+        """The argument block of a call with q and out laid out like these ([batch, heads, head_dim])."""
+        lib = _lib.load()
+        L, NB, Hkv, bs, D = cache.keys.shape
+        Hq = self.n_q_heads
+        if self.uploaded is not None:
+            st.wait_event(self.uploaded)
+        cnt, scr = _shared_workspace(lib, q.device, st, (self.n_slabs, self.batch, Hq, Hkv, D, self.max_own_len))
+        d, a = self._dev, _lib.SharedPrefixArgs()
+        a.k_pool, a.v_pool = cache.keys.data_ptr(), cache.values.data_ptr()
+        a.pool_strides[:] = cache.keys.stride()[:4]
+        a.num_blocks, a.block_size, a.n_layers = NB, bs, L
+        a.n_q_heads, a.n_kv_heads, a.head_dim, a.dtype, a.batch, a.flags = Hq, Hkv, D, _ops.dtype_code(q), self.batch, flags
+        a.q_strides[:] = q.stride()[:2]
+        a.out_strides[:] = out.stride()[:2]
+        a.block_tables, a.tables_stride, a.max_blocks = self.blocks.data_ptr(), self.blocks.stride(0), self.blocks.shape[1]
+        a.seq_lens, a.shared_lens, a.max_own_len = self.lens.data_ptr(), d["shared"].data_ptr(), self.max_own_len
+        a.n_items, a.n_members, a.n_run_blocks, a.n_refs, a.n_slabs = (
+            self.n_items, self.n_members, self.n_run_blocks, self.n_refs, self.n_slabs)
+        a.items, a.members, a.run_blocks = d["items"].data_ptr(), d["members"].data_ptr(), d["run_blocks"].data_ptr()
+        a.ref_starts, a.refs = d["starts"].data_ptr(), d["refs"].data_ptr()
+        a.scratch, a.scratch_bytes = scr.data_ptr(), scr.numel()
+        a.counters, a.counters_bytes = cnt.data_ptr(), cnt.numel() * 4
+        a.status = _ops.status_word(q.device).data_ptr()
+        a._keep = (cnt, scr, cache)  # what the block points into stays alive with it
+        return a
+
+
+_shared_workspaces: dict[tuple[int, int], tuple[Tensor, Tensor]] = {}
+_sm_counts: dict[int, int] = {}
+
+
+def _sm_count(device: torch.device) -> int:
+    if device.type != "cuda":
+        return 148
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    if idx not in _sm_counts:
+        _sm_counts[idx] = torch.cuda.get_device_properties(idx).multi_processor_count
+    return _sm_counts[idx]
+
+
+def _shared_workspace(lib, device: torch.device, st: torch.cuda.Stream, sizes: tuple) -> tuple[Tensor, Tensor]:
+    """Counters (zeroed once; every call leaves them zero) and scratch, one pair per (device,
+    stream), grown on demand: calls on one stream run in order, so they can share them."""
+    need_c, need_s = ctypes.c_int64(0), ctypes.c_int64(0)
+    _lib.check(lib.augur_kv_shared_prefix_workspace(*sizes, ctypes.byref(need_c), ctypes.byref(need_s)),
+               "augur_kv_shared_prefix_workspace")
+    key = (device.index, st.cuda_stream)
+    cnt, scr = _shared_workspaces.get(key, (None, None))
+    if cnt is None or cnt.numel() * 4 < need_c.value or scr.numel() < need_s.value:
+        with torch.cuda.stream(st):
+            if cnt is None or cnt.numel() * 4 < need_c.value:
+                cnt = torch.zeros(max(1, need_c.value // 4), dtype=torch.int32, device=device)
+            if scr is None or scr.numel() < need_s.value:
+                scr = torch.empty(max(64, need_s.value), dtype=torch.uint8, device=device)
+        if not torch.cuda.is_current_stream_capturing():  # a graph owns what its capture allocates
+            _shared_workspaces[key] = (cnt, scr)
+    return cnt, scr
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def paged_shared_prefix_attention(
+    q: Tensor,
+    cache: PagedKVCache,
+    layer_idx: int,
+    tables: Sequence[SequenceBlockTable] | SharedPrefixTables,
+    out: Tensor | None = None,
+    kernel: str = "auto",
+    stream: torch.cuda.Stream | None = None,
+) -> Tensor:
+    """paged_decode_attention for a batch whose sequences share blocks: each shared block is
+    read once for all the sequences that hold it (one layer, two launches; one when nothing
+    is shared).
+
+    q: ``[batch, n_q_heads, head_dim]`` or ``[batch, n_q_heads, 1, head_dim]`` (after RoPE), in
+    the cache dtype. tables: the batch's block tables, or a SharedPrefixTables built from
+    them once per step and reused across its layers. Returns the attention output in q's
+    shape. kernel: "auto" (tensor cores for bf16 / fp16 at head_dim 64 or 128, at most 16
+    query heads per KV head, 16-byte aligned rows and blocks of 8, 16, 32, 64 or a multiple of
+    128 tokens; CUDA cores in float32 otherwise), "tcgen05" (insist on the former) or
+    "generic" (force the latter). Sums, maxima and partial results are float32 and the output
+    is rounded once, so results differ from paged_decode_attention's, which rounds scores and
+    probabilities where the reference does, within that rounding.
+    """
+    fast = tables._fast if type(tables) is SharedPrefixTables else None
+    if (fast is not None and out is None and stream is None and kernel == "auto" and fast[0] is cache
+            and q.shape == fast[1] and q.stride() == fast[2] and q.dtype is fast[3] and q.get_device() == fast[4]
+            and cache.keys.data_ptr() == fast[5] and 0 <= layer_idx < fast[6]
+            and _current_device() == fast[4]):
+        st_raw = _raw_stream(fast[4])
+        if st_raw == fast[7]:
+            res = torch.empty_like(q, memory_format=torch.contiguous_format)
+            code = fast[9](fast[8], layer_idx, q.data_ptr(), res.data_ptr(), st_raw)
+            if code != 0:
+                _lib.check(code, "augur_kv_shared_prefix_attention")
+            _ops.launch_count += fast[10]
+            return res
+    if kernel not in ("auto", "tcgen05", "generic"):
+        raise ValueError("kernel must be 'auto', 'tcgen05' or 'generic'")
+    squeeze = q.dim() == 4
+    if squeeze:
+        if q.shape[2] != 1:
+            raise ValueError("paged_shared_prefix_attention takes one query token per sequence")
+        q3 = q[:, :, 0, :]
+    elif q.dim() == 3:
+        q3 = q
+    else:
+        raise ValueError("q must be [batch, heads, head_dim] or [batch, heads, 1, head_dim]")
+    _ops.require_cuda("paged_shared_prefix_attention", q3, cache.keys, cache.values, out)
+    if not 0 <= layer_idx < cache.keys.shape[0]:
+        raise ValueError("layer_idx is outside the cache layer range")
+    L, NB, Hkv, bs, D = cache.keys.shape
+    B, Hq, Dq = q3.shape
+    if Dq != D or Hq == 0 or Hq % Hkv != 0:
+        raise ValueError("query shape does not match the cache (head_dim, or heads not a multiple of KV heads)")
+    if q3.dtype != cache.keys.dtype or cache.values.dtype != cache.keys.dtype:
+        raise ValueError("query and cache dtypes differ")
+    if cache.keys.stride() != cache.values.stride() or cache.keys.shape != cache.values.shape or cache.keys.stride(-1) != 1:
+        raise ValueError("keys and values must share one layout, head_dim contiguous")
+    device = cache.keys.device
+    if q3.device != device or cache.values.device != device:
+        raise ValueError("query and cache must be on one device")
+    plan = tables if isinstance(tables, SharedPrefixTables) else SharedPrefixTables(cache, tables, Hq, stream=stream)
+    if plan.batch != B:
+        raise ValueError("one block table per sequence is required")
+    if plan.n_q_heads != Hq or plan.block_size != bs or plan._device != device:
+        raise ValueError("the SharedPrefixTables were built for another cache or another number of query heads")
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != device or out.stride(-1) != 1):
+        raise ValueError("out must have q's shape, dtype and device, head_dim contiguous")
+    if B == 0:
+        return out if out is not None else torch.empty_like(q)
+    rows = q3 if q3.stride(-1) == 1 else q3.contiguous()
+    res = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
+    res3 = res[:, :, 0, :] if squeeze else res
+    st = stream if stream is not None else torch.cuda.current_stream(device)
+    flags = {"auto": _lib.ATTN_AUTO, "tcgen05": _lib.ATTN_TCGEN05, "generic": _lib.ATTN_GENERIC}[kernel]
+    with _ops._DeviceGuard(device):
+        a = plan._prepare(rows, res3, cache, st, flags)
+        fn = _lib.load().augur_kv_shared_prefix_attention
+        _lib.check(fn(ctypes.addressof(a), layer_idx, rows.data_ptr(), res.data_ptr(), st.cuda_stream),
+                   "augur_kv_shared_prefix_attention")
+    launches = 1 + (plan.n_items > 0)
+    _ops.launch_count += launches
+    _ops.keep_until_done(st, rows, res, *plan._dev.values(), *a._keep[:2])
+    if (rows is q3 and out is None and stream is None and kernel == "auto"
+            and not torch.cuda.is_current_stream_capturing()):
+        plan._fast = (cache, q.shape, q.stride(), q.dtype, q.get_device(), cache.keys.data_ptr(), L, st.cuda_stream,
+                      ctypes.addressof(a), fn, launches, a)
+    return res

@@ -1,0 +1,1440 @@
+// augur_shared.cu — decode attention of a batch whose sequences share blocks,
+// each shared block read once for all of its sequences.
+//
+// Every sequence has one query token, which attends to all its cached
+// positions. Softmax attention over a set of keys K splits over any partition
+// of K: with scores x_j = scale log2(e) q.k_j and, for a part, a reference m,
+//   l = sum_j 2^(x_j - m),  O = sum_j 2^(x_j - m) v_j,
+// the parts join as  M = max m_i,  out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i.
+// The plan (built on the host from the block tables) names the runs of blocks
+// that several sequences share. Two launches do the rest:
+//  * the shared launch: a work item is (run, KV head, row tile, key range); the rows
+//    are the query heads of every sequence of the run, so one pass over the
+//    run's keys serves all of them. It leaves (m, l, O) per row and range in
+//    float32 scratch ("slabs" of 128 rows).
+//  * the own launch: a CTA per (sequence, KV head, part) attends to the
+//    sequence's own blocks, then joins its rows' slabs and writes the output.
+//    It is a programmatic dependent launch: its own part runs beside the shared
+//    launch, and only the join waits for it.
+// bf16 / fp16 with head_dim 64 or 128 run on the tensor cores
+// (shared_umma_kernel, own_mma_kernel, described there); everything else on
+// CUDA cores in float32 (shared_generic_kernel, own_generic_kernel).
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+#include <string.h>
+
+#include "augur_kv.h"
+#include "common.cuh"
+
+namespace augur_kv_sh {
+
+using augur_kv_dev::record_status;
+
+constexpr float kNegInf = -INFINITY;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kSlabRows = 128;
+constexpr int kMaxGroups = 16;  // query heads per KV head on the tensor cores
+
+// One work item of the shared launch (int32 fields, as the plan stores them).
+struct Item {
+  int32_t member0;   // first of the run's sequences in `members`
+  int32_t n_rows;    // rows of the run: sequences x query heads per KV head
+  int32_t block0;    // first of the run's blocks in `run_blocks`
+  int32_t n_blocks;  // blocks of the run
+  int32_t kv_head;
+  int32_t row0;      // first row of this item (128 rows, or 256 with `pair`)
+  int32_t key0, key1;  // positions within the run (key0 a multiple of 128)
+  int32_t slab0;     // slab of rows row0 .. row0 + 127
+  int32_t slab1;     // slab of the next 128 rows, or -1
+  int32_t reserved0, reserved1;
+};
+static_assert(sizeof(Item) == 48, "12 int32 per item");
+
+struct Args {
+  const char* q;
+  int64_t q_stride_b, q_stride_h;  // bytes
+  const char* k;
+  const char* v;
+  int64_t blk_stride, head_stride, row_stride;  // bytes
+  int64_t num_blocks;
+  int32_t block_size;
+  const int32_t* tables;
+  int64_t tables_stride, max_blocks;
+  const int32_t* seq_lens;
+  const int32_t* shared_lens;  // positions of each sequence that its runs cover
+  int32_t batch, hq, hkv, groups, head_dim;
+  float scale;  // log2(e) / sqrt(head_dim)
+  char* out;
+  int64_t out_stride_b, out_stride_h;
+  const Item* items;
+  int32_t n_items;
+  const int32_t* members;
+  int32_t n_members;
+  const int32_t* run_blocks;
+  int32_t n_run_blocks;
+  const int32_t* ref_starts;  // [batch + 1] into refs
+  const int4* refs;           // first slab of the run, key ranges, sequence's place in the run, row tiles
+  int32_t n_refs, n_slabs;
+  float* slab_ml;  // [n_slabs][128][2]
+  float* slab_o;   // [n_slabs][128][head_dim]
+  int32_t n_split;     // parts of a sequence's own keys
+  float* split_ml;     // [batch * hkv][n_split][groups][2]
+  float* split_o;      // [batch * hkv][n_split][groups][head_dim]
+  int32_t* counters;   // [batch * hkv], zero between launches
+  int32_t* status;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ float ex2(float x) {  // 2^x; ex2(-inf) = 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_prerequisites() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename T> struct Elem;
+template <> struct Elem<float> {
+  static __device__ __forceinline__ float to_f(float x) { return x; }
+  static __device__ __forceinline__ float from_f(float x) { return x; }
+};
+template <> struct Elem<__half> {
+  static __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
+  static __device__ __forceinline__ __half from_f(float x) { return __float2half_rn(x); }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static constexpr uint32_t kFormat = 0;
+  static constexpr CUtensorMapDataType kTma = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+};
+template <> struct Elem<__nv_bfloat16> {
+  static __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+  static __device__ __forceinline__ __nv_bfloat16 from_f(float x) { return __float2bfloat16_rn(x); }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static constexpr uint32_t kFormat = 1;
+  static constexpr CUtensorMapDataType kTma = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+};
+
+// The item, or false (and EBOUNDS) where its fields do not fit the plan's arrays.
+__device__ __forceinline__ bool read_item(const Args& a, int i, Item& it) {
+  it = a.items[i];
+  const int seqs = (it.n_rows + a.groups - 1) / a.groups;
+  const bool ok = it.member0 >= 0 && it.n_rows > 0 && int64_t(it.member0) + seqs <= a.n_members && it.block0 >= 0 &&
+                  it.n_blocks >= 0 && int64_t(it.block0) + it.n_blocks <= a.n_run_blocks && it.kv_head >= 0 &&
+                  it.kv_head < a.hkv && it.row0 >= 0 && it.row0 < it.n_rows && it.key0 >= 0 && it.key0 < it.key1 &&
+                  int64_t(it.key1) <= int64_t(it.n_blocks) * a.block_size && (it.key0 & 127) == 0 && it.slab0 >= 0 &&
+                  it.slab0 < a.n_slabs && it.slab1 < a.n_slabs;
+  if (!ok && threadIdx.x == 0) record_status(a.status, AUGUR_KV_EBOUNDS);
+  return ok;
+}
+
+// Query row r of the item's run: the q row, or null past the run (and for a sequence outside the batch).
+__device__ __forceinline__ const char* query_row(const Args& a, const Item& it, int r) {
+  if (r >= it.n_rows) return nullptr;
+  const int i = r / a.groups, b = __ldg(a.members + it.member0 + i);
+  if (b < 0 || b >= a.batch) {
+    record_status(a.status, AUGUR_KV_EBOUNDS);
+    return nullptr;
+  }
+  return a.q + int64_t(b) * a.q_stride_b + int64_t(it.kv_head * a.groups + (r - i * a.groups)) * a.q_stride_h;
+}
+
+// Offset in bytes of position `pos` of sequence b in the pool (KV head hk), or -1 (and EBOUNDS).
+__device__ __forceinline__ int64_t own_row(const Args& a, int b, int hk, int pos) {
+  const int lb = pos / a.block_size;
+  const int blk = lb < a.max_blocks ? __ldg(a.tables + int64_t(b) * a.tables_stride + lb) : -1;
+  if (blk < 0 || blk >= a.num_blocks) {
+    record_status(a.status, AUGUR_KV_EBOUNDS);
+    return -1;
+  }
+  return int64_t(blk) * a.blk_stride + int64_t(hk) * a.head_stride + int64_t(pos - lb * a.block_size) * a.row_stride;
+}
+
+// The sequence's own positions [first, last); the runs cover [0, first).
+__device__ __forceinline__ void own_range(const Args& a, int b, int& first, int& last) {
+  last = max(0, __ldg(a.seq_lens + b));
+  first = max(0, __ldg(a.shared_lens + b));
+  if (int64_t(last) > a.max_blocks * int64_t(a.block_size) || first > last) {
+    record_status(a.status, AUGUR_KV_EBOUNDS);
+    last = int(min(int64_t(last), a.max_blocks * int64_t(a.block_size)));
+    first = min(first, last);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The join: a sequence's parts of one KV head. Source 0 .. n_local - 1 are the
+// sequence's own parts, the rest its runs' slabs in order.
+// ---------------------------------------------------------------------------
+
+// Slab row of source `s` (a slab source) for row h; false for a reference outside the plan.
+__device__ __forceinline__ bool slab_row(const Args& a, int b, int hk, int h, int s, int64_t& row) {
+  const int r0 = __ldg(a.ref_starts + b), r1 = __ldg(a.ref_starts + b + 1);
+  for (int r = r0; r < r1 && r < a.n_refs; ++r) {
+    const int4 f = __ldg(a.refs + r);  // slab base, ranges, place, tiles
+    if (s < f.y) {
+      const int at = f.z * a.groups + h, tile = at / kSlabRows;
+      const int64_t slab = int64_t(f.x) + (int64_t(hk) * f.w + tile) * f.y + s;
+      if (slab < 0 || slab >= a.n_slabs || tile >= f.w) {
+        record_status(a.status, AUGUR_KV_EBOUNDS);
+        return false;
+      }
+      row = slab * kSlabRows + (at - tile * kSlabRows);
+      return true;
+    }
+    s -= f.y;
+  }
+  return false;
+}
+__device__ __forceinline__ int slab_sources(const Args& a, int b) {
+  int n = 0;
+  const int r0 = max(0, __ldg(a.ref_starts + b)), r1 = __ldg(a.ref_starts + b + 1);
+  for (int r = r0; r < r1 && r < a.n_refs; ++r) n += max(0, __ldg(a.refs + r).y);
+  return n;
+}
+
+constexpr int kJoinChunk = 64;  // sources joined at a time
+
+// Joins row parts of `groups` rows and writes the output rows. local_ml / local_o: the
+// n_local own parts, [part][local_rows][2] and [part][local_rows][o_stride] (shared or global
+// memory, stride in floats). smem: groups * (kJoinChunk * 3 + 3) floats. All threads of the CTA call it.
+template <typename T>
+__device__ void join_rows(const Args& a, int b, int hk, int n_local, const float* local_ml, const float* local_o,
+                          int local_rows, int o_stride, float* smem) {
+  const int G = a.groups, D = a.head_dim, n_thr = blockDim.x, tid = threadIdx.x;
+  const int n_src = n_local + slab_sources(a, b);
+  float* fac = smem;                                                 // [G][kJoinChunk]
+  int64_t* rows = reinterpret_cast<int64_t*>(fac + G * kJoinChunk);  // [G][kJoinChunk]
+  float* run_m = reinterpret_cast<float*>(rows + G * kJoinChunk);    // [G] running reference
+  float* run_l = run_m + G;                                          // [G]
+  float* run_s = run_l + G;                                          // [G] scale of what is joined so far
+  for (int h = tid; h < G; h += n_thr) {
+    run_m[h] = kNegInf;
+    run_l[h] = 0.f;
+  }
+  constexpr int kMaxVal = 32;  // output values a thread holds: groups * head_dim <= 32 * threads
+  float acc[kMaxVal];
+#pragma unroll
+  for (int i = 0; i < kMaxVal; ++i) acc[i] = 0.f;
+  for (int s0 = 0; s0 < n_src; s0 += kJoinChunk) {
+    const int ns = min(kJoinChunk, n_src - s0);
+    __syncthreads();
+    for (int i = tid; i < G * ns; i += n_thr) {
+      const int h = i / ns, s = i - h * ns;
+      float m = kNegInf;
+      int64_t row = -1;
+      if (s0 + s < n_local) {
+        row = int64_t(s0 + s) * local_rows + h;
+        m = local_ml[row * 2];
+      } else if (slab_row(a, b, hk, h, s0 + s - n_local, row)) {
+        m = a.slab_ml[row * 2];
+      }
+      fac[h * kJoinChunk + s] = m;
+      rows[h * kJoinChunk + s] = row;
+    }
+    __syncthreads();
+    for (int h = tid; h < G; h += n_thr) {
+      float m = run_m[h];
+      for (int s = 0; s < ns; ++s) m = fmaxf(m, fac[h * kJoinChunk + s]);
+      run_s[h] = m == kNegInf ? 0.f : ex2(run_m[h] - m);
+      run_m[h] = m;
+      float l = run_l[h] * run_s[h];
+      for (int s = 0; s < ns; ++s) {
+        const int64_t row = rows[h * kJoinChunk + s];
+        const float f = (m == kNegInf || row < 0) ? 0.f : ex2(fac[h * kJoinChunk + s] - m);
+        if (f != 0.f) l += f * (s0 + s < n_local ? local_ml[row * 2 + 1] : a.slab_ml[row * 2 + 1]);
+        fac[h * kJoinChunk + s] = f;
+      }
+      run_l[h] = l;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kMaxVal; ++j) {
+      const int i = tid + j * n_thr;
+      if (i >= G * D) break;
+      const int h = i / D, d = i - h * D;
+      float x = 0.f;
+#pragma unroll 4
+      for (int s = 0; s < ns; ++s) {
+        const float f = fac[h * kJoinChunk + s];
+        const int64_t row = rows[h * kJoinChunk + s];
+        // a part with factor 0 (empty, or far below the maximum) is not read
+        if (f != 0.f) x = fmaf(f, s0 + s < n_local ? local_o[row * o_stride + d] : a.slab_o[row * D + d], x);
+      }
+      acc[j] = acc[j] * run_s[h] + x;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kMaxVal; ++j) {
+    const int i = tid + j * n_thr;
+    if (i >= G * D) break;
+    const int h = i / D, d = i - h * D;
+    const float x = acc[j];
+    const float l = n_src > 0 ? run_l[h] : 0.f;
+    // no key at all (an empty sequence): zero
+    reinterpret_cast<T*>(a.out + int64_t(b) * a.out_stride_b + int64_t(hk * G + h) * a.out_stride_h)[d] =
+        Elem<T>::from_f(l > 0.f ? x / l : 0.f);
+  }
+}
+__host__ __device__ constexpr int join_bytes(int groups) { return groups * (kJoinChunk * 12 + 12); }
+
+// ---------------------------------------------------------------------------
+// CUDA cores: any type and shape, float32 throughout
+// ---------------------------------------------------------------------------
+
+constexpr int kGRows = 64;   // rows at a time: four threads each
+constexpr int kGKeys = 32;   // keys at a time
+constexpr int kGThreads = kGRows * 4;
+constexpr int kGMaxDim = 256;
+
+// Shared memory of the generic kernels, in floats: q [64][pitch], k and v [32][pitch], p [64][33].
+__host__ __device__ constexpr int generic_pitch(int D) { return ((D + 3) & ~3) + 4; }
+__host__ __device__ constexpr int generic_floats(int D) {
+  return (kGRows + 2 * kGKeys) * generic_pitch(D) + kGRows * (kGKeys + 1);
+}
+
+// Attention of up to 64 rows (already in sq) over n keys; key_off(j) is key j's byte offset in the
+// pool (-1: skipped). Thread tid works for row tid / 4 and dims 4 (4 i + tid % 4) ..: leaves m, l and o.
+template <typename T, typename F>
+__device__ __forceinline__ void generic_attend(const Args& a, float* sq, int n, F key_off, float& m, float& l,
+                                               float (&o)[kGMaxDim / 4]) {
+  const int D = a.head_dim, P = generic_pitch(D), tid = threadIdx.x, r = tid >> 2, part = tid & 3;
+  float* sk = sq + kGRows * P;
+  float* sv = sk + kGKeys * P;
+  float* sp = sv + kGKeys * P;
+  m = kNegInf;
+  l = 0.f;
+#pragma unroll
+  for (int i = 0; i < kGMaxDim / 4; ++i) o[i] = 0.f;
+  for (int k0 = 0; k0 < n; k0 += kGKeys) {
+    __syncthreads();
+    for (int i = tid >> 5; i < kGKeys; i += kGThreads / 32) {  // a warp per key
+      const int64_t off = k0 + i < n ? key_off(k0 + i) : -1;
+      for (int d = tid & 31; d < D; d += 32) {
+        sk[i * P + d] = off >= 0 ? Elem<T>::to_f(reinterpret_cast<const T*>(a.k + off)[d]) : 0.f;
+        sv[i * P + d] = off >= 0 ? Elem<T>::to_f(reinterpret_cast<const T*>(a.v + off)[d]) : 0.f;
+      }
+      if ((tid & 31) == 0) sp[i * (kGKeys + 1) + kGKeys] = off >= 0 ? 0.f : kNegInf;  // the mask, beside p
+    }
+    __syncthreads();
+    float s[kGKeys / 4];
+#pragma unroll
+    for (int j = 0; j < kGKeys / 4; ++j) s[j] = 0.f;
+    if ((D & 3) == 0) {
+      for (int d = 0; d < D; d += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(sq + r * P + d);
+#pragma unroll
+        for (int j = 0; j < kGKeys / 4; ++j) {
+          const float4 y = *reinterpret_cast<const float4*>(sk + (j * 4 + part) * P + d);
+          s[j] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, s[j]))));
+        }
+      }
+    } else {
+      for (int d = 0; d < D; ++d) {
+        const float x = sq[r * P + d];
+#pragma unroll
+        for (int j = 0; j < kGKeys / 4; ++j) s[j] = fmaf(x, sk[(j * 4 + part) * P + d], s[j]);
+      }
+    }
+    float mx = kNegInf;
+#pragma unroll
+    for (int j = 0; j < kGKeys / 4; ++j) {
+      s[j] = s[j] * a.scale + sp[(j * 4 + part) * (kGKeys + 1) + kGKeys];
+      mx = fmaxf(mx, s[j]);
+    }
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    const float mn = fmaxf(m, mx);
+    const float alpha = mn == kNegInf ? 1.f : ex2(m - mn);
+    m = mn;
+    l *= alpha;
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < kGKeys / 4; ++j) {
+      const float p = mn == kNegInf ? 0.f : ex2(s[j] - mn);
+      l += p;
+      sp[r * (kGKeys + 1) + j * 4 + part] = p;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kGMaxDim / 4; ++i) o[i] *= alpha;
+    for (int j = 0; j < kGKeys; ++j) {
+      const float p = sp[r * (kGKeys + 1) + j];
+#pragma unroll
+      for (int i = 0; i < kGMaxDim / 16; ++i) {
+        const int d = 16 * i + 4 * part;
+        if (d < D) {  // of the last four, those past D lie in the row's padding and are not stored
+          const float4 y = *reinterpret_cast<const float4*>(sv + j * P + d);
+          o[4 * i] = fmaf(p, y.x, o[4 * i]);
+          o[4 * i + 1] = fmaf(p, y.y, o[4 * i + 1]);
+          o[4 * i + 2] = fmaf(p, y.z, o[4 * i + 2]);
+          o[4 * i + 3] = fmaf(p, y.w, o[4 * i + 3]);
+        }
+      }
+    }
+  }
+  l += __shfl_xor_sync(0xffffffffu, l, 1);
+  l += __shfl_xor_sync(0xffffffffu, l, 2);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kGThreads) shared_generic_kernel(Args a) {
+  extern __shared__ __align__(16) float gsm[];
+  launch_dependents();
+  Item it;
+  if (!read_item(a, blockIdx.x, it)) return;
+  const int D = a.head_dim, P = generic_pitch(D), tid = threadIdx.x, r = tid >> 2, part = tid & 3;
+  const int rows = min(it.slab1 >= 0 ? 2 * kSlabRows : kSlabRows, it.n_rows - it.row0);
+  for (int r0 = 0; r0 < rows; r0 += kGRows) {
+    __syncthreads();
+    for (int i = tid >> 5; i < kGRows; i += kGThreads / 32) {
+      const char* src = r0 + i < rows ? query_row(a, it, it.row0 + r0 + i) : nullptr;
+      for (int d = tid & 31; d < D; d += 32)
+        gsm[i * P + d] = src != nullptr ? Elem<T>::to_f(reinterpret_cast<const T*>(src)[d]) : 0.f;
+    }
+    auto key_off = [&](int j) -> int64_t {
+      const int pos = it.key0 + j, lb = pos / a.block_size;
+      const int blk = __ldg(a.run_blocks + it.block0 + lb);
+      if (blk < 0 || blk >= a.num_blocks) {
+        record_status(a.status, AUGUR_KV_EBOUNDS);
+        return -1;
+      }
+      return int64_t(blk) * a.blk_stride + int64_t(it.kv_head) * a.head_stride +
+             int64_t(pos - lb * a.block_size) * a.row_stride;
+    };
+    float m, l, o[kGMaxDim / 4];
+    generic_attend<T>(a, gsm, it.key1 - it.key0, key_off, m, l, o);
+    const int row = r0 + r;
+    if (row < rows) {
+      const int64_t at = int64_t(row < kSlabRows ? it.slab0 : it.slab1) * kSlabRows + (row & (kSlabRows - 1));
+      if (part == 0) *reinterpret_cast<float2*>(a.slab_ml + at * 2) = make_float2(m, l);
+#pragma unroll
+      for (int i = 0; i < kGMaxDim / 16; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (16 * i + 4 * part + c < D) a.slab_o[at * D + 16 * i + 4 * part + c] = o[4 * i + c];
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kGThreads) own_generic_kernel(Args a) {
+  extern __shared__ __align__(16) float gsm[];
+  const int b = blockIdx.x / a.hkv, hk = blockIdx.x - b * a.hkv;
+  const int D = a.head_dim, P = generic_pitch(D), tid = threadIdx.x, r = tid >> 2, part = tid & 3;
+  int first, last;
+  own_range(a, b, first, last);
+  for (int i = tid >> 5; i < kGRows; i += kGThreads / 32) {
+    const char* src = a.q + int64_t(b) * a.q_stride_b + int64_t(hk * a.groups + i) * a.q_stride_h;
+    for (int d = tid & 31; d < D; d += 32)
+      gsm[i * P + d] = i < a.groups ? Elem<T>::to_f(reinterpret_cast<const T*>(src)[d]) : 0.f;
+  }
+  float m, l, o[kGMaxDim / 4];
+  generic_attend<T>(a, gsm, last - first, [&](int j) { return own_row(a, b, hk, first + j); }, m, l, o);
+  __syncthreads();
+  float* ml = gsm + generic_floats(D);  // [64][2]; the queries' place takes the output rows
+  if (r < a.groups) {
+    if (part == 0) {
+      ml[2 * r] = m;
+      ml[2 * r + 1] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < kGMaxDim / 16; ++i)
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (16 * i + 4 * part + c < D) gsm[r * P + 16 * i + 4 * part + c] = o[4 * i + c];
+  }
+  wait_prerequisites();  // the shared launch's slabs
+  join_rows<T>(a, b, hk, 1, ml, gsm, kGRows, P, ml + 2 * kGRows);
+}
+
+// ---------------------------------------------------------------------------
+// Tensor cores: a sequence's own keys (mma.sync)
+// ---------------------------------------------------------------------------
+//
+// A CTA per (sequence, KV head, part). With one query token the products are
+// a few rows wide, so they run transposed: S^T = K Q^T and O^T = V^T P^T put the
+// tokens (and dims) on the 16 mma rows and the query heads of the group on
+// the 8 columns. Each of four warps stages 32 tokens of K and V at a time
+// (cp.async, two buffers) and keeps its own running softmax; the CTA joins
+// the warps, the run's slabs and (for long own parts) the other CTAs' parts,
+// whose last arrival writes the output (it joins them in their order, so the
+// result does not depend on the order of arrival). Bound by HBM: K and V rows are read once.
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(p));
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t (&r)[4], uint32_t p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(p));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+constexpr int kOwnWarps = 4;
+constexpr int kOwnThreads = kOwnWarps * 32;
+constexpr int kOwnTok = 32;  // tokens of a warp's stage
+
+template <int D>
+struct OwnCfg {
+  static constexpr int kRow = D * 2 + 16;  // padded: ldmatrix rows hit distinct banks
+  static constexpr int kTile = kOwnTok * kRow;
+  static constexpr int kBufs = 2;
+  static constexpr int kPipe = kOwnWarps * kBufs * 2 * kTile;
+};
+// warps' parts [4][heads][2] and [4][heads][D] over the stages, then the join's memory
+__host__ __device__ constexpr int own_parts_bytes(int D, int heads) { return kOwnWarps * heads * (D + 2) * 4; }
+
+template <typename T, int D, int NG>
+__global__ void __launch_bounds__(kOwnThreads) own_mma_kernel(Args a) {
+  using CF = OwnCfg<D>;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ int last_flag;
+  constexpr int H = NG * 8;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int unit = blockIdx.x / a.n_split, part = blockIdx.x - unit * a.n_split;
+  const int b = unit / a.hkv, hk = unit - b * a.hkv;
+  int first, last;
+  own_range(a, b, first, last);
+  {
+    const int stages = (last - first + kOwnTok - 1) / kOwnTok;
+    const int cut = (stages + a.n_split - 1) / a.n_split * kOwnTok;
+    first = min(last, first + part * cut);
+    last = min(last, first + cut);
+  }
+  const int n_st = (last - first + kOwnTok - 1) / kOwnTok;
+  unsigned char* mine = smem + warp * CF::kBufs * 2 * CF::kTile;
+  const uint32_t mine_s = smem_u32(mine);
+
+  constexpr int CH = D / 8;  // 16-byte pieces of a row
+  auto load_stage = [&](int st, int buf) {
+    const int pos = first + st * kOwnTok + lane;
+    const int64_t off = pos < last ? own_row(a, b, hk, pos) : -1;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int row = i * (32 / CH) + lane / CH, c = lane % CH;
+      const int64_t o = __shfl_sync(0xffffffffu, off, row);
+      const uint32_t dst = mine_s + buf * 2 * CF::kTile + row * CF::kRow + c * 16;
+      cp_async16(dst, a.k + (o >= 0 ? o + c * 16 : 0), o >= 0 ? 16 : 0);
+      cp_async16(dst + CF::kTile, a.v + (o >= 0 ? o + c * 16 : 0), o >= 0 ? 16 : 0);
+    }
+  };
+  if (warp < n_st) load_stage(warp, 0);
+  asm volatile("cp.async.commit_group;" ::: "memory");
+
+  uint32_t qb[NG][D / 16][2];
+#pragma unroll
+  for (int n = 0; n < NG; ++n) {
+    const int h = n * 8 + g;
+    const char* qr = a.q + int64_t(b) * a.q_stride_b + int64_t(hk * a.groups + h) * a.q_stride_h;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      qb[n][ks][0] = h < a.groups ? *reinterpret_cast<const uint32_t*>(qr + (ks * 16 + 2 * t) * 2) : 0u;
+      qb[n][ks][1] = h < a.groups ? *reinterpret_cast<const uint32_t*>(qr + (ks * 16 + 8 + 2 * t) * 2) : 0u;
+    }
+  }
+  float o[NG][D / 16][4];
+  float mr[NG][2], lr[NG][2];
+#pragma unroll
+  for (int n = 0; n < NG; ++n) {
+    mr[n][0] = mr[n][1] = kNegInf;
+    lr[n][0] = lr[n][1] = 0.f;
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) o[n][d][0] = o[n][d][1] = o[n][d][2] = o[n][d][3] = 0.f;
+  }
+  int buf = 0;
+  for (int st = warp; st < n_st; st += kOwnWarps, buf ^= 1) {
+    if (st + kOwnWarps < n_st) load_stage(st + kOwnWarps, buf ^ 1);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncwarp();
+    const uint32_t ks_ = mine_s + buf * 2 * CF::kTile, vs_ = ks_ + CF::kTile;
+    float s[2][NG][4];
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+      for (int n = 0; n < NG; ++n) s[mt][n][0] = s[mt][n][1] = s[mt][n][2] = s[mt][n][3] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        uint32_t ka[4];
+        ldsm_x4(ka, ks_ + (mt * 16 + (lane & 15)) * CF::kRow + (ks * 16 + (lane >> 4) * 8) * 2);
+#pragma unroll
+        for (int n = 0; n < NG; ++n) Elem<T>::mma(s[mt][n], ka, qb[n][ks][0], qb[n][ks][1]);
+      }
+    }
+    const int left = last - first - st * kOwnTok;  // tokens of this stage
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      float mx[2] = {kNegInf, kNegInf};
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int tok = mt * 16 + g + (i >> 1) * 8;
+          const float x = tok < left ? s[mt][n][i] * a.scale : kNegInf;
+          s[mt][n][i] = x;
+          mx[i & 1] = fmaxf(mx[i & 1], x);
+        }
+      }
+      float alpha[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 4));
+        mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 8));
+        mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], 16));
+        const float mn = fmaxf(mr[n][c], mx[c]);
+        alpha[c] = mn == kNegInf ? 1.f : ex2(mr[n][c] - mn);
+        mr[n][c] = mn;
+        lr[n][c] *= alpha[c];
+      }
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        o[n][d][0] *= alpha[0];
+        o[n][d][1] *= alpha[1];
+        o[n][d][2] *= alpha[0];
+        o[n][d][3] *= alpha[1];
+      }
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float mn = mr[n][i & 1];
+          const float p = mn == kNegInf ? 0.f : ex2(s[mt][n][i] - mn);
+          lr[n][i & 1] += p;  // the sum takes the unrounded value; P V takes it rounded to the cache type
+          s[mt][n][i] = p;
+        }
+    }
+    uint32_t pb[2][NG][2];
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+      for (int n = 0; n < NG; ++n) {
+        pb[mt][n][0] = transpose8(Elem<T>::pack(s[mt][n][0], s[mt][n][1]));
+        pb[mt][n][1] = transpose8(Elem<T>::pack(s[mt][n][2], s[mt][n][3]));
+      }
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        uint32_t va[4];
+        const int mat = lane >> 3;
+        ldsm_x4_t(va, vs_ + (mt * 16 + (mat >> 1) * 8 + (lane & 7)) * CF::kRow + (d * 16 + (mat & 1) * 8) * 2);
+#pragma unroll
+        for (int n = 0; n < NG; ++n) Elem<T>::mma(o[n][d], va, pb[mt][n][0], pb[mt][n][1]);
+      }
+    }
+    __syncwarp();  // every lane is done with this buffer before it is filled again
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  float* part_ml = reinterpret_cast<float*>(smem);  // [4][H][2]
+  float* part_o = part_ml + kOwnWarps * H * 2;      // [4][H][D]
+#pragma unroll
+  for (int n = 0; n < NG; ++n) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float l = lr[n][c];
+      l += __shfl_xor_sync(0xffffffffu, l, 4);
+      l += __shfl_xor_sync(0xffffffffu, l, 8);
+      l += __shfl_xor_sync(0xffffffffu, l, 16);
+      const int h = n * 8 + 2 * t + c;
+      if (g == 0) {
+        part_ml[(warp * H + h) * 2] = mr[n][c];
+        part_ml[(warp * H + h) * 2 + 1] = l;
+      }
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        part_o[(warp * H + h) * D + d * 16 + g] = o[n][d][c];
+        part_o[(warp * H + h) * D + d * 16 + g + 8] = o[n][d][c + 2];
+      }
+    }
+  }
+  float* join_mem = part_o + kOwnWarps * H * D;
+  __syncthreads();
+  if (a.n_split == 1) {
+    wait_prerequisites();  // the shared launch's slabs
+    join_rows<T>(a, b, hk, kOwnWarps, part_ml, part_o, H, D, join_mem);
+    return;
+  }
+  // this CTA's part to scratch; the last CTA of the unit to arrive joins them all
+  const int64_t base = (int64_t(unit) * a.n_split + part) * a.groups;
+  for (int i = threadIdx.x; i < a.groups * D; i += kOwnThreads) {
+    const int h = i / D, d = i - h * D;
+    float m = kNegInf, l = 0.f, x = 0.f;
+#pragma unroll
+    for (int w = 0; w < kOwnWarps; ++w) m = fmaxf(m, part_ml[(w * H + h) * 2]);
+#pragma unroll
+    for (int w = 0; w < kOwnWarps; ++w) {
+      const float f = m == kNegInf ? 0.f : ex2(part_ml[(w * H + h) * 2] - m);
+      l += f * part_ml[(w * H + h) * 2 + 1];
+      x += f * part_o[(w * H + h) * D + d];
+    }
+    a.split_o[(base + h) * D + d] = x;
+    if (d == 0) *reinterpret_cast<float2*>(a.split_ml + (base + h) * 2) = make_float2(m, l);
+  }
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const int seen = atomicAdd(a.counters + unit, 1);
+    last_flag = seen == a.n_split - 1;
+    if (last_flag) a.counters[unit] = 0;
+    __threadfence();
+  }
+  __syncthreads();
+  if (!last_flag) return;
+  wait_prerequisites();
+  const int64_t unit0 = int64_t(unit) * a.n_split * a.groups;
+  join_rows<T>(a, b, hk, a.n_split, a.split_ml + unit0 * 2, a.split_o + unit0 * D, a.groups, D, join_mem);
+}
+
+// ---------------------------------------------------------------------------
+// Tensor cores: the shared runs (tcgen05, accumulators in tensor memory)
+// ---------------------------------------------------------------------------
+//
+// One CTA per item: ten warps. Two groups of four warps each own a tile of
+// 128 query rows, one row a thread; warp 8 fetches K and V tiles of 128 keys
+// (TMA, one box per block and 64 dims, 128-byte swizzle; keys past the range
+// and bad block ids take an out-of-range block coordinate, which TMA fills
+// with zeros), warp 9 issues the products. Per tile: S = Q K^T into tensor
+// memory (M = N = 128), each thread loads its row of S, takes the running
+// maximum, writes P = 2^(x - m) in the cache type over S, and O += P V takes
+// P as the operand in tensor memory and accumulates there. O is rescaled only
+// when a row's maximum has grown by more than 2^8 over the reference its
+// exponents use (P then stays below 2^8, and the float32 sums do not care),
+// so most tiles touch it not at all. The groups work on the same keys with
+// different rows (`pair`: a run with over 128 rows reads its keys once for
+// 256), or on the same rows with even and odd key tiles, whose results are
+// joined in shared memory. While one group's softmax runs, the tensor core
+// works for the other.
+//
+// Bound by the 16 exponentials a clock an SM has: a 256 x 128 tile needs 2,048
+// clocks of them, its products 1,024 (head_dim 64) or 2,048 (128). With few
+// rows it is bound by HBM instead.
+//
+// Every wait is bounded (2 s of %globaltimer); on expiry the CTA records
+// AUGUR_KV_ETIMEOUT, drains its copies and products, frees its tensor memory and returns.
+
+constexpr int kShThreads = 320;
+constexpr int kTileKeys = 128;
+
+template <int D>
+struct ShCfg {
+  static constexpr int kHalves = D / 64;
+  static constexpr int kTileBytes = kTileKeys * D * 2;  // K, V or Q tile: [half][128 rows][128 bytes], swizzled
+  static constexpr int kKBufs = D == 128 ? 2 : 4;
+  static constexpr int kVBufs = D == 128 ? 3 : 5;
+  static constexpr int kQ = 0;
+  static constexpr int kK = kQ + 2 * kTileBytes;
+  static constexpr int kV = kK + kKBufs * kTileBytes;
+  static constexpr int kBar = kV + kVBufs * kTileBytes;
+  static constexpr int kBytes = kBar + 256 + 1024;  // and the alignment of the first tile
+  static constexpr uint32_t kS = 0, kO = 256, kCols = 512;  // tensor memory: S0, S1 (P over them), O0, O1
+};
+
+__device__ __forceinline__ uint64_t global_ns() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+  return t;
+}
+__device__ __forceinline__ void mbar_init(uint32_t bar, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred P1;\n\tmbarrier.try_wait.parity.shared::cta.b64 P1, [%1], %2;\n\t"
+      "selp.b32 %0, 1, 0, P1;\n\t}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Wait for the phase with this parity to complete; false after 2 s or once another role gave up.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
+  if (mbar_try(bar, parity)) return true;
+  const uint64_t t0 = global_ns();
+  while (!mbar_try(bar, parity)) {
+    if (*gave_up || global_ns() - t0 > 2000000000ull) {
+      *gave_up = 1;
+      return false;
+    }
+  }
+  return true;
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int row, int head,
+                                        int block) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::
+          "r"(dst),
+      "l"(map), "r"(bar), "r"(x), "r"(row), "r"(head), "r"(block)
+      : "memory");
+}
+// Shared-memory matrix descriptor, 128-byte swizzle: start address, the
+// leading offset (between 64-element columns of an MN-major operand; unused
+// K-major), the stride between groups of 8 rows (1,024 bytes), version 1.
+__device__ __forceinline__ uint64_t sw128_desc(uint32_t addr, uint32_t lead) {
+  return uint64_t((addr & 0x3FFFFu) >> 4) | (uint64_t(lead >> 4) << 16) | (uint64_t(1024 >> 4) << 32) |
+         (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
+// Instruction descriptor for kind::f16: float32 accumulator, A and B of one type, A K-major, M = 128.
+template <typename T>
+__device__ constexpr uint32_t mma_desc(int n, bool b_mn_major) {
+  return (1u << 4) | (Elem<T>::kFormat << 7) | (Elem<T>::kFormat << 10) | (uint32_t(b_mn_major) << 16) |
+         (uint32_t(n >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(acc))
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(acc))
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// 32 consecutive columns of this thread's tensor-memory lane; the values are there after tmem_wait_ld
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kShThreads, 1)
+    shared_umma_kernel(const __grid_constant__ Args a, const __grid_constant__ CUtensorMap k_map,
+                       const __grid_constant__ CUtensorMap v_map) {
+  using CF = ShCfg<D>;
+  extern __shared__ unsigned char smem_raw[];
+  // the swizzle pattern follows address bits: tiles start on 1,024 bytes
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int gave_up;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  launch_dependents();
+  Item it;
+  if (!read_item(a, blockIdx.x, it)) return;
+  const bool pair = it.slab1 >= 0;
+  const int n_keys = it.key1 - it.key0, n_tiles = (n_keys + kTileKeys - 1) / kTileKeys;
+  const uint32_t sb = smem_u32(smem), bars = sb + CF::kBar;
+  auto k_full = [&](int i) { return bars + 8u * uint32_t(i); };
+  auto k_empty = [&](int i) { return bars + 8u * uint32_t(CF::kKBufs + i); };
+  auto v_full = [&](int i) { return bars + 8u * uint32_t(2 * CF::kKBufs + i); };
+  auto v_empty = [&](int i) { return bars + 8u * uint32_t(2 * CF::kKBufs + CF::kVBufs + i); };
+  const uint32_t rest = bars + 8u * uint32_t(2 * CF::kKBufs + 2 * CF::kVBufs);
+  auto s_full = [&](int i) { return rest + 8u * uint32_t(i); };
+  auto p_full = [&](int i) { return rest + 16u + 8u * uint32_t(i); };
+  auto o_done = [&](int i) { return rest + 32u + 8u * uint32_t(i); };
+  const uint32_t drain = rest + 48u;
+  static_assert(8 * (2 * CF::kKBufs + 2 * CF::kVBufs + 7) <= 256, "barriers");
+
+  if (tid == 0) {
+    for (int i = 0; i < CF::kKBufs; ++i) {
+      mbar_init(k_full(i), 1);
+      mbar_init(k_empty(i), 1);
+    }
+    for (int i = 0; i < CF::kVBufs; ++i) {
+      mbar_init(v_full(i), 1);
+      mbar_init(v_empty(i), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full(i), 1);
+      mbar_init(p_full(i), 128);
+      mbar_init(o_done(i), 1);
+    }
+    mbar_init(drain, 1);
+    gave_up = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
+                 "r"(CF::kCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (warp < 8) {  // the query rows, K-major with the 128-byte swizzle; rows past the run are zero
+    constexpr int CH = D / 8;
+    const int n_q = pair ? 256 : 128;
+    for (int p = tid; p < n_q * CH; p += 256) {
+      const int r = p / CH, c = p - r * CH;
+      const char* src = query_row(a, it, it.row0 + r);
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (src != nullptr) x = *reinterpret_cast<const uint4*>(src + c * 16);
+      const int rr = r & 127;
+      *reinterpret_cast<uint4*>(smem + CF::kQ + (r >> 7) * CF::kTileBytes + (c >> 3) * (kTileKeys * 128) + rr * 128 +
+                                (((c & 7) ^ (rr & 7)) << 4)) = x;
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = tmem_slot;
+
+  if (warp == 8) {
+    // ---- K and V tiles
+    const int bs = a.block_size;
+    const int box = bs < kTileKeys ? bs : kTileKeys;     // rows of a TMA box
+    const int boxes = kTileKeys / box * CF::kHalves;     // boxes of a K or V tile
+    int n_k = 0, n_v = 0;
+    bool ok = true;
+    for (int t = 0; t < n_tiles && ok; ++t) {
+      // this lane's boxes: lane, lane + 32 (128 keys of 8-token blocks at head_dim 128 make 32)
+      const int j = lane / CF::kHalves, half = lane - j * CF::kHalves;
+      const int pos = it.key0 + t * kTileKeys + j * box;
+      int blk = -1, row = 0;
+      if (lane < boxes && pos < it.key1) {
+        const int lb = pos / bs;
+        row = pos - lb * bs;
+        blk = __ldg(a.run_blocks + it.block0 + lb);
+        if (blk < 0 || blk >= a.num_blocks) {
+          record_status(a.status, AUGUR_KV_EBOUNDS);
+          blk = -1;
+        }
+      }
+      const int at = blk >= 0 ? blk : int(a.num_blocks);  // past the pool: zeros
+      const uint32_t off = uint32_t(half) * (kTileKeys * 128) + uint32_t(j) * uint32_t(box) * 128u;
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        const int bufs = kv ? CF::kVBufs : CF::kKBufs, buf = t % bufs, use = t / bufs;
+        const uint32_t full = kv ? v_full(buf) : k_full(buf), empty = kv ? v_empty(buf) : k_empty(buf);
+        if (use > 0) ok = mbar_wait(empty, uint32_t(use - 1) & 1u, &gave_up);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) mbar_expect(full, CF::kTileBytes);
+        __syncwarp();
+        if (lane < boxes)
+          tma_box(sb + (kv ? CF::kV : CF::kK) + uint32_t(buf) * CF::kTileBytes + off, kv ? &v_map : &k_map, full,
+                  half * 64, row, it.kv_head, at);
+        if (kv) n_v = t + 1;
+        else n_k = t + 1;
+      }
+    }
+    if (!ok) {  // no copy may be in flight when the CTA ends
+      volatile int ignore = 0;
+      for (int i = max(0, n_k - CF::kKBufs); i < n_k; ++i)
+        mbar_wait(k_full(i % CF::kKBufs), uint32_t(i / CF::kKBufs) & 1u, &ignore);
+      for (int i = max(0, n_v - CF::kVBufs); i < n_v; ++i)
+        mbar_wait(v_full(i % CF::kVBufs), uint32_t(i / CF::kVBufs) & 1u, &ignore);
+    }
+  } else if (warp == 9) {
+    // ---- the products: one thread issues. Group i's tiles are i, i + 2, .. (pair: all of them)
+    if (lane == 0) {
+      constexpr uint32_t idesc_s = mma_desc<T>(kTileKeys, false), idesc_o = mma_desc<T>(D, true);
+      const int step = pair ? 1 : 2;
+      auto issue_s = [&](int i, int t) {
+        const uint32_t q = sb + CF::kQ + (pair ? uint32_t(i) * CF::kTileBytes : 0u);
+        const uint32_t k = sb + CF::kK + uint32_t(t % CF::kKBufs) * CF::kTileBytes;
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) {
+          const uint32_t o = uint32_t(s >> 2) * (kTileKeys * 128) + uint32_t(s & 3) * 32u;
+          mma_ss(tmem + CF::kS + uint32_t(i) * 128u, sw128_desc(q + o, 16), sw128_desc(k + o, 16), idesc_s, s > 0);
+        }
+        mma_commit(s_full(i));
+        if (!pair || i == 1) mma_commit(k_empty(t % CF::kKBufs));
+      };
+      auto issue_o = [&](int i, int t, bool acc) {
+        const uint32_t v = sb + CF::kV + uint32_t(t % CF::kVBufs) * CF::kTileBytes;
+        const uint32_t p = tmem + CF::kS + uint32_t(i) * 128u;
+#pragma unroll
+        for (int s = 0; s < kTileKeys / 16; ++s)
+          mma_ts(tmem + CF::kO + uint32_t(i) * 128u, p + uint32_t(s) * 8u,
+                 sw128_desc(v + uint32_t(s) * 2048u, kTileKeys * 128), idesc_o, acc || s > 0);
+        mma_commit(o_done(i));
+        if (!pair || i == 1) mma_commit(v_empty(t % CF::kVBufs));
+      };
+      auto wait_k = [&](int t) { return mbar_wait(k_full(t % CF::kKBufs), uint32_t(t / CF::kKBufs) & 1u, &gave_up); };
+      auto wait_v = [&](int t) { return mbar_wait(v_full(t % CF::kVBufs), uint32_t(t / CF::kVBufs) & 1u, &gave_up); };
+      bool ok = true;
+      for (int i = 0; i < 2 && ok; ++i) {
+        const int t = pair ? 0 : i;
+        if (t >= n_tiles) break;
+        if (i == 0 || !pair) ok = wait_k(t);
+        if (ok) {
+          tc_after();
+          issue_s(i, t);
+        }
+      }
+      for (int u = 0; ok; ++u) {
+        bool any = false;
+        for (int i = 0; i < 2 && ok; ++i) {
+          const int t = pair ? u : 2 * u + i;
+          if (t >= n_tiles) break;
+          any = true;
+          const int next = t + step;
+          if (i == 0 || !pair) {
+            ok = wait_v(t);
+            if (ok && next < n_tiles) ok = wait_k(next);
+          }
+          if (ok) ok = mbar_wait(p_full(i), uint32_t(u) & 1u, &gave_up);
+          if (!ok) break;
+          tc_after();
+          issue_o(i, t, u > 0);
+          if (next < n_tiles) issue_s(i, next);  // in order behind the product that reads P from there
+        }
+        if (!any) break;
+      }
+      if (!ok) {  // no product may be in flight when tensor memory is freed
+        volatile int ignore = 0;
+        mma_commit(drain);
+        mbar_wait(drain, 0, &ignore);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---- softmax: group i, one row a thread
+    const int i = warp >> 2, r = tid & 127;
+    const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + CF::kS + uint32_t(i) * 128u + lanes, t_o = tmem + CF::kO + uint32_t(i) * 128u + lanes;
+    const int n_mine = pair ? n_tiles : (n_tiles - i + 1) / 2;
+    float m = kNegInf, l = 0.f;
+    bool ok = true;
+    for (int u = 0; u < n_mine && ok; ++u) {
+      const int t = pair ? u : 2 * u + i;
+      ok = mbar_wait(s_full(i), uint32_t(u) & 1u, &gave_up);
+      if (!__all_sync(0xffffffffu, ok)) {
+        ok = false;
+        break;
+      }
+      tc_after();
+      uint32_t s[128];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, s + c * 32);
+      tmem_wait_ld();
+      const int left = n_keys - t * kTileKeys;
+      if (left < kTileKeys) {
+#pragma unroll
+        for (int j = 0; j < 128; ++j)
+          if (j >= left) s[j] = 0xff800000u;  // -inf
+      }
+      float mx0 = kNegInf, mx1 = kNegInf;
+#pragma unroll
+      for (int j = 0; j < 128; j += 2) {
+        mx0 = fmaxf(mx0, __uint_as_float(s[j]));
+        mx1 = fmaxf(mx1, __uint_as_float(s[j + 1]));
+      }
+      const float mx = fmaxf(mx0, mx1) * a.scale;
+      const bool grow = mx > m + 8.f;  // the first tile, and rarely later
+      if (__any_sync(0xffffffffu, grow)) {
+        const float mn = grow ? mx : m;
+        if (u > 0) {
+          ok = mbar_wait(o_done(i), uint32_t(u - 1) & 1u, &gave_up);
+          if (!__all_sync(0xffffffffu, ok)) {
+            ok = false;
+            break;
+          }
+          tc_after();
+          const float alpha = ex2(m - mn);
+          l *= alpha;
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t x[32];
+            tmem_ld32(t_o + c * 32, x);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * alpha);
+            tmem_st32(t_o + c * 32, x);
+          }
+          tmem_wait_st();
+        }
+        m = mn;
+      }
+      const float neg = m == kNegInf ? 0.f : -m;  // scores of -inf only so far: their exponentials are 0
+      float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t p[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          const float x = ex2(fmaf(__uint_as_float(s[c * 64 + 2 * j]), a.scale, neg));
+          const float y = ex2(fmaf(__uint_as_float(s[c * 64 + 2 * j + 1]), a.scale, neg));
+          l0 += x;  // the sum takes the unrounded values; P V takes them rounded to the cache type
+          l1 += y;
+          p[j] = Elem<T>::pack(x, y);
+        }
+        tmem_st32(t_s + c * 32, p);
+      }
+      l += l0 + l1;
+      tmem_wait_st();
+      tc_before();
+      mbar_arrive(p_full(i));
+    }
+    if (ok && n_mine > 0) ok = mbar_wait(o_done(i), uint32_t(n_mine - 1) & 1u, &gave_up);
+    ok = __all_sync(0xffffffffu, ok);
+    tc_after();
+    const int row = it.row0 + (pair ? i * 128 : 0) + r;
+    const int64_t at = int64_t(pair && i ? it.slab1 : it.slab0) * kSlabRows + r;
+    float* other = reinterpret_cast<float*>(smem + CF::kK);  // [D][128] then m, l: the rings are idle by then
+    static_assert((D + 2) * 512 <= (CF::kKBufs + CF::kVBufs) * CF::kTileBytes, "the join fits the rings");
+    if (!pair) {
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // both groups' products have read the rings
+      if (i == 1) {
+        if (ok && n_mine > 0) {
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t x[32];
+            tmem_ld32(t_o + c * 32, x);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) other[(c * 32 + j) * 128 + r] = __uint_as_float(x[j]);
+          }
+        }
+        other[D * 128 + r] = m;
+        other[(D + 1) * 128 + r] = l;
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+    }
+    if (ok && (pair || i == 0)) {
+      float f0 = 1.f, f1 = 0.f;
+      if (!pair) {
+        const float m1 = other[D * 128 + r], l1 = other[(D + 1) * 128 + r];
+        const float mn = fmaxf(m, m1);
+        f0 = ex2(m - mn);
+        f1 = m1 == kNegInf ? 0.f : ex2(m1 - mn);
+        l = l * f0 + l1 * f1;
+        m = mn;
+      }
+      const bool joined = !pair && n_tiles > 1;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t x[32];
+        tmem_ld32(t_o + c * 32, x);
+        tmem_wait_ld();
+        if (joined) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            x[j] = __float_as_uint(__uint_as_float(x[j]) * f0 + other[(c * 32 + j) * 128 + r] * f1);
+        }
+        if (row < it.n_rows) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 4)
+            *reinterpret_cast<uint4*>(a.slab_o + at * D + c * 32 + j) = make_uint4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+        }
+      }
+      if (row < it.n_rows) *reinterpret_cast<float2*>(a.slab_ml + at * 2) = make_float2(m, l);
+    }
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  if (tid == 0 && gave_up) record_status(a.status, AUGUR_KV_ETIMEOUT);
+  if (warp == 9)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(CF::kCols) : "memory");
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {  // the driver's entry point (no link against libcuda), or null
+  static EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found = cudaDriverEntryPointSymbolNotFound;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return fn;
+}
+
+// Sets a kernel's dynamic shared memory limit once per device.
+int allow_smem(const void* kernel, int bytes, int (&done)[augur_kv_dev::kMaxDevices], const char* what) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= augur_kv_dev::kMaxDevices)
+    return augur_kv_dev::fail(AUGUR_KV_ECUDA, "%s: cannot query the current device", what);
+  std::lock_guard<std::recursive_mutex> lock(augur_kv_dev::g_cache_mutex);
+  if (done[dev] < bytes) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+      return augur_kv_dev::check_launch(what);
+    done[dev] = bytes;
+  }
+  return AUGUR_KV_OK;
+}
+
+// The own launch; behind a shared launch it is a programmatic dependent one.
+template <typename K>
+int launch_own(K kernel, const Args& a, int grid, int threads, size_t smem, bool dependent, cudaStream_t st,
+               const char* what) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(grid));
+  cfg.blockDim = dim3(unsigned(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = dependent ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) return augur_kv_dev::check_launch(what);
+  return AUGUR_KV_OK;
+}
+
+template <typename T, int D>
+int run_tensor(const Args& a, cudaStream_t st) {
+  using augur_kv_dev::fail;
+  if (a.n_items > 0) {
+    EncodeTiled encode = encode_tiled();
+    if (encode == nullptr) return fail(AUGUR_KV_ECUDA, "shared_prefix_attention: no cuTensorMapEncodeTiled in the driver");
+    CUtensorMap map[2];
+    const cuuint64_t dims[4] = {cuuint64_t(D), cuuint64_t(a.block_size), cuuint64_t(a.hkv), cuuint64_t(a.num_blocks)};
+    const cuuint64_t strides[3] = {cuuint64_t(a.row_stride), cuuint64_t(a.head_stride), cuuint64_t(a.blk_stride)};
+    const cuuint32_t box[4] = {64, cuuint32_t(a.block_size < kTileKeys ? a.block_size : kTileKeys), 1, 1};
+    const cuuint32_t one[4] = {1, 1, 1, 1};
+    for (int i = 0; i < 2; ++i) {
+      const CUresult r = encode(&map[i], Elem<T>::kTma, 4, const_cast<char*>(i ? a.v : a.k), dims, strides, box, one,
+                                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+      if (r != CUDA_SUCCESS) return fail(AUGUR_KV_EINVAL, "shared_prefix_attention: the pool has no tensor map (%d)", int(r));
+    }
+    static int done[augur_kv_dev::kMaxDevices] = {0};
+    const int rc = allow_smem(reinterpret_cast<const void*>(shared_umma_kernel<T, D>), ShCfg<D>::kBytes, done, "shared_umma_kernel");
+    if (rc != AUGUR_KV_OK) return rc;
+    shared_umma_kernel<T, D><<<unsigned(a.n_items), kShThreads, ShCfg<D>::kBytes, st>>>(a, map[0], map[1]);
+    const int lc = augur_kv_dev::check_launch("shared_umma_kernel");
+    if (lc != AUGUR_KV_OK) return lc;
+  }
+  const int grid = a.batch * a.hkv * a.n_split;
+  auto own = [&](auto kernel, int heads, int (&done)[augur_kv_dev::kMaxDevices]) {
+    const int parts = own_parts_bytes(D, heads) + join_bytes(a.groups);
+    const int smem = parts > OwnCfg<D>::kPipe ? parts : OwnCfg<D>::kPipe;
+    const int rc = allow_smem(reinterpret_cast<const void*>(kernel), smem, done, "own_mma_kernel");
+    if (rc != AUGUR_KV_OK) return rc;
+    return launch_own(kernel, a, grid, kOwnThreads, size_t(smem), a.n_items > 0, st, "own_mma_kernel");
+  };
+  static int done1[augur_kv_dev::kMaxDevices] = {0}, done2[augur_kv_dev::kMaxDevices] = {0};
+  return a.groups <= 8 ? own(own_mma_kernel<T, D, 1>, 8, done1) : own(own_mma_kernel<T, D, 2>, 16, done2);
+}
+
+template <typename T>
+int run_generic(const Args& a, cudaStream_t st) {
+  const int shared = generic_floats(a.head_dim) * 4;
+  const int smem = shared + 2 * kGRows * 4 + join_bytes(a.groups);
+  static int done_s[augur_kv_dev::kMaxDevices] = {0}, done_o[augur_kv_dev::kMaxDevices] = {0};
+  if (a.n_items > 0) {
+    const int rc = allow_smem(reinterpret_cast<const void*>(shared_generic_kernel<T>), shared, done_s, "shared_generic_kernel");
+    if (rc != AUGUR_KV_OK) return rc;
+    shared_generic_kernel<T><<<unsigned(a.n_items), kGThreads, size_t(shared), st>>>(a);
+    const int lc = augur_kv_dev::check_launch("shared_generic_kernel");
+    if (lc != AUGUR_KV_OK) return lc;
+  }
+  const int rc = allow_smem(reinterpret_cast<const void*>(own_generic_kernel<T>), smem, done_o, "own_generic_kernel");
+  if (rc != AUGUR_KV_OK) return rc;
+  return launch_own(own_generic_kernel<T>, a, a.batch * a.hkv, kGThreads, size_t(smem), a.n_items > 0, st, "own_generic_kernel");
+}
+
+// Parts of a sequence's own keys: enough CTAs for the GPU, and at least 128 keys a part.
+int own_split(int64_t units, int64_t max_own) {
+  const int64_t slots = int64_t(augur_kv_dev::sm_count()) * 2;
+  int64_t n = units > 0 ? slots / units : 1;
+  const int64_t most = max_own / 128;
+  if (n > most) n = most;
+  if (n > 32) n = 32;
+  return int(n < 1 ? 1 : n);
+}
+
+}  // namespace augur_kv_sh
+
+#define AUGUR_KV_EXPORT extern "C" __attribute__((visibility("default")))
+
+AUGUR_KV_EXPORT int augur_kv_shared_prefix_workspace(int32_t n_slabs, int32_t batch, int32_t n_q_heads,
+                                                     int32_t n_kv_heads, int32_t head_dim, int32_t max_own_len,
+                                                     int64_t* counters_bytes, int64_t* scratch_bytes) {
+  using namespace augur_kv_sh;
+  augur_kv_dev::g_last_error[0] = '\0';
+  if (n_slabs < 0 || batch < 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads != 0 || head_dim <= 0 ||
+      max_own_len < 0 || counters_bytes == nullptr || scratch_bytes == nullptr)
+    return augur_kv_dev::fail(AUGUR_KV_EINVAL, "shared_prefix_workspace: bad arguments");
+  const int64_t units = int64_t(batch) * n_kv_heads;
+  const int split = own_split(units, max_own_len);
+  const int64_t rows = int64_t(n_slabs) * kSlabRows + (split > 1 ? units * split * (n_q_heads / n_kv_heads) : 0);
+  *counters_bytes = split > 1 ? units * 4 : 0;
+  *scratch_bytes = rows * (int64_t(head_dim) + 2) * 4 + 64;
+  return AUGUR_KV_OK;
+}
+
+AUGUR_KV_EXPORT int augur_kv_shared_prefix_attention(const augur_kv_shared_prefix_args* p, int32_t layer,
+                                                     const void* q, void* out, void* stream) {
+  using namespace augur_kv_sh;
+  using augur_kv_dev::fail;
+  augur_kv_dev::g_last_error[0] = '\0';
+  if (p == nullptr) return fail(AUGUR_KV_EINVAL, "shared_prefix_attention: null args");
+  if (layer < 0 || layer >= p->n_layers)
+    return fail(AUGUR_KV_EINVAL, "shared_prefix_attention: layer %d outside [0, %d)", layer, p->n_layers);
+  const int es = augur_kv_dev::elem_size(p->dtype);
+  if (es == 0) return fail(AUGUR_KV_EINVAL, "shared_prefix_attention: unknown dtype %d", p->dtype);
+  if (p->batch < 0 || p->n_items < 0) return fail(AUGUR_KV_EINVAL, "shared_prefix_attention: negative sizes");
+  if (p->batch == 0) return AUGUR_KV_OK;
+  if (q == nullptr || out == nullptr || p->k_pool == nullptr || p->v_pool == nullptr || p->block_tables == nullptr ||
+      p->seq_lens == nullptr || p->shared_lens == nullptr || p->ref_starts == nullptr)
+    return fail(AUGUR_KV_EINVAL, "shared_prefix_attention: null pointer argument");
+  if (p->n_q_heads <= 0 || p->n_kv_heads <= 0 || p->n_q_heads % p->n_kv_heads != 0 || p->head_dim <= 0 ||
+      p->block_size <= 0 || p->num_blocks <= 0 || p->max_blocks <= 0 || p->max_own_len < 0 ||
+      p->num_blocks > 0x7ffffffe || int64_t(p->batch) * p->n_kv_heads > (int64_t(1) << 25))
+    return fail(AUGUR_KV_EINVAL, "shared_prefix_attention: bad sizes");
+  if (p->n_items > 0 && (p->items == nullptr || p->members == nullptr || p->run_blocks == nullptr ||
+                         p->refs == nullptr || p->n_slabs <= 0 || p->scratch == nullptr))
+    return fail(AUGUR_KV_EINVAL, "shared_prefix_attention: a plan with items needs its arrays and scratch");
+  if (p->flags != AUGUR_KV_ATTN_AUTO && p->flags != AUGUR_KV_ATTN_GENERIC && p->flags != AUGUR_KV_ATTN_TCGEN05)
+    return fail(AUGUR_KV_EINVAL, "shared_prefix_attention: unknown flags %d", p->flags);
+  Args a;
+  memset(&a, 0, sizeof(a));
+  a.groups = p->n_q_heads / p->n_kv_heads;
+  if (a.groups > kGRows || p->head_dim > kGMaxDim || a.groups * p->head_dim > 32 * kGThreads)
+    return fail(AUGUR_KV_EINVAL,
+                "shared_prefix_attention: at most %d query heads per KV head, head_dim %d, and %d values of both together",
+                kGRows, kGMaxDim, 32 * kGThreads);
+  const int64_t ls = p->pool_strides[0] * es;
+  a.q = static_cast<const char*>(q);
+  a.q_stride_b = p->q_strides[0] * es;
+  a.q_stride_h = p->q_strides[1] * es;
+  a.k = static_cast<const char*>(p->k_pool) + int64_t(layer) * ls;
+  a.v = static_cast<const char*>(p->v_pool) + int64_t(layer) * ls;
+  a.blk_stride = p->pool_strides[1] * es;
+  a.head_stride = p->pool_strides[2] * es;
+  a.row_stride = p->pool_strides[3] * es;
+  a.num_blocks = p->num_blocks;
+  a.block_size = p->block_size;
+  a.tables = p->block_tables;
+  a.tables_stride = p->tables_stride;
+  a.max_blocks = p->max_blocks;
+  a.seq_lens = p->seq_lens;
+  a.shared_lens = p->shared_lens;
+  a.batch = p->batch;
+  a.hq = p->n_q_heads;
+  a.hkv = p->n_kv_heads;
+  a.head_dim = p->head_dim;
+  a.scale = kLog2e / sqrtf(float(p->head_dim));
+  a.out = static_cast<char*>(out);
+  a.out_stride_b = p->out_strides[0] * es;
+  a.out_stride_h = p->out_strides[1] * es;
+  a.items = reinterpret_cast<const Item*>(p->items);
+  a.n_items = p->n_items;
+  a.members = p->members;
+  a.n_members = p->n_members;
+  a.run_blocks = p->run_blocks;
+  a.n_run_blocks = p->n_run_blocks;
+  a.ref_starts = p->ref_starts;
+  a.refs = reinterpret_cast<const int4*>(p->refs);
+  a.n_refs = p->n_refs;
+  a.n_slabs = p->n_slabs;
+  a.status = p->status;
+  if ((reinterpret_cast<uintptr_t>(p->refs) & 15u) != 0 || (reinterpret_cast<uintptr_t>(p->scratch) & 15u) != 0)
+    return fail(AUGUR_KV_EINVAL, "shared_prefix_attention: refs and scratch must be 16-byte aligned");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+
+  // tensor cores: a 16-bit type, head_dim 64 or 128, at most 16 query heads
+  // per KV head, dense 16-byte aligned rows, and blocks that tile 128 keys in
+  // groups of 8 rows (the swizzle's period)
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
+                         reinterpret_cast<uintptr_t>(q) | uintptr_t(a.q_stride_b) | uintptr_t(a.q_stride_h) |
+                         uintptr_t(a.blk_stride) | uintptr_t(a.head_stride) | uintptr_t(a.row_stride);
+  const int bs = p->block_size;
+  const bool blocks_fit = bs % 8 == 0 && (bs < kTileKeys ? kTileKeys % bs == 0 : bs % kTileKeys == 0);
+  const bool tensor_ok = (p->dtype == AUGUR_KV_BF16 || p->dtype == AUGUR_KV_F16) &&
+                         (p->head_dim == 64 || p->head_dim == 128) && a.groups <= kMaxGroups && (bits & 15u) == 0 &&
+                         a.row_stride > 0 && a.head_stride > 0 && a.blk_stride > 0 && blocks_fit;
+  if (p->flags == AUGUR_KV_ATTN_TCGEN05 && !tensor_ok)
+    return fail(AUGUR_KV_EINVAL,
+                "shared_prefix_attention: the tcgen05 kernel needs bf16/fp16, head_dim 64 or 128, <= 16 query heads per "
+                "KV head, 16-byte aligned rows and blocks of 8, 16, 32, 64 or a multiple of 128 tokens");
+  const bool tensor = tensor_ok && p->flags != AUGUR_KV_ATTN_GENERIC;
+  const int64_t units = int64_t(a.batch) * a.hkv;
+  a.n_split = tensor ? own_split(units, p->max_own_len) : 1;
+  {  // scratch: slab sums, slab rows, then the parts'
+    const int64_t slab_rows = int64_t(a.n_slabs) * kSlabRows;
+    const int64_t part_rows = a.n_split > 1 ? units * a.n_split * a.groups : 0;
+    if ((slab_rows + part_rows) * (a.head_dim + 2) * 4 + 64 > p->scratch_bytes && slab_rows + part_rows > 0)
+      return fail(AUGUR_KV_EINVAL, "shared_prefix_attention: the scratch is too small");
+    if (a.n_split > 1 && (p->counters == nullptr || p->counters_bytes < units * 4))
+      return fail(AUGUR_KV_EINVAL, "shared_prefix_attention: the counters are too small");
+    float* f = static_cast<float*>(p->scratch);
+    a.slab_o = f;
+    f += slab_rows * a.head_dim;
+    a.slab_ml = f;
+    f += slab_rows * 2;
+    a.split_ml = f;
+    f += part_rows * 2;
+    a.split_o = f;
+    a.counters = p->counters;
+  }
+  if (units * a.n_split > 0x7fffffff) return fail(AUGUR_KV_EINVAL, "shared_prefix_attention: too many sequences");
+  if (tensor) {
+    if (p->dtype == AUGUR_KV_BF16)
+      return p->head_dim == 64 ? run_tensor<__nv_bfloat16, 64>(a, st) : run_tensor<__nv_bfloat16, 128>(a, st);
+    return p->head_dim == 64 ? run_tensor<__half, 64>(a, st) : run_tensor<__half, 128>(a, st);
+  }
+  if (p->dtype == AUGUR_KV_F32) return run_generic<float>(a, st);
+  if (p->dtype == AUGUR_KV_F16) return run_generic<__half>(a, st);
+  return run_generic<__nv_bfloat16>(a, st);
+}

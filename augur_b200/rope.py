@@ -329,3 +329,113 @@ def write_paged_kv_batch_rope(
         rope_theta=rope_theta, max_position=int(max_position), n_tokens=n_tokens, n_layers=1,
         n_heads=num_heads, head_dim=head_dim, stream=stream)
     return q_out
+
+
+class RopeAxes:
+    """Which axis of a several-axis position (time, height, width, ...) turns each frequency of a
+    head, and the frequencies, on the device: built once per model and reused.
+
+    axis_of_frequency: head_dim / 2 axis numbers; inv_freq: float32 ``[head_dim / 2]`` (its device
+    is the handle's). RopeAxes.runs and RopeAxes.dealt build the two usual layouts.
+    """
+
+    def __init__(self, axis_of_frequency: Sequence[int], inv_freq: Tensor) -> None:
+        axes = [int(a) for a in axis_of_frequency]
+        if not axes or min(axes) < 0:
+            raise ValueError("axis_of_frequency must hold an axis number of at least 0 for every frequency")
+        if tuple(inv_freq.shape) != (len(axes),) or inv_freq.dtype != torch.float32:
+            raise ValueError("inv_freq must be float32 with one value for every frequency")
+        self.n_axes = max(axes) + 1
+        self.half = len(axes)
+        self.inv_freq = inv_freq.contiguous()
+        self.axis = torch.tensor(axes, dtype=torch.int32).to(inv_freq.device)
+
+    @staticmethod
+    def frequencies(head_dim: int, rope_theta: float, device: torch.device) -> Tensor:
+        """inv_freq[j] = rope_theta ** (-2 j / head_dim), as rope_tables has it (float32)."""
+        if head_dim % 2 != 0:
+            raise ValueError(f"head_dim must be even for RoPE, got {head_dim}")
+        return (1.0 / (rope_theta ** (torch.arange(0, head_dim, 2, dtype=torch.float32) / head_dim))).to(device)
+
+    @classmethod
+    def runs(cls, sections: Sequence[int], rope_theta: float, device: torch.device) -> "RopeAxes":
+        """sections[a] consecutive frequencies for axis a (their sum is head_dim / 2)."""
+        axes = [a for a, n in enumerate(sections) for _ in range(n)]
+        return cls(axes, cls.frequencies(2 * len(axes), rope_theta, device))
+
+    @classmethod
+    def dealt(cls, sections: Sequence[int], rope_theta: float, device: torch.device) -> "RopeAxes":
+        """Frequencies dealt to the axes in turn: frequency j goes to axis j % len(sections) while
+        that axis has fewer than sections[axis] of them, and to axis 0 otherwise."""
+        half, n = sum(sections), len(sections)
+        axes = [j % n if j // n < sections[j % n] else 0 for j in range(half)]
+        return cls(axes, cls.frequencies(2 * half, rope_theta, device))
+
+
+def write_paged_kv_batch_rope_axes(
+    cache: PagedKVCache,
+    q: Tensor,
+    key: Tensor,
+    value: Tensor,
+    slot_mapping: Tensor,
+    positions: Tensor,
+    axes: RopeAxes,
+    layer_idx: int,
+    stream: torch.cuda.Stream | None = None,
+) -> Tensor:
+    """write_paged_kv_batch_rope with positions on several axes: rotate q ``[tokens, heads, D]`` and
+    key ``[tokens, kv_heads, D]`` by ``positions[axis, t]`` (int64 ``[axes, tokens]``), write key and
+    value to ``slot_mapping[t]`` of one layer (-1 skips the write, q is still rotated); returns the
+    rotated q.
+
+    Angles are float32 (position times inv_freq), the rotation is computed in float32 and rounded
+    once to the cache dtype. There is no table of positions: nothing to build or to grow, no host
+    sync, and any call can be captured in a CUDA graph.
+    """
+    if key.shape != value.shape or key.dim() != 3 or q.dim() != 3 or q.shape[0] != key.shape[0]:
+        raise ValueError("q [tokens, heads, D], key/value [tokens, kv_heads, D] expected")
+    L, NB, Hkv, bs, D = cache.keys.shape
+    if not 0 <= layer_idx < L:
+        raise ValueError("layer_idx is outside the cache layer range")
+    n_tokens, num_heads, head_dim = key.shape
+    if (num_heads, head_dim) != (Hkv, D) or q.shape[2] != D:
+        raise ValueError("key/value shape does not match cache shape")
+    if axes.half * 2 != D:
+        raise ValueError("axes must have head_dim / 2 frequencies")
+    if slot_mapping.shape != (n_tokens,):
+        raise ValueError("slot_mapping must have shape [tokens]")
+    if positions.dim() != 2 or positions.shape[0] < axes.n_axes or positions.shape[1] != n_tokens:
+        raise ValueError("positions must have shape [axes, tokens]")
+    kc, vc = cache.keys, cache.values
+    dt = kc.dtype
+    if q.dtype != dt or key.dtype != dt or value.dtype != dt or vc.dtype != dt:
+        raise ValueError("q, key, value and the cache must share one dtype")
+    if kc.stride() != vc.stride() or kc.stride(4) != 1:
+        raise ValueError("keys and values must share one layout, head_dim contiguous")
+    device = kc.device
+    _ops.require_cuda("write_paged_kv_batch_rope_axes", kc, vc, q, key, value, slot_mapping, positions, axes.inv_freq)
+    if not (q.device == key.device == value.device == vc.device == slot_mapping.device == positions.device
+            == axes.inv_freq.device == device):
+        raise ValueError("all tensors must be on the cache's device")
+    q, key, value = (_last_dim_contiguous(t) for t in (q, key, value))
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if n_tokens == 0 or q.shape[1] == 0:
+        return q_out
+    slots = slot_mapping if slot_mapping.dtype == torch.int64 else slot_mapping.to(torch.int64)
+    pos = positions if positions.dtype == torch.int64 else positions.to(torch.int64)
+    st = stream if stream is not None else torch.cuda.current_stream(device)
+    es = kc.element_size()
+    off = layer_idx * kc.stride(0) * es
+    with _ops._DeviceGuard(device):
+        code = _lib.load().augur_kv_rope_axes_scatter(
+            q.data_ptr(), _lib.i64_array(q.stride()[:2]), q_out.data_ptr(), _lib.i64_array(q_out.stride()[:2]), q.shape[1],
+            key.data_ptr(), _lib.i64_array(key.stride()[:2]), value.data_ptr(), _lib.i64_array(value.stride()[:2]),
+            _ops.dtype_code(kc), kc.data_ptr() + off, vc.data_ptr() + off, _lib.i64_array(kc.stride()[1:4]), NB, bs,
+            slots.data_ptr(), slots.stride(0), pos.data_ptr(), _lib.i64_array(pos.stride()), pos.shape[0],
+            axes.inv_freq.data_ptr(), axes.axis.data_ptr(), n_tokens, Hkv, D,
+            _ops.status_word(device).data_ptr(), st.cuda_stream)
+    _lib.check(code, "augur_kv_rope_axes_scatter")
+    _ops.launch_count += 1
+    if stream is not None:
+        _ops.keep_until_done(st, q, key, value, q_out, slots, pos, axes.inv_freq, axes.axis)
+    return q_out

@@ -1,0 +1,93 @@
+"""Sampling a token per row of logits: temperature, top-k, top-p and min-p from given random numbers.
+
+augur's generate takes the argmax of the last logits (augur/generation.py); a batch of samples
+forked from one prompt (PagedSequences.fork) needs a draw instead. sample_tokens does it in one
+launch (augur_kv_sample) that reads the logits once: each row's weights are whole numbers, so the
+token depends on the row and its random number alone, not on the batch, the shape of the launch
+or the order of additions.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch import Tensor
+
+from . import _lib, _ops
+
+_MAX_VOCAB = 1 << 21
+
+
+def _setting(name: str, value: float | int | Tensor, rows: int, dtype: torch.dtype, device: torch.device):
+    """(per-row tensor or None, scalar) of a sampling setting."""
+    if isinstance(value, Tensor):
+        if value.shape != (rows,):
+            raise ValueError(f"{name} must be a number or a tensor of shape [rows]")
+        if value.device != device:
+            raise ValueError(f"{name} must be on the logits' device")
+        if value.dtype != dtype:
+            value = value.to(dtype)
+        return value if value.is_contiguous() else value.contiguous(), 0
+    return None, value
+
+
+def sample_tokens(
+    logits: Tensor,
+    uniform: Tensor,
+    temperature: float | Tensor = 1.0,
+    top_k: int | Tensor = 0,
+    top_p: float | Tensor = 1.0,
+    min_p: float | Tensor = 0.0,
+    stream: torch.cuda.Stream | None = None,
+) -> tuple[Tensor, Tensor]:
+    """Draw one token per row; returns (tokens int64 ``[rows]``, logprobs float32 ``[rows]``).
+
+    logits: ``[rows, vocab]`` float32, float16 or bfloat16, vocab contiguous. uniform: float32
+    ``[rows]`` random numbers in [0, 1). Each setting is a number for all rows or a tensor
+    ``[rows]``; they apply in this order:
+
+    - temperature: logits are divided by it; 0 (or less) is greedy, the lowest index of the maximum;
+    - top_k: the k largest stay, ties to the lowest index (0 or less, or vocab and above: all);
+    - top_p: of those, the fewest whose probabilities reach top_p stay (1 and above: all);
+    - min_p: of those, tokens at least min_p times as likely as the likeliest stay.
+
+    The token is the first, in index order, at which the remaining probabilities' running sum
+    passes uniform times their total, and its logprob is taken among them. Tokens with logit
+    -inf or NaN are never drawn; a row without any other gives token -1, logprob -inf.
+    Probabilities below 2^-31 of the likeliest token's count as zero.
+    """
+    if logits.dim() != 2:
+        raise ValueError("logits must be [rows, vocab]")
+    rows, vocab = logits.shape
+    _ops.require_cuda("sample_tokens", logits, uniform)
+    if not 0 < vocab <= _MAX_VOCAB:
+        raise ValueError(f"vocab must be between 1 and {_MAX_VOCAB}")
+    if uniform.shape != (rows,) or uniform.dtype != torch.float32 or uniform.device != logits.device:
+        raise ValueError("uniform must be a float32 tensor of shape [rows] on the logits' device")
+    dtype = _ops._DTYPE_CODES.get(logits.dtype)
+    if dtype is None:
+        raise ValueError(f"unsupported logits dtype {logits.dtype}; use float32, float16 or bfloat16")
+    device = logits.device
+    if logits.stride(1) != 1 and vocab > 1:
+        logits = logits.contiguous()
+    if not uniform.is_contiguous():
+        uniform = uniform.contiguous()
+    t, t_all = _setting("temperature", temperature, rows, torch.float32, device)
+    k, k_all = _setting("top_k", top_k, rows, torch.int32, device)
+    p, p_all = _setting("top_p", top_p, rows, torch.float32, device)
+    m, m_all = _setting("min_p", min_p, rows, torch.float32, device)
+    tokens = torch.empty_like(uniform, dtype=torch.int64)
+    logprobs = torch.empty_like(uniform)
+    if rows == 0:
+        return tokens, logprobs
+    st = stream if stream is not None else torch.cuda.current_stream(device)
+    with _ops._DeviceGuard(device):
+        code = _lib.load().augur_kv_sample(
+            logits.data_ptr(), logits.stride(0), rows, vocab, dtype, uniform.data_ptr(),
+            None if t is None else t.data_ptr(), t_all, None if k is None else k.data_ptr(), k_all,
+            None if p is None else p.data_ptr(), p_all, None if m is None else m.data_ptr(), m_all,
+            tokens.data_ptr(), logprobs.data_ptr(), st.cuda_stream)
+    _lib.check(code, "augur_kv_sample")
+    _ops.launch_count += 1
+    if stream is not None:
+        _ops.keep_until_done(st, logits, uniform, t, k, p, m, tokens, logprobs)
+    return tokens, logprobs

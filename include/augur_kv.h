@@ -445,6 +445,149 @@ int augur_kv_copy_runs_noalloc(const void* src_k, const void* src_v,
                                int32_t n_layers, int32_t n_heads, int32_t head_dim,
                                int32_t flags, int32_t* status, void* stream);
 
+/*
+ * augur_kv_shared_prefix_attention — decode attention of a batch whose
+ * sequences share blocks (forks of one prompt, prompts with a common prefix):
+ * every shared block is read once for all the sequences that hold it.
+ *
+ * The result is augur_kv_paged_decode_attention's: sequence b's query token
+ * attends to its positions [0, seq_lens[b]), out = softmax(q k^T /
+ * sqrt(head_dim)) v, with float32 sums and one rounding at the end (the
+ * probabilities are rounded to the cache dtype before the product with v on
+ * the tensor cores). A sequence of length 0 gives zeros.
+ *
+ * The plan. A run is a range of consecutive blocks that a set of sequences
+ * (its members) hold at the same place in their tables; a sequence's runs
+ * follow one another from its position 0 and cover its first shared_lens[b]
+ * positions (a multiple of block_size, at most seq_lens[b]). The rows of a run
+ * are its members x (n_q_heads / n_kv_heads) query heads of one KV head,
+ * member-major; they are cut into tiles of 128, and the run's positions into
+ * `ranges` ranges. Slab (kv_head * tiles + tile) * ranges + range past the
+ * run's first slab takes that tile's part over that range. An item covers
+ * one range for one tile, or for two neighbouring tiles (slab1 >= 0):
+ *   items[i]: member0, n_rows, block0, n_blocks, kv_head, row0, key0, key1,
+ *             slab0, slab1, 0, 0
+ * with the run's members at members[member0..], its blocks at
+ * run_blocks[block0..block0+n_blocks), the first of its rows row0, and its
+ * positions [key0, key1) counted from the run's first (key0 a multiple of
+ * 128). refs[r] = {first slab, ranges, member's place in the run, tiles} for r
+ * in [ref_starts[b], ref_starts[b+1]) are sequence b's runs.
+ * augur_b200.attention.SharedPrefixTables builds all of this from block tables.
+ *
+ * bf16/fp16 with head_dim 64 or 128, at most 16 query heads per KV head,
+ * 16-byte aligned rows and blocks of 8, 16, 32, 64 or a multiple of 128 tokens
+ * run on the tensor cores (AUGUR_KV_ATTN_TCGEN05 insists on that); everything
+ * else on CUDA cores in float32 (AUGUR_KV_ATTN_GENERIC forces that): at most
+ * 64 query heads per KV head, head_dim at most 256, their product at most
+ * 8,192. Indices outside the tables, the pool or the plan record
+ * AUGUR_KV_EBOUNDS and read as zeros; a bounded wait that gives up records
+ * AUGUR_KV_ETIMEOUT. counters are zeroed once and left zero by every call;
+ * scratch needs no initial contents.
+ */
+typedef struct augur_kv_shared_prefix_args {
+  const void* k_pool; /* layer 0 of the pools */
+  const void* v_pool;
+  int64_t pool_strides[4]; /* elements: layer, block, kv head, row */
+  int64_t num_blocks;
+  int32_t block_size;
+  int32_t n_layers;
+  int32_t n_q_heads;
+  int32_t n_kv_heads;
+  int32_t head_dim;
+  int32_t dtype;
+  int32_t batch;
+  int32_t flags;         /* AUGUR_KV_ATTN_AUTO, _GENERIC or _TCGEN05 */
+  int64_t q_strides[2];  /* elements: sequence, head; head_dim contiguous */
+  int64_t out_strides[2];
+  const int32_t* block_tables; /* [batch][tables_stride] */
+  int64_t tables_stride;
+  int64_t max_blocks;
+  const int32_t* seq_lens;    /* [batch] */
+  const int32_t* shared_lens; /* [batch] positions its runs cover */
+  int32_t max_own_len;        /* largest seq_lens[b] - shared_lens[b], or more */
+  int32_t n_items;
+  const int32_t* items; /* [n_items][12] */
+  const int32_t* members;
+  const int32_t* run_blocks;
+  const int32_t* ref_starts; /* [batch + 1] */
+  const int32_t* refs;       /* [n_refs][4], 16-byte aligned */
+  int32_t n_members;
+  int32_t n_run_blocks;
+  int32_t n_refs;
+  int32_t n_slabs;
+  void* scratch; /* 16-byte aligned */
+  int64_t scratch_bytes;
+  int32_t* counters;
+  int64_t counters_bytes;
+  int32_t* status; /* device int32 or NULL */
+} augur_kv_shared_prefix_args;
+
+int augur_kv_shared_prefix_attention(const augur_kv_shared_prefix_args* args, int32_t layer, const void* q,
+                                     void* out, void* stream);
+
+/* Bytes of counters and scratch augur_kv_shared_prefix_attention needs. */
+int augur_kv_shared_prefix_workspace(int32_t n_slabs, int32_t batch, int32_t n_q_heads, int32_t n_kv_heads,
+                                     int32_t head_dim, int32_t max_own_len, int64_t* counters_bytes,
+                                     int64_t* scratch_bytes);
+
+/*
+ * augur_kv_rope_axes_scatter — rotary positions with several axes (time,
+ * height, width for images and video), fused with the append of keys and
+ * values to a paged pool layer.
+ *
+ * Token t has position positions[axis*S[0] + t*S[1]] on each of n_axes axes
+ * (S = position_strides). Frequency j (0 <= j < head_dim/2) turns elements j
+ * and j + head_dim/2 of every q and k row by
+ *   angle = float(position on axis axis_of_frequency[j]) * inv_freq[j]
+ * in float32, rounded once to the dtype. q goes to q_out, k and v to slot
+ * slots[t*slot_stride] of the pool (block = slot / block_size); a negative
+ * slot writes no k and v. A slot outside the pool, or an axis outside
+ * [0, n_axes), records AUGUR_KV_EBOUNDS (the row is not written; the frequency
+ * turns nothing). Positions are exact up to 2^24.
+ * All strides are in elements: q, q_out, k, v: token, head; pool: block, kv
+ * head, row; head_dim elements are contiguous. k and v pools share strides.
+ */
+int augur_kv_rope_axes_scatter(const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides,
+                               int32_t n_q_heads, const void* k, const int64_t* k_strides, const void* v,
+                               const int64_t* v_strides, int32_t dtype, void* k_pool, void* v_pool,
+                               const int64_t* pool_strides, int64_t num_blocks, int32_t block_size,
+                               const int64_t* slots, int64_t slot_stride, const int64_t* positions,
+                               const int64_t* position_strides, int32_t n_axes,
+                               const float* inv_freq,            /* device [head_dim/2] */
+                               const int32_t* axis_of_frequency, /* device [head_dim/2] */
+                               int64_t n_tokens, int32_t n_kv_heads, int32_t head_dim,
+                               int32_t* status, /* device int32 or NULL */
+                               void* stream);
+
+/*
+ * augur_kv_sample — one token per row of logits from a given uniform number:
+ * temperature, then top-k, then top-p, then min-p.
+ *
+ * With m the row's maximum, z_i = (x_i - m) * (1 / T) and whole-number weights
+ * w_i = floor(2^31 exp(z_i)) (so sums are exact and the token does not depend
+ * on the order of additions):
+ *   top-k  keeps the k largest z, ties to the lowest index (k <= 0 or k >=
+ *          vocab: all);
+ *   top-p  of those, in falling order, keeps the entries before which less
+ *          than ceil(p * their sum) has been passed (p >= 1: all; the first
+ *          always stays);
+ *   min-p  of those, keeps the entries with exp(z_i) >= min_p (at most 1 is
+ *          used, so the maximum stays);
+ *   token  the first index, in rising order, at which the kept weights'
+ *          running sum passes floor(u * their sum).
+ * T <= 0 is greedy (the lowest index of the maximum). NaN logits count as
+ * -inf; -inf is never drawn; a row with nothing else gives token -1 and
+ * log-probability -inf. Infinite maxima share the draw between them.
+ * logprobs (or NULL) take log(w_token / the kept weights' sum).
+ * temperature, top_k, top_p and min_p are device arrays [rows], or NULL for
+ * the scalar beside them. logits: row_stride elements between rows, vocab <=
+ * 2^21 contiguous entries, aligned to their type.
+ */
+int augur_kv_sample(const void* logits, int64_t row_stride, int32_t rows, int32_t vocab, int32_t dtype,
+                    const float* uniform, const float* temperature, float temperature_all, const int32_t* top_k,
+                    int32_t top_k_all, const float* top_p, float top_p_all, const float* min_p, float min_p_all,
+                    int64_t* tokens, float* logprobs, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
