@@ -18,20 +18,21 @@
 //
 // What bounds it: a row is read once (the floor is its bytes over the HBM
 // rate); the rest is the latency of a handful of cluster exchanges.
-//  * A row belongs to a cluster of 1 to 8 CTAs; each keeps its part of the row
-//    in shared memory as float32, so HBM is read once and the later passes run
-//    from shared memory.
-//  * Only entries that can still matter get a weight. With top-k, entries
-//    below a bound of the k-th largest (the smallest, over the CTAs, of their
-//    ceil(k / CTAs)-th largest per-thread maximum: at least k entries reach
-//    it) are dropped by one comparison. With top-p alone a coarse histogram
-//    of the entries within e^-12 of the maximum shows where the nucleus ends.
-//    What remains (at most kList entries, in index order) goes to CTA 0 of the
-//    cluster, which sorts it, cuts it and draws.
-//  * Where more than kList entries remain (flat rows) the cut is found by a
-//    radix search over the bits of |z| (count for top-k, mass for top-p), and
-//    the draw walks the row in place; a row with neither top-k nor top-p walks
-//    at once.
+//  * A row belongs to a cluster of 1 to 8 CTAs; each copies its part of the row
+//    to shared memory (cp.async), so HBM is read once and every later pass
+//    runs from there.
+//  * Top-k: the per-thread maxima, binned by |z|, bound the k-th largest (at
+//    least k entries reach the bin by which k maxima are counted). The few
+//    entries at or above that bin go to a list in index order, which CTA 0 of
+//    the cluster sorts, cuts and draws from.
+//  * Top-p: a histogram of |z| (counts and masses, 512 bins over the range
+//    that has a weight) shows the bin where the nucleus ends. If the bins up to
+//    it hold at most kList entries the list takes them all; else the bin is
+//    split again until the entries in question fit the list or share one key,
+//    which gives the cut exactly, and the draw walks the row in place. Top-k
+//    takes this way too where its own bound leaves too many.
+//  * With neither, the draw walks the row at once; greedy rows look for the
+//    lowest index of the maximum only.
 
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -50,11 +51,9 @@ namespace cg = cooperative_groups;
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kList = 2048;     // most entries CTA 0 sorts
-constexpr int kBins = 64;       // coarse bins of |z| in [0, kBinRange)
-constexpr float kBinRange = 12.f;
-constexpr float kBinScale = kBins / kBinRange;
-constexpr int kDigits = 256;    // radix search: 8 bits a level
+constexpr int kList = 2048;  // most entries CTA 0 sorts
+constexpr int kBins = kThreads;  // bins of a histogram, one a thread
+constexpr float kBinScale = kBins / 21.6f;  // linear bins of |z|: e^-21.6 has no weight any more
 constexpr int kMaxCluster = 8;
 constexpr float kNegInf = -INFINITY;
 constexpr float kUnit = 2147483648.f;  // 2^31
@@ -73,26 +72,29 @@ struct SampleArgs {
   int32_t top_k_s;
   int64_t* tokens;
   float* logprobs;  // may be null
-  int32_t granules;  // 16-byte granules a CTA's part holds at most (its shared memory)
 };
 
 // What the CTAs of a cluster tell one another (each writes its own copy).
 struct Shared {
-  float cta_max, cta_tau;
+  float cta_max;
+  uint32_t first;  // greedy: the lowest index of the maximum
   uint32_t count, ties;
   unsigned long long mass;
   uint32_t warp_count[kWarps];
   unsigned long long warp_mass[kWarps];
-  uint32_t hist_count[kDigits];
-  unsigned long long hist_mass[kDigits];
-  // results of a CTA-wide step, written by one thread
-  uint32_t r0, r1;
-  unsigned long long r2, r3;
+  // histogram; masses in halves of 16 bits (a part has at most 65,536 entries), or whole where it has more
+  uint32_t bin_count[kBins], bin_lo[kBins], bin_hi[kBins];
+  // results of a step, written by one thread; cut: by CTA 0 for the cluster
+  uint32_t found, found_n;
+  unsigned long long found_m, found_bin_m;
+  uint32_t cut_key, cut_ties;
+  unsigned long long cut_mass;
 };
 
 template <typename T> struct Logit;
 template <> struct Logit<float> {
-  static constexpr int kVec = 4;
+  static constexpr int kVec = 4;  // entries of 16 bytes
+  static constexpr uint32_t kLowest = 0xff800000u;  // -inf, as stored
   static __device__ __forceinline__ float one(const char* p) { return *reinterpret_cast<const float*>(p); }
   static __device__ __forceinline__ void unpack(const uint4& u, float* f) {
     f[0] = __uint_as_float(u.x);
@@ -103,6 +105,7 @@ template <> struct Logit<float> {
 };
 template <> struct Logit<__nv_bfloat16> {
   static constexpr int kVec = 8;
+  static constexpr uint32_t kLowest = 0xff80ff80u;
   static __device__ __forceinline__ float one(const char* p) {
     return __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(p));
   }
@@ -117,6 +120,7 @@ template <> struct Logit<__nv_bfloat16> {
 };
 template <> struct Logit<__half> {
   static constexpr int kVec = 8;
+  static constexpr uint32_t kLowest = 0xfc00fc00u;
   static __device__ __forceinline__ float one(const char* p) {
     return __half2float(*reinterpret_cast<const __half*>(p));
   }
@@ -132,23 +136,17 @@ template <> struct Logit<__half> {
 };
 
 __device__ __forceinline__ float no_nan(float x) { return x == x ? x : kNegInf; }  // a NaN is never drawn
-// floats as unsigned integers of the same order
-__device__ __forceinline__ uint32_t ordered(float x) {
-  const uint32_t b = __float_as_uint(x);
-  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-}
-__device__ __forceinline__ float from_ordered(uint32_t o) {
-  return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
-}
 
 // The row's scale: z of an entry, its weight, and its key (bits of |z|: rising
 // keys are falling z; kDead for entries that can never be drawn).
 struct Scale {
-  float m, inv;  // inv = 0: greedy
+  float m, inv;
   bool greedy;
+  bool plain;  // m and inv finite: no case needs care
   __device__ __forceinline__ float z(float x) const {
-    if (x == m) return 0.f;
     const float v = (x - m) * inv;
+    if (plain) return v;
+    if (x == m) return 0.f;
     return (greedy || !(v <= 0.f)) ? kNegInf : v;  // -inf * 0 and the like: dead
   }
 };
@@ -182,16 +180,66 @@ __device__ __forceinline__ unsigned long long draw_target(float u, unsigned long
   return v < s ? v : s - 1;
 }
 
+__device__ __forceinline__ float bin_of(float z) { return fabsf(z) * kBinScale; }
+// The smallest key whose bin is b or above.
+__device__ __forceinline__ uint32_t bin_edge(int b) {
+  uint32_t lo = 0, hi = kDead;  // the key of an infinite |z| is past every bin
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    if (__uint_as_float(mid) * kBinScale >= float(b)) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo;
+}
+
+// The first position of CTA-wide running sums: found = the thread whose inclusive sum `incl` is the
+// first to reach goal (kBins if none does).
+__device__ __forceinline__ void scan_pair(Shared& sh, uint32_t n, unsigned long long m, uint32_t& cum_n,
+                                          unsigned long long& cum_m) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  cum_n = warp_scan(n, lane);
+  cum_m = warp_scan(m, lane);
+  if (lane == 31) {
+    sh.warp_count[warp] = cum_n;
+    sh.warp_mass[warp] = cum_m;
+  }
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) {
+    cum_n += sh.warp_count[w];
+    cum_m += sh.warp_mass[w];
+  }
+  __syncthreads();
+}
+
+// Sorts n entries (a power of two from 32 on) in shared memory, rising.
+__device__ __forceinline__ void sort_entries(unsigned long long* e, int n) {
+  for (int size = 2; size <= n; size <<= 1) {
+    for (int stride = size >> 1; stride > 0; stride >>= 1) {
+      for (int p = threadIdx.x; p < n / 2; p += kThreads) {
+        const int i = ((p & ~(stride - 1)) << 1) | (p & (stride - 1)), j = i + stride;
+        const unsigned long long x = e[i], y = e[j];
+        if ((x > y) == ((i & size) == 0)) {
+          e[i] = y;
+          e[j] = x;
+        }
+      }
+      __syncthreads();
+    }
+  }
+}
+
 template <typename T, bool kResident>
-__global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
   constexpr int VEC = Logit<T>::kVec;
+  constexpr int kStep = 32 * VEC;  // slots a warp takes at a time
+  constexpr int kPer = kList / kThreads;
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ Shared sh;
-  uint32_t* list_key = reinterpret_cast<uint32_t*>(dyn);  // CTA 0: the remaining entries in index order
-  uint32_t* list_idx = list_key + kList;
-  // CTA 0's sort buffer; it lies over the row, which is no longer read then
-  unsigned long long* sorted = reinterpret_cast<unsigned long long*>(dyn + kList * 8);
-  float* xs = reinterpret_cast<float*>(dyn + kList * 8);  // this CTA's part of the row
+  // entries in question, (key, index), in index order; CTA 0's hold the cluster's
+  unsigned long long* list = reinterpret_cast<unsigned long long*>(dyn);
+  // this CTA's part of the row, as stored; CTA 0's sorted copy of the list lies over it once it is no longer read
+  unsigned char* part = dyn + kList * 8;
+  unsigned long long* sorted = reinterpret_cast<unsigned long long*>(part);
 
   cg::cluster_group cluster = cg::this_cluster();
   const int C = int(cluster.num_blocks()), rank = int(cluster.block_rank());
@@ -203,89 +251,75 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a) {
   const int lead = int((reinterpret_cast<uintptr_t>(base) & 15u) / sizeof(T));
   const int total_g = int((int64_t(lead) + a.vocab + VEC - 1) / VEC);
   const int g0 = int(int64_t(total_g) * rank / C), g1 = int(int64_t(total_g) * (rank + 1) / C);
-  const int n_slots = (g1 - g0) * VEC;
+  const int n_g = g1 - g0, n_slots = n_g * VEC;
   const int first = g0 * VEC - lead;
-  auto granule = [&](int g, float* f) {  // entries of granule g of this part; those outside the row: -inf
-    const int i0 = first + g * VEC;
-    if (i0 >= 0 && i0 + VEC <= a.vocab) {
-      const uint4 u = __ldcs(reinterpret_cast<const uint4*>(base + int64_t(i0) * int64_t(sizeof(T))));
-      Logit<T>::unpack(u, f);
+  const char* part_base = base + int64_t(first) * int64_t(sizeof(T));  // 16-byte aligned
+  // granules that lie in the row whole: [in0, in1)
+  const int in0 = first < 0 ? 1 : 0, in1 = first + n_slots > a.vocab ? n_g - 1 : n_g;
+  auto edge_granule = [&](int g) -> uint4 {  // entries outside the row: -inf
+    uint4 u = make_uint4(Logit<T>::kLowest, Logit<T>::kLowest, Logit<T>::kLowest, Logit<T>::kLowest);
+    T* e = reinterpret_cast<T*>(&u);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) f[j] = no_nan(f[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const int i = i0 + j;
-        f[j] = i >= 0 && i < a.vocab ? no_nan(Logit<T>::one(base + int64_t(i) * int64_t(sizeof(T)))) : kNegInf;
+    for (int j = 0; j < VEC; ++j) {
+      const int i = first + g * VEC + j;
+      if (i >= 0 && i < a.vocab) e[j] = reinterpret_cast<const T*>(base)[i];
+    }
+    return u;
+  };
+  if constexpr (kResident) {
+    for (int g = tid; g < n_g; g += kThreads) {
+      if (g >= in0 && g < in1) {
+        const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(part + g * 16));
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(part_base + int64_t(g) * 16) : "memory");
+      } else {
+        *reinterpret_cast<uint4*>(part + g * 16) = edge_granule(g);
       }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  }
+  auto granule = [&](int g, float* f) {
+    uint4 u;
+    if constexpr (kResident) u = *reinterpret_cast<const uint4*>(part + g * 16);
+    else u = g >= in0 && g < in1 ? __ldg(reinterpret_cast<const uint4*>(part_base + int64_t(g) * 16)) : edge_granule(g);
+    Logit<T>::unpack(u, f);
   };
+  const float temperature = a.temperature ? __ldg(a.temperature + row) : a.temperature_s;
+  int k = a.top_k ? __ldg(a.top_k + row) : a.top_k_s;
+  const float top_p = a.top_p ? __ldg(a.top_p + row) : a.top_p_s;
+  const float min_p_given = a.min_p ? __ldg(a.min_p + row) : a.min_p_s;
+  const float min_p = min_p_given > 0.f ? fminf(min_p_given, 1.f) : 0.f;
+  const float u = __ldg(a.uniform + row);
 
-  float tmax = kNegInf;
+  float tmax = kNegInf;  // fmaxf passes NaN over
 #pragma unroll 4
-  for (int g = tid; g < g1 - g0; g += kThreads) {
+  for (int g = tid; g < n_g; g += kThreads) {  // the granules this thread copied itself
     float f[VEC];
     granule(g, f);
 #pragma unroll
     for (int j = 0; j < VEC; ++j) tmax = fmaxf(tmax, f[j]);
-    if constexpr (kResident) {
-#pragma unroll
-      for (int j = 0; j < VEC; j += 4)
-        *reinterpret_cast<float4*>(xs + g * VEC + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
-    }
   }
-  const float temperature = a.temperature ? __ldg(a.temperature + row) : a.temperature_s;
-  int k = a.top_k ? __ldg(a.top_k + row) : a.top_k_s;
-  const float top_p = a.top_p ? __ldg(a.top_p + row) : a.top_p_s;
-  const float min_p = fminf(a.min_p ? __ldg(a.min_p + row) : a.min_p_s, 1.f);
-  const float u = __ldg(a.uniform + row);
-  const bool greedy = !(temperature > 0.f);
-  if (greedy) k = 1;
-  const bool use_k = k > 0 && k < a.vocab;
-  const bool use_p = top_p < 1.f;
-
-  // the CTA's maximum, and its ceil(k / C)-th largest per-thread maximum
-  const int k_part = (k + C - 1) / C;
-  const bool use_tau = use_k && k_part <= kThreads / 4;
   {
-    uint32_t lo = ordered(tmax), hi = lo;
-    lo = __reduce_min_sync(0xffffffffu, lo);
-    hi = __reduce_max_sync(0xffffffffu, hi);
-    if (lane == 0) {
-      sh.warp_count[warp] = lo;
-      sh.warp_mass[warp] = hi;
-    }
+    float m = tmax;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) sh.warp_count[warp] = __float_as_uint(m);
+    sh.bin_count[tid] = 0;
     __syncthreads();
-    lo = sh.warp_count[lane & (kWarps - 1)];
-    hi = uint32_t(sh.warp_mass[lane & (kWarps - 1)]);
-    lo = __reduce_min_sync(0xffffffffu, lo);
-    hi = __reduce_max_sync(0xffffffffu, hi);
-    if (tid == 0) sh.cta_max = from_ordered(hi);
-    if (use_tau && k_part == 1) {
-      lo = hi;
-    } else if (use_tau) {
-      // k_part threads reach lo throughout, so stopping early only loosens the bound
-      const uint32_t mine = ordered(tmax);
-      for (int it = 0; it < 20 && lo < hi; ++it) {
-        const uint32_t mid = lo + (hi - lo) / 2 + 1;
-        if (__syncthreads_count(mine >= mid) >= k_part) lo = mid;
-        else hi = mid - 1;
-      }
+    if (tid == 0) {
+      for (int w = 1; w < kWarps; ++w) m = fmaxf(m, __uint_as_float(sh.warp_count[w]));
+      sh.cta_max = m;
     }
-    if (tid == 0) sh.cta_tau = from_ordered(lo);
   }
   cluster.sync();
   Scale sc;
-  float tau = INFINITY;
   sc.m = kNegInf;
-  for (int c = 0; c < C; ++c) {
-    const Shared* o = cluster.map_shared_rank(&sh, c);
-    sc.m = fmaxf(sc.m, o->cta_max);
-    tau = fminf(tau, o->cta_tau);
-  }
-  if (k == 1) tau = sc.m;
-  sc.greedy = greedy;
-  sc.inv = greedy ? 0.f : 1.f / temperature;
+  for (int c = 0; c < C; ++c) sc.m = fmaxf(sc.m, cluster.map_shared_rank(&sh, c)->cta_max);
+  sc.greedy = !(temperature > 0.f);
+  sc.inv = sc.greedy ? 0.f : 1.f / temperature;
+  sc.plain = !sc.greedy && fabsf(sc.m) < INFINITY && sc.inv > 0.f && sc.inv < INFINITY;
+  if (sc.greedy) k = 1;
+  bool use_k = k > 0 && k < a.vocab;
+  const bool use_p = top_p < 1.f;
   if (sc.m == kNegInf) {  // nothing can be drawn
     if (rank == 0 && tid == 0) {
       a.tokens[row] = -1;
@@ -295,190 +329,133 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a) {
     return;
   }
 
-  // warp w owns slots [w0, w1), four consecutive ones a lane and step, so warps hold rising indices
-  const int per = ((n_slots + kWarps - 1) / kWarps + 127) & ~127;
+  // warp w owns slots [w0, w1), VEC consecutive ones a lane and step, so warps hold rising indices
+  const int per = ((n_slots + kWarps - 1) / kWarps + kStep - 1) / kStep * kStep;
   const int w0 = min(warp * per, n_slots), w1 = min(w0 + per, n_slots);
-  auto load4 = [&](int s, float* f) {  // slots s .. s + 3 (s a multiple of 4); past the part: -inf
-    if constexpr (kResident) {
-      if (s < w1) {
-        const float4 v = *reinterpret_cast<const float4*>(xs + s);
-        f[0] = v.x;
-        f[1] = v.y;
-        f[2] = v.z;
-        f[3] = v.w;
-        return;
-      }
-      f[0] = f[1] = f[2] = f[3] = kNegInf;
+  auto load = [&](int s, float* f) {  // slots s .. s + VEC - 1 (whole granules); past the warp's: -inf
+    if (s < w1) {
+      granule(s / VEC, f);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) f[j] = no_nan(f[j]);
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int i = first + s + j;
-        f[j] = s < w1 && i >= 0 && i < a.vocab ? no_nan(Logit<T>::one(base + int64_t(i) * int64_t(sizeof(T)))) : kNegInf;
-      }
+      for (int j = 0; j < VEC; ++j) f[j] = kNegInf;
     }
   };
 
-  // ---- which entries remain: x >= tau, or coarse bins up to `last_bin`; n of them in all
-  bool listed = false;
-  int last_bin = -1;
-  unsigned long long total = 0;  // the row's whole mass, where it is known
-  if (use_tau) {
-    listed = true;
-  } else if (use_k || use_p) {
-    for (int i = tid; i < kBins; i += kThreads) {
-      sh.hist_count[i] = 0;
-      sh.hist_mass[i] = 0;
-    }
-    __syncthreads();
-    unsigned long long sum = 0;
-    for (int s = w0 + lane * 4; s < w1; s += 128) {
-      float f[4];
-      load4(s, f);
+  if (k == 1) {  // the lowest index of the maximum
+    uint32_t best = 0xffffffffu;
+    for (int g = tid; g < n_g && best == 0xffffffffu; g += kThreads) {
+      float f[VEC];
+      granule(g, f);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float z = sc.z(f[j]);
-        const uint32_t w = weight(expf(z));
-        sum += w;
-        const float b = fabsf(z) * kBinScale;
-        if (b < float(kBins)) {
-          atomicAdd(&sh.hist_count[int(b)], 1u);
-          atomicAdd(&sh.hist_mass[int(b)], (unsigned long long)w);
-        }
-      }
+      for (int j = VEC - 1; j >= 0; --j)
+        if (f[j] == sc.m) best = uint32_t(first + g * VEC + j);
     }
-    sum = warp_sum(sum);
-    if (lane == 0) sh.warp_mass[warp] = sum;
+    best = __reduce_min_sync(0xffffffffu, best);
+    if (lane == 0) sh.warp_count[warp] = best;
     __syncthreads();
     if (tid == 0) {
-      unsigned long long m = 0;
-      for (int w = 0; w < kWarps; ++w) m += sh.warp_mass[w];
-      sh.mass = m;
+      for (int w = 1; w < kWarps; ++w) best = min(best, sh.warp_count[w]);
+      sh.first = best;
     }
     cluster.sync();
-    if (warp == 0) {
-      unsigned long long all = 0, m0 = 0, m1 = 0;
-      uint32_t c0 = 0, c1 = 0;
-      for (int c = 0; c < C; ++c) {
-        const Shared* o = cluster.map_shared_rank(&sh, c);
-        all += o->mass;
-        c0 += o->hist_count[2 * lane];
-        c1 += o->hist_count[2 * lane + 1];
-        m0 += o->hist_mass[2 * lane];
-        m1 += o->hist_mass[2 * lane + 1];
-      }
-      const uint32_t cs = warp_scan(c0 + c1, lane);
-      const unsigned long long ms = warp_scan(m0 + m1, lane);
-      // the first bin by which k entries, or the nucleus of the whole row, are reached
-      bool at0, at1;
-      if (use_k) {
-        at0 = cs - c1 >= uint32_t(k);
-        at1 = cs >= uint32_t(k);
-      } else {
-        const unsigned long long need = mass_needed(top_p, all);
-        at0 = ms - m1 >= need;
-        at1 = ms >= need;
-      }
-      const uint32_t has = __ballot_sync(0xffffffffu, at1);
-      if (lane == 0) {
-        sh.r0 = 0xffffffffu;
-        sh.r1 = 0xffffffffu;
-        sh.r2 = all;
-      }
-      __syncwarp();
-      if (has != 0 && lane == __ffs(has) - 1) {
-        sh.r0 = uint32_t(2 * lane + (at0 ? 0 : 1));
-        sh.r1 = at0 ? cs - c1 : cs;
-      }
+    if (rank == 0 && tid == 0) {
+      for (int c = 1; c < C; ++c) best = min(best, cluster.map_shared_rank(&sh, c)->first);
+      a.tokens[row] = int64_t(best);
+      if (a.logprobs) a.logprobs[row] = 0.f;
     }
-    __syncthreads();
-    total = sh.r2;
-    if (sh.r1 <= uint32_t(kList)) {
-      listed = true;
-      last_bin = int(sh.r0);
-    }
-    cluster.sync();  // everyone has read the bins
+    cluster.sync();
+    return;
   }
 
-  auto remains = [&](float x) -> bool {
-    return last_bin < 0 ? (x >= tau && x > kNegInf) : fabsf(sc.z(x)) * kBinScale < float(last_bin + 1);
-  };
-  uint32_t n_all = 0;
-  if (listed) {
+  // ---- the bins up to `last_bin` hold all that can be drawn, if they fit the list
+  int last_bin = -1;
+  unsigned long long total = 0;  // the row's mass, where it is known
+  if (use_k) {  // per-thread maxima: k of them reach this bin, so k entries do
+    const float b = bin_of(sc.z(tmax));
+    if (b < float(kBins)) atomicAdd(&sh.bin_count[int(b)], 1u);
+    cluster.sync();
+    uint32_t n = 0;
+    for (int c = 0; c < C; ++c) n += cluster.map_shared_rank(&sh, c)->bin_count[tid];
+    if (tid == 0) sh.found = kBins;
+    uint32_t cum_n;
+    unsigned long long cum_m;
+    scan_pair(sh, n, 0ull, cum_n, cum_m);
+    if (cum_n >= uint32_t(k) && cum_n - n < uint32_t(k)) sh.found = uint32_t(tid);
+    __syncthreads();
+    if (sh.found < uint32_t(kBins)) last_bin = int(sh.found);
+    else cluster.sync();  // everyone has read the bins
+  }
+
+  // Entries that `in` picks, into CTA 0's list in index order. Returns how many there are in the
+  // cluster; only where they fit (kList) is the list filled, and only in CTA 0.
+  auto collect = [&](auto in) -> uint32_t {
     uint32_t mine = 0;
-    for (int s = w0 + lane * 4; s < w1; s += 128) {
-      float f[4];
-      load4(s, f);
+    for (int s = w0 + lane * VEC; s < w1; s += kStep) {
+      float f[VEC];
+      load(s, f);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) mine += remains(f[j]) ? 1u : 0u;
+      for (int j = 0; j < VEC; ++j) mine += in(sc.z(f[j])) ? 1u : 0u;
     }
     mine = __reduce_add_sync(0xffffffffu, mine);
     if (lane == 0) sh.warp_count[warp] = mine;
     __syncthreads();
-    if (tid == 0) {
-      uint32_t n = 0;
-      for (int w = 0; w < kWarps; ++w) n += sh.warp_count[w];
-      sh.count = n;
+    uint32_t before = 0, here_all = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      const uint32_t n = sh.warp_count[w];
+      before += w < warp ? n : 0;
+      here_all += n;
     }
-    cluster.sync();
-    uint32_t before = 0;
-    for (int c = 0; c < C; ++c) {
-      const uint32_t n = cluster.map_shared_rank(&sh, c)->count;
-      before += c < rank ? n : 0;
-      n_all += n;
-    }
-    listed = n_all <= uint32_t(kList);
-    if (listed && mine != 0) {  // to CTA 0's list, in index order
-      for (int w = 0; w < warp; ++w) before += sh.warp_count[w];
-      uint32_t* keys = cluster.map_shared_rank(list_key, 0);
-      uint32_t* idxs = cluster.map_shared_rank(list_idx, 0);
-      for (int s0 = w0; s0 < w1; s0 += 128) {
-        float f[4];
-        load4(s0 + lane * 4, f);
-        uint32_t here = 0;
+    if (tid == 0) sh.count = here_all;
+    if (mine != 0 && here_all <= uint32_t(kList)) {
+      for (int s0 = w0; s0 < w1; s0 += kStep) {
+        float f[VEC];
+        load(s0 + lane * VEC, f);
+        uint32_t bits = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) here |= remains(f[j]) ? 1u << j : 0u;
-        if (__ballot_sync(0xffffffffu, here != 0) == 0) continue;
-        const uint32_t incl = warp_scan(uint32_t(__popc(here)), lane);
-        uint32_t at = before + incl - __popc(here);
+        for (int j = 0; j < VEC; ++j) bits |= in(sc.z(f[j])) ? 1u << j : 0u;
+        if (__ballot_sync(0xffffffffu, bits != 0) == 0) continue;
+        const uint32_t incl = warp_scan(uint32_t(__popc(bits)), lane);
+        uint32_t at = before + incl - __popc(bits);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (here >> j & 1u) {
-            keys[at] = key_of(sc.z(f[j]));
-            idxs[at] = uint32_t(first + s0 + lane * 4 + j);
-            ++at;
-          }
+        for (int j = 0; j < VEC; ++j) {
+          if (bits >> j & 1u)
+            list[at++] = (uint64_t(key_of(sc.z(f[j]))) << 32) | uint32_t(first + s0 + lane * VEC + j);
         }
         before += __shfl_sync(0xffffffffu, incl, 31);
       }
     }
     cluster.sync();
-  }
-
-  if (listed) {
-    if (rank != 0) return;  // CTA 0 reads only its own memory from here on
-    const int n = int(n_all);
-    int np = 32;
-    while (np < n) np <<= 1;
-    for (int i = tid; i < np; i += kThreads)
-      sorted[i] = i < n ? (uint64_t(list_key[i]) << 32) | uint32_t(i) : ~0ull;
-    __syncthreads();
-    for (int size = 2; size <= np; size <<= 1) {
-      for (int stride = size >> 1; stride > 0; stride >>= 1) {
-        for (int p = tid; p < np / 2; p += kThreads) {
-          const int i = (p / stride) * stride * 2 + (p & (stride - 1)), j = i + stride;
-          const bool up = (i & size) == 0;
-          const unsigned long long x = sorted[i], y = sorted[j];
-          if ((x > y) == up) {
-            sorted[i] = y;
-            sorted[j] = x;
-          }
-        }
-        __syncthreads();
+    uint32_t n_all = 0;
+    for (int c = 0; c < C; ++c) n_all += cluster.map_shared_rank(&sh, c)->count;
+    if (n_all <= uint32_t(kList) && rank == 0) {
+      uint32_t at = sh.count;
+      for (int c = 1; c < C; ++c) {
+        const uint32_t n = cluster.map_shared_rank(&sh, c)->count;
+        const unsigned long long* from = cluster.map_shared_rank(list, c);
+        for (uint32_t i = tid; i < n; i += kThreads) list[at + i] = from[i];
+        at += n;
       }
     }
-    // falling z: the weights' running sums, four neighbours a thread
-    constexpr int kPer = kList / kThreads;
-    unsigned long long w[kPer], sum = 0;
+    cluster.sync();
+    return n_all;
+  };
+  // CTA 0: the first n list entries sorted into `to`, padded to a power of two (returned).
+  auto sort_list = [&](unsigned long long* to, int n) -> int {
+    int np = 32;
+    while (np < n) np <<= 1;
+    for (int i = tid; i < np; i += kThreads) to[i] = i < n ? list[i] : ~0ull;
+    __syncthreads();
+    sort_entries(to, np);
+    return np;
+  };
+  // CTA 0: draws from the list, which holds all that can be drawn, and writes the row's result.
+  auto draw_from_list = [&](int n) {
+    sort_list(sorted, n);
+    // falling z: the weights' running sums, kPer neighbours a thread
+    unsigned long long w[kPer], sum = 0, run, none;
+    uint32_t zero;
     float e[kPer];
     const int n_k = use_k ? min(k, n) : n;  // entries top-k leaves
 #pragma unroll
@@ -488,164 +465,210 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a) {
       w[j] = weight(e[j]);
       sum += w[j];
     }
-    unsigned long long run = warp_scan(sum, lane);
-    if (lane == 31) sh.warp_mass[warp] = run;
+    scan_pair(sh, 0u, sum, zero, run);
+    if (tid == kThreads - 1) sh.found_m = run;
     __syncthreads();
-    unsigned long long whole = 0;
-    for (int x = 0; x < kWarps; ++x) {
-      const unsigned long long m = sh.warp_mass[x];
-      run += x < warp ? m : 0;
-      whole += m;
-    }
+    // without top-k the list may be the row's upper part only: its whole mass is `total`
+    const unsigned long long need = use_p ? mass_needed(top_p, use_k ? sh.found_m : total) : ~0ull;
     run -= sum;
-    // without top-k the list may be the row's upper part only, so its whole mass is `total`
-    const unsigned long long need = use_p ? mass_needed(top_p, use_k ? whole : total) : ~0ull;
     uint32_t kept = 0;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       kept += tid * kPer + j < n_k && run < need && !(e[j] < min_p) ? 1u : 0u;
       run += w[j];
     }
-    kept = __reduce_add_sync(0xffffffffu, kept);
-    if (lane == 0) sh.warp_count[warp] = kept;
+    scan_pair(sh, kept, 0ull, kept, none);
+    if (tid == kThreads - 1) sh.found = kept;
     __syncthreads();
-    kept = 0;
-    for (int x = 0; x < kWarps; ++x) kept += sh.warp_count[x];
-    const unsigned long long cut = sorted[kept - 1];  // the entry with z = 0 always stays
-    __syncthreads();
+    const unsigned long long cut = sorted[sh.found - 1];  // the entry with z = 0 always stays
     // rising index: the kept weights' running sum, and the first to pass the target
     sum = 0;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       const int i = tid * kPer + j;
-      const bool in = i < n && ((uint64_t(list_key[i]) << 32) | uint32_t(i)) <= cut;
-      w[j] = in ? weight(expf(z_of(list_key[i]))) : 0;
+      w[j] = i < n && list[i] <= cut ? weight(expf(z_of(uint32_t(list[i] >> 32)))) : 0;
       sum += w[j];
     }
-    run = warp_scan(sum, lane);
-    if (lane == 31) sh.warp_mass[warp] = run;
+    scan_pair(sh, 0u, sum, zero, run);
+    if (tid == kThreads - 1) sh.found_m = run;
     __syncthreads();
-    whole = 0;
-    for (int x = 0; x < kWarps; ++x) {
-      const unsigned long long m = sh.warp_mass[x];
-      run += x < warp ? m : 0;
-      whole += m;
-    }
+    const unsigned long long whole = sh.found_m, target = draw_target(u, whole);
     run -= sum;
-    const unsigned long long target = draw_target(u, whole);
     if (run <= target && target < run + sum) {
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
         if (run <= target && target < run + w[j]) {
-          const int i = tid * kPer + j;
-          a.tokens[row] = int64_t(list_idx[i]);
-          if (a.logprobs) a.logprobs[row] = z_of(list_key[i]) - logf(float(double(whole) / double(kUnit)));
+          const unsigned long long it = list[tid * kPer + j];
+          a.tokens[row] = int64_t(uint32_t(it));
+          if (a.logprobs) a.logprobs[row] = z_of(uint32_t(it >> 32)) - logf(float(double(whole) / double(kUnit)));
         }
         run += w[j];
       }
     }
-    return;
-  }
+  };
+  auto list_up_to = [&](int bin) -> bool {  // true: the row is done
+    const float end = float(bin + 1);
+    const uint32_t n = collect([&](float z) { return bin_of(z) < end; });
+    if (n > uint32_t(kList)) return false;
+    if (rank == 0) draw_from_list(int(n));  // from CTA 0's memory alone
+    return true;
+  };
+  if (last_bin >= 0 && list_up_to(last_bin)) return;
 
-  // ---- the cut by a radix search: entries with key < cut_key stay, and of those equal to it the first
-  // `cut_ties` by index
-  uint32_t cut_key = kDead, cut_ties = 0xffffffffu;
+  uint32_t cut_key = kDead, cut_ties = 0xffffffffu;  // entries below the key stay, and of those at it the first ties
   if (use_k || use_p) {
-    unsigned long long goal = use_k ? (unsigned long long)k : mass_needed(top_p, total);
-    bool by_count = use_k;
-    for (int search = 0; search < 2; ++search) {
-      if (search == 1 && !(use_k && use_p)) break;
-      uint32_t prefix = 0;
-      unsigned long long below_n = 0, below_m = 0;  // entries and mass with smaller keys than `prefix`
-      for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = tid; i < kDigits; i += kThreads) {
-          sh.hist_count[i] = 0;
-          sh.hist_mass[i] = 0;
-        }
-        __syncthreads();
-        const uint32_t high = shift == 24 ? 0u : ~0u << (shift + 8);
-        for (int s = w0 + lane * 4; s < w1; s += 128) {
-          float f[4];
-          load4(s, f);
+    // One histogram over the cluster: this thread's bin, and the running sums up to and with it.
+    auto histogram = [&](auto bin, uint32_t& n, unsigned long long& m, uint32_t& cum_n, unsigned long long& cum_m) {
+      sh.bin_count[tid] = sh.bin_lo[tid] = sh.bin_hi[tid] = 0;
+      __syncthreads();
+      for (int s = w0 + lane * VEC; s < w1; s += kStep) {
+        float f[VEC];
+        load(s, f);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int i = first + s + j;
-            const float z = sc.z(f[j]);
-            const uint32_t key = key_of(z);
-            if (i >= 0 && i < a.vocab && (key & high) == prefix) {
-              const uint32_t d = (key >> shift) & 255u;
-              atomicAdd(&sh.hist_count[d], 1u);
-              const uint32_t w = weight(expf(z));
-              if (w != 0) atomicAdd(&sh.hist_mass[d], (unsigned long long)w);
-            }
+        for (int j = 0; j < VEC; ++j) {
+          const float z = sc.z(f[j]);
+          const int b = bin(z);
+          if (b < 0) continue;
+          atomicAdd(&sh.bin_count[b], 1u);
+          if (!use_p) continue;
+          const uint32_t w = weight(expf(z));
+          if constexpr (kResident) {
+            atomicAdd(&sh.bin_lo[b], w & 0xffffu);
+            atomicAdd(&sh.bin_hi[b], w >> 16);
+          } else {  // parts may be longer: carry by hand
+            const uint32_t old = atomicAdd(&sh.bin_lo[b], w);
+            if (old + w < old) atomicAdd(&sh.bin_hi[b], 1u);
           }
         }
-        cluster.sync();
-        if (warp < kDigits / 32) {  // bins over the cluster, running sums over the digits
-          unsigned long long m = 0;
-          uint32_t n = 0;
-          for (int c = 0; c < C; ++c) {
-            const Shared* o = cluster.map_shared_rank(&sh, c);
-            n += o->hist_count[tid];
-            m += o->hist_mass[tid];
-          }
-          const uint32_t ns = warp_scan(n, lane);
-          const unsigned long long ms = warp_scan(m, lane);
-          cluster.sync();  // everyone has read the bins
-          sh.hist_count[tid] = ns;
-          sh.hist_mass[tid] = ms;
-        } else {
-          cluster.sync();
-        }
-        __syncthreads();
-        if (tid == 0) {  // the first digit whose running sum reaches the goal
-          unsigned long long n = below_n, m = below_m;
-          int d = 0;
-          bool found = false;
-          for (int w = 0; w < kDigits / 32 && !found; ++w) {
-            const unsigned long long wn = sh.hist_count[w * 32 + 31], wm = sh.hist_mass[w * 32 + 31];
-            if ((by_count ? n + wn : m + wm) >= goal) {
-              unsigned long long pn = 0, pm = 0;
-              for (d = w * 32; d < w * 32 + 31; ++d) {
-                const unsigned long long dn = sh.hist_count[d], dm = sh.hist_mass[d];
-                if ((by_count ? n + dn : m + dm) >= goal) break;
-                pn = dn;
-                pm = dm;
-              }
-              n += pn;
-              m += pm;
-              found = true;
-            } else {
-              n += wn;
-              m += wm;
-            }
-          }
-          if (!found) d = kDigits - 1;
-          sh.r0 = uint32_t(d);
-          sh.r2 = n;
-          sh.r3 = m;
-        }
-        __syncthreads();
-        prefix |= sh.r0 << shift;
-        below_n = sh.r2;
-        below_m = sh.r3;
-        __syncthreads();
       }
-      const unsigned long long w = weight(expf(z_of(prefix)));
-      unsigned long long ties;
-      if (by_count) ties = goal - below_n;
-      else ties = w != 0 ? (goal - below_m + w - 1) / w : 0xffffffffull;
-      if (ties > 0xffffffffull) ties = 0xffffffffull;
-      // a nucleus lies within the top k: where both end at one key, the smaller part stays
-      if (search == 1 && prefix == cut_key && ties > cut_ties) ties = cut_ties;
-      cut_key = prefix;
-      cut_ties = uint32_t(ties);
-      if (search == 0 && use_k && use_p) {
-        goal = mass_needed(top_p, below_m + w * ties);
-        by_count = false;
+      cluster.sync();
+      n = 0;
+      m = 0;
+      for (int c = 0; c < C; ++c) {
+        const Shared* o = cluster.map_shared_rank(&sh, c);
+        n += o->bin_count[tid];
+        m += (unsigned long long)o->bin_lo[tid] + ((unsigned long long)o->bin_hi[tid] << (kResident ? 16 : 32));
+      }
+      scan_pair(sh, n, m, cum_n, cum_m);
+      cluster.sync();  // everyone has read the bins
+    };
+    // The bin whose running sum is the first to reach the goal; what lies before it, and in it.
+    auto find = [&](bool by_count, unsigned long long goal, uint32_t n, unsigned long long m, uint32_t cum_n,
+                    unsigned long long cum_m, unsigned long long& below_n, unsigned long long& below_m, uint32_t& in_n) -> int {
+      const unsigned long long c0 = by_count ? below_n + cum_n - n : below_m + cum_m - m;
+      const unsigned long long c1 = by_count ? below_n + cum_n : below_m + cum_m;
+      __syncthreads();
+      if (c0 < goal && goal <= c1) {
+        sh.found = uint32_t(tid);
+        sh.found_n = n;
+        sh.found_m = below_n + cum_n - n;
+        sh.found_bin_m = below_m + cum_m - m;
+      }
+      __syncthreads();
+      in_n = sh.found_n;
+      below_n = sh.found_m;
+      below_m = sh.found_bin_m;
+      return int(sh.found);
+    };
+    // The exact cut within keys [lo, hi), which hold in_n entries behind below_n entries of mass below_m;
+    // leaves cut_key and cut_ties and returns the mass up to the cut.
+    auto refine = [&](bool by_count, unsigned long long goal, uint32_t lo, uint32_t hi, unsigned long long below_n,
+                      unsigned long long below_m, uint32_t in_n) -> unsigned long long {
+      while (in_n > uint32_t(kList) && hi - lo > 1) {
+        int shift = 0;
+        while ((hi - lo - 1) >> shift >= uint32_t(kBins)) ++shift;
+        uint32_t n, cum_n;
+        unsigned long long m, cum_m;
+        histogram([&](float z) {
+          const uint32_t key = key_of(z);
+          return key >= lo && key < hi ? int((key - lo) >> shift) : -1;
+        }, n, m, cum_n, cum_m);
+        const int b = find(by_count, goal, n, m, cum_n, cum_m, below_n, below_m, in_n);
+        lo += uint32_t(b) << shift;
+        hi = min(hi, lo + (1u << shift));
+      }
+      if (in_n > uint32_t(kList)) {  // one key
+        const unsigned long long w = weight(expf(z_of(lo)));
+        unsigned long long ties = by_count ? goal - below_n : w != 0 ? (goal - below_m + w - 1) / w : 1;
+        ties = min(ties, (unsigned long long)in_n);
+        cut_key = lo;
+        cut_ties = uint32_t(ties);
+        return below_m + w * ties;
+      }
+      collect([&](float z) {
+        const uint32_t key = key_of(z);
+        return key >= lo && key < hi;
+      });
+      if (rank == 0) {  // sorted in place: the part is still needed
+        int np = 32;
+        while (np < int(in_n)) np <<= 1;
+        for (int i = tid; i < np; i += kThreads)
+          if (i >= int(in_n)) list[i] = ~0ull;
+        __syncthreads();
+        sort_entries(list, np);
+        unsigned long long w[kPer], sum = 0, run;
+        uint32_t zero;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          const int i = tid * kPer + j;
+          w[j] = i < int(in_n) ? weight(expf(z_of(uint32_t(list[i] >> 32)))) : 0;
+          sum += w[j];
+        }
+        scan_pair(sh, 0u, sum, zero, run);
+        run = run - sum + below_m;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          const int i = tid * kPer + j;
+          const bool here = by_count ? below_n + i + 1 == goal : run < goal && goal <= run + w[j];
+          run += w[j];
+          if (here && i < int(in_n)) {
+            const uint32_t key = uint32_t(list[i] >> 32);
+            int f = i;  // ties: how many entries of this key lie up to here
+            while (f > 0 && uint32_t(list[f - 1] >> 32) == key) --f;
+            sh.cut_key = key;
+            sh.cut_ties = uint32_t(i - f + 1);
+            sh.cut_mass = run;
+          }
+        }
+      }
+      cluster.sync();
+      const Shared* o = cluster.map_shared_rank(&sh, 0);
+      cut_key = o->cut_key;
+      cut_ties = o->cut_ties;
+      const unsigned long long mass = o->cut_mass;
+      cluster.sync();  // everyone has read the cut
+      return mass;
+    };
+
+    uint32_t n, cum_n, in_n;
+    unsigned long long m, cum_m;
+    histogram([&](float z) {
+      const float b = bin_of(z);
+      return b < float(kBins) ? int(b) : -1;
+    }, n, m, cum_n, cum_m);
+    if (tid == kThreads - 1) {
+      sh.found_n = cum_n;
+      sh.found_m = cum_m;
+    }
+    __syncthreads();
+    total = sh.found_m;
+    use_k = use_k && sh.found_n > uint32_t(k);  // entries past the bins have no weight
+    if (use_k || use_p) {
+      unsigned long long below_n = 0, below_m = 0;
+      const unsigned long long goal = use_k ? (unsigned long long)k : mass_needed(top_p, total);
+      const int b = find(use_k, goal, n, m, cum_n, cum_m, below_n, below_m, in_n);
+      if (below_n + in_n <= (unsigned long long)kList && list_up_to(b)) return;
+      const unsigned long long mass = refine(use_k, goal, bin_edge(b), bin_edge(b + 1), below_n, below_m, in_n);
+      if (use_k && use_p) {
+        const uint32_t k_key = cut_key, k_ties = cut_ties;
+        const unsigned long long need = mass_needed(top_p, mass);
+        below_n = below_m = 0;
+        const int b2 = find(false, need, n, m, cum_n, cum_m, below_n, below_m, in_n);
+        refine(false, need, bin_edge(b2), bin_edge(b2 + 1), below_n, below_m, in_n);
+        // the nucleus lies within the top k: where both end at one key, the smaller part stays
+        if (cut_key == k_key) cut_ties = min(cut_ties, k_ties);
       }
     }
-    cluster.sync();
   }
 
   // ---- walk the row: where this CTA's and this warp's ties begin, then the kept mass
@@ -653,14 +676,11 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a) {
   uint32_t tie0 = 0;
   if (limit_ties) {
     uint32_t mine = 0;
-    for (int s = w0 + lane * 4; s < w1; s += 128) {
-      float f[4];
-      load4(s, f);
+    for (int s = w0 + lane * VEC; s < w1; s += kStep) {
+      float f[VEC];
+      load(s, f);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int i = first + s + j;
-        mine += i >= 0 && i < a.vocab && key_of(sc.z(f[j])) == cut_key ? 1u : 0u;
-      }
+      for (int j = 0; j < VEC; ++j) mine += key_of(sc.z(f[j])) == cut_key ? 1u : 0u;
     }
     mine = __reduce_add_sync(0xffffffffu, mine);
     if (lane == 0) sh.warp_count[warp] = mine;
@@ -674,25 +694,33 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a) {
     for (int c = 0; c < rank; ++c) tie0 += cluster.map_shared_rank(&sh, c)->ties;
     for (int w = 0; w < warp; ++w) tie0 += sh.warp_count[w];
   }
-  // the kept weights of this lane's four slots; advances the warp's tie count
-  auto kept4 = [&](int s, uint32_t& ties, uint32_t* w) {
-    float f[4];
-    load4(s, f);
-    uint32_t key[4], tie = 0;
+  // the kept weights of this lane's slots (an entry without weight is never kept); advances the warp's tie count
+  auto kept = [&](int s, uint32_t& ties, uint32_t* w) -> unsigned long long {
+    float f[VEC];
+    load(s, f);
+    unsigned long long sum = 0;
+    if (!limit_ties) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = first + s + j;
-      const float z = sc.z(f[j]), e = expf(z);
-      key[j] = key_of(z);
-      const bool in = i >= 0 && i < a.vocab && key[j] <= cut_key && !(e < min_p);
-      w[j] = in ? weight(e) : 0u;
-      tie |= i >= 0 && i < a.vocab && key[j] == cut_key ? 1u << j : 0u;
+      for (int j = 0; j < VEC; ++j) {
+        const float e = expf(sc.z(f[j]));
+        w[j] = e < min_p ? 0u : weight(e);
+        sum += w[j];
+      }
+      return sum;
     }
-    if (limit_ties && __ballot_sync(0xffffffffu, tie != 0) != 0) {
+    uint32_t tie = 0;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const float z = sc.z(f[j]), e = expf(z);
+      const uint32_t key = key_of(z);
+      w[j] = key > cut_key || e < min_p ? 0u : weight(e);
+      tie |= key == cut_key ? 1u << j : 0u;
+    }
+    if (__ballot_sync(0xffffffffu, tie != 0) != 0) {
       const uint32_t incl = warp_scan(uint32_t(__popc(tie)), lane);
       uint32_t at = ties + incl - __popc(tie);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < VEC; ++j) {
         if (tie >> j & 1u) {
           if (at >= cut_ties) w[j] = 0;
           ++at;
@@ -700,14 +728,16 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a) {
       }
       ties += __shfl_sync(0xffffffffu, incl, 31);
     }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) sum += w[j];
+    return sum;
   };
   {
     unsigned long long sum = 0;
     uint32_t ties = tie0;
-    for (int s0 = w0; s0 < w1; s0 += 128) {
-      uint32_t w[4];
-      kept4(s0 + lane * 4, ties, w);
-      sum += (unsigned long long)w[0] + w[1] + w[2] + w[3];
+    for (int s0 = w0; s0 < w1; s0 += kStep) {
+      uint32_t w[VEC];
+      sum += kept(s0 + lane * VEC, ties, w);
     }
     sum = warp_sum(sum);
     if (lane == 0) sh.warp_mass[warp] = sum;
@@ -729,17 +759,16 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a) {
   for (int w = 0; w < warp; ++w) before += sh.warp_mass[w];
   if (before <= target && target < before + sh.warp_mass[warp]) {
     uint32_t ties = tie0;
-    for (int s0 = w0; s0 < w1; s0 += 128) {
-      uint32_t w[4];
-      kept4(s0 + lane * 4, ties, w);
-      const unsigned long long sum = (unsigned long long)w[0] + w[1] + w[2] + w[3];
+    for (int s0 = w0; s0 < w1; s0 += kStep) {
+      uint32_t w[VEC];
+      const unsigned long long sum = kept(s0 + lane * VEC, ties, w);
       const unsigned long long incl = warp_scan(sum, lane);
       unsigned long long run = before + incl - sum;
       if (run <= target && target < run + sum) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < VEC; ++j) {
           if (run <= target && target < run + w[j]) {
-            const int i = first + s0 + lane * 4 + j;
+            const int i = first + s0 + lane * VEC + j;
             a.tokens[row] = i;
             if (a.logprobs) {
               const float z = sc.z(no_nan(Logit<T>::one(base + int64_t(i) * int64_t(sizeof(T)))));
@@ -829,19 +858,20 @@ AUGUR_KV_EXPORT int augur_kv_sample(const void* logits, int64_t row_stride, int3
   a.tokens = tokens;
   a.logprobs = logprobs;
   // CTAs per row: as many as keep the GPU's resident CTAs (two an SM) busy, at
-  // least enough for the row to fit their shared memory, and parts of at
+  // least enough for two parts to fit an SM's shared memory, and parts of at
   // least 2,048 entries
   const int vec = 16 / es;
   constexpr size_t kMost = 200 * 1024;  // of the 227 KB a CTA may have
-  auto bytes = [&](int c) {
+  auto bytes = [&](int c) {  // the list, and the part or (CTA 0, if larger) the sorted list over it
     const int64_t granules = ((int64_t(vocab) + vec - 1) / vec + 1 + c - 1) / c;
-    const size_t part = size_t(granules) * size_t(vec) * 4;
+    const size_t part = size_t(granules) * 16;
     return size_t(kList) * 8 + (part > size_t(kList) * 8 ? part : size_t(kList) * 8);
   };
   const int64_t slots = int64_t(augur_kv_dev::sm_count()) * 2;
   int c = 1;
   while (c < kMaxCluster && (bytes(c) > kMost / 2 || (int64_t(rows) * c * 2 <= slots * 2 && vocab / (c * 2) >= 2048))) c *= 2;
-  const bool resident = bytes(c) <= kMost;
+  // masses are added in halves of 16 bits: a part has at most 65,536 entries
+  const bool resident = bytes(c) <= kMost && (vocab + 2 * vec) / c + vec <= 65536;
   const size_t smem = resident ? bytes(c) : size_t(kList) * 16;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == AUGUR_KV_F32)
