@@ -396,14 +396,14 @@ def _shared_runs(rows: np.ndarray, full: np.ndarray, min_saved: int) -> tuple[li
     return runs, covered
 
 
-def _ranges(tiles: Sequence[int], units: Sequence[int], ctas: int) -> list[int]:
+def _ranges(tiles: Sequence[int], units: Sequence[int], ctas: int, least: int) -> list[int]:
     """Into how many key ranges each run's tiles are cut: tiles[i] key tiles, each range an
     item for each of units[i] (row tiles x KV heads). The ranges are as short as one wave of
-    CTAs (one an SM) allows; where the runs alone exceed a wave, as long as three waves make
-    them, so that the last wave's waste is small."""
+    CTAs (one an SM) allows, but `least` tiles; where the runs alone exceed a wave, as long as
+    three waves make them, so that the last wave's waste is small."""
     total = sum(t * u for t, u in zip(tiles, units))
     waves = 1 if sum(units) <= ctas else 3
-    per = max(2, -(-total // (ctas * waves)))
+    per = max(least, -(-total // (ctas * waves)))
     while waves == 1 and sum(-(-t // per) * u for t, u in zip(tiles, units)) > ctas:
         per += max(1, per // 16)
     return [-(-t // per) for t in tiles]
@@ -445,7 +445,8 @@ class SharedPrefixTables:
         ctas = _sm_count(device)
         row_tiles = [-(-m.size * groups // _TILE_ROWS) for m, _, _ in runs]
         tiles = [-(-(end - start) * bs // _TILE_KEYS) for _, start, end in runs]
-        ranges = _ranges(tiles, [-(-rt // 2) * Hkv for rt in row_tiles], ctas)
+        # a tensor-core item works on two key tiles at a time; the float32 kernel is slower a tile
+        ranges = _ranges(tiles, [-(-rt // 2) * Hkv for rt in row_tiles], ctas, 1 if cache.keys.dtype == torch.float32 else 2)
         items: list[tuple[int, ...]] = []
         refs: list[list[tuple[int, ...]]] = [[] for _ in range(B)]
         member0 = block0 = slab = 0

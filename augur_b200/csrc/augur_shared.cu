@@ -71,6 +71,7 @@ struct Args {
   float scale;  // log2(e) / sqrt(head_dim)
   char* out;
   int64_t out_stride_b, out_stride_h;
+  int32_t out_wide;  // output rows are aligned to four values
   const Item* items;
   int32_t n_items;
   const int32_t* members;
@@ -219,87 +220,133 @@ constexpr int kJoinChunk = 64;  // sources joined at a time
 
 // Joins row parts of `groups` rows and writes the output rows. local_ml / local_o: the
 // n_local own parts, [part][local_rows][2] and [part][local_rows][o_stride] (shared or global
-// memory, stride in floats). smem: groups * (kJoinChunk * 3 + 3) floats. All threads of the CTA call it.
-template <typename T>
-__device__ void join_rows(const Args& a, int b, int hk, int n_local, const float* local_ml, const float* local_o,
-                          int local_rows, int o_stride, float* smem) {
-  const int G = a.groups, D = a.head_dim, n_thr = blockDim.x, tid = threadIdx.x;
+// memory, stride in floats, rows 16-byte aligned with V = 4). smem: join_bytes. All threads call it.
+// A warp takes a row's factors, lanes its sources; then a thread takes V neighbouring dims of a row.
+template <typename T, int V>
+__device__ void join_rows_v(const Args& a, int b, int hk, int n_local, const float* local_ml, const float* local_o,
+                            int local_rows, int o_stride, float* smem) {
+  const int G = a.groups, D = a.head_dim, n_thr = blockDim.x, tid = threadIdx.x, lane = tid & 31;
   const int n_src = n_local + slab_sources(a, b);
-  float* fac = smem;                                                 // [G][kJoinChunk]
-  int64_t* rows = reinterpret_cast<int64_t*>(fac + G * kJoinChunk);  // [G][kJoinChunk]
-  float* run_m = reinterpret_cast<float*>(rows + G * kJoinChunk);    // [G] running reference
-  float* run_l = run_m + G;                                          // [G]
-  float* run_s = run_l + G;                                          // [G] scale of what is joined so far
+  float* fac = smem;                                               // [G][kJoinChunk]
+  int32_t* rows = reinterpret_cast<int32_t*>(fac + G * kJoinChunk);  // [G][kJoinChunk] rows of the source's array
+  float* run_m = reinterpret_cast<float*>(rows + G * kJoinChunk);  // [G] running reference
+  float* run_l = run_m + G;                                        // [G]
+  float* run_s = run_l + G;                                        // [G] scale of what is joined so far
   for (int h = tid; h < G; h += n_thr) {
     run_m[h] = kNegInf;
     run_l[h] = 0.f;
   }
-  constexpr int kMaxVal = 32;  // output values a thread holds: groups * head_dim <= 32 * threads
-  float acc[kMaxVal];
+  constexpr int kMaxVal = 32 / V;  // V-wide values a thread holds: groups * head_dim <= 32 * threads
+  float acc[kMaxVal][V];
 #pragma unroll
-  for (int i = 0; i < kMaxVal; ++i) acc[i] = 0.f;
+  for (int i = 0; i < kMaxVal; ++i)
+#pragma unroll
+    for (int c = 0; c < V; ++c) acc[i][c] = 0.f;
+  const int dv = D / V, tasks = G * dv;
   for (int s0 = 0; s0 < n_src; s0 += kJoinChunk) {
     const int ns = min(kJoinChunk, n_src - s0);
     __syncthreads();
-    for (int i = tid; i < G * ns; i += n_thr) {
-      const int h = i / ns, s = i - h * ns;
-      float m = kNegInf;
-      int64_t row = -1;
-      if (s0 + s < n_local) {
-        row = int64_t(s0 + s) * local_rows + h;
-        m = local_ml[row * 2];
-      } else if (slab_row(a, b, hk, h, s0 + s - n_local, row)) {
-        m = a.slab_ml[row * 2];
+    for (int h = tid >> 5; h < G; h += n_thr >> 5) {
+      float2 ml[kJoinChunk / 32];
+      const float m_old = run_m[h];
+      float m = m_old;
+#pragma unroll
+      for (int i = 0; i < kJoinChunk / 32; ++i) {
+        const int s = lane + 32 * i;
+        ml[i] = make_float2(kNegInf, 0.f);
+        int32_t at = 0;
+        if (s < ns) {
+          int64_t row;
+          if (s0 + s < n_local) {
+            row = int64_t(s0 + s) * local_rows + h;
+            ml[i] = *reinterpret_cast<const float2*>(local_ml + row * 2);
+            at = int32_t(row);
+          } else if (slab_row(a, b, hk, h, s0 + s - n_local, row)) {
+            ml[i] = *reinterpret_cast<const float2*>(a.slab_ml + row * 2);
+            at = int32_t(row);
+          }
+          rows[h * kJoinChunk + s] = at;
+        }
+        m = fmaxf(m, ml[i].x);
       }
-      fac[h * kJoinChunk + s] = m;
-      rows[h * kJoinChunk + s] = row;
-    }
-    __syncthreads();
-    for (int h = tid; h < G; h += n_thr) {
-      float m = run_m[h];
-      for (int s = 0; s < ns; ++s) m = fmaxf(m, fac[h * kJoinChunk + s]);
-      run_s[h] = m == kNegInf ? 0.f : ex2(run_m[h] - m);
-      run_m[h] = m;
-      float l = run_l[h] * run_s[h];
-      for (int s = 0; s < ns; ++s) {
-        const int64_t row = rows[h * kJoinChunk + s];
-        const float f = (m == kNegInf || row < 0) ? 0.f : ex2(fac[h * kJoinChunk + s] - m);
-        if (f != 0.f) l += f * (s0 + s < n_local ? local_ml[row * 2 + 1] : a.slab_ml[row * 2 + 1]);
-        fac[h * kJoinChunk + s] = f;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      float l = 0.f;
+#pragma unroll
+      for (int i = 0; i < kJoinChunk / 32; ++i) {
+        const float f = ml[i].x == kNegInf ? 0.f : ex2(ml[i].x - m);
+        if (lane + 32 * i < ns) fac[h * kJoinChunk + lane + 32 * i] = f;
+        l += f * ml[i].y;
       }
-      run_l[h] = l;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+      __syncwarp();
+      if (lane == 0) {
+        const float scale = m_old == kNegInf ? 0.f : ex2(m_old - m);
+        run_m[h] = m;
+        run_s[h] = scale;
+        run_l[h] = run_l[h] * scale + l;
+      }
     }
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < kMaxVal; ++j) {
       const int i = tid + j * n_thr;
-      if (i >= G * D) break;
-      const int h = i / D, d = i - h * D;
-      float x = 0.f;
-#pragma unroll 4
-      for (int s = 0; s < ns; ++s) {
-        const float f = fac[h * kJoinChunk + s];
-        const int64_t row = rows[h * kJoinChunk + s];
-        // a part with factor 0 (empty, or far below the maximum) is not read
-        if (f != 0.f) x = fmaf(f, s0 + s < n_local ? local_o[row * o_stride + d] : a.slab_o[row * D + d], x);
-      }
-      acc[j] = acc[j] * run_s[h] + x;
+      if (i >= tasks) break;
+      const int h = i / dv, d = (i - h * dv) * V;
+      const float* f = fac + h * kJoinChunk;
+      const int32_t* r = rows + h * kJoinChunk;
+      float x[V];
+#pragma unroll
+      for (int c = 0; c < V; ++c) x[c] = acc[j][c] * run_s[h];
+      const int nl = max(0, min(ns, n_local - s0));
+      auto add = [&](const float* o, float w) {
+        if constexpr (V == 4) {
+          const float4 y = *reinterpret_cast<const float4*>(o);
+          x[0] = fmaf(w, y.x, x[0]);
+          x[1] = fmaf(w, y.y, x[1]);
+          x[2] = fmaf(w, y.z, x[2]);
+          x[3] = fmaf(w, y.w, x[3]);
+        } else {
+          x[0] = fmaf(w, *o, x[0]);
+        }
+      };
+      for (int s = 0; s < nl; ++s) add(local_o + int64_t(r[s]) * o_stride + d, f[s]);
+#pragma unroll 8
+      for (int s = nl; s < ns; ++s) add(a.slab_o + int64_t(r[s]) * D + d, f[s]);
+#pragma unroll
+      for (int c = 0; c < V; ++c) acc[j][c] = x[c];
     }
   }
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < kMaxVal; ++j) {
     const int i = tid + j * n_thr;
-    if (i >= G * D) break;
-    const int h = i / D, d = i - h * D;
-    const float x = acc[j];
+    if (i >= tasks) break;
+    const int h = i / dv, d = (i - h * dv) * V;
     const float l = n_src > 0 ? run_l[h] : 0.f;
-    // no key at all (an empty sequence): zero
-    reinterpret_cast<T*>(a.out + int64_t(b) * a.out_stride_b + int64_t(hk * G + h) * a.out_stride_h)[d] =
-        Elem<T>::from_f(l > 0.f ? x / l : 0.f);
+    const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;  // no key at all: zero; NaN stays
+    T* o = reinterpret_cast<T*>(a.out + int64_t(b) * a.out_stride_b + int64_t(hk * G + h) * a.out_stride_h) + d;
+    struct alignas(V * sizeof(T)) Out {
+      T v[V];
+    } y;
+#pragma unroll
+    for (int c = 0; c < V; ++c) y.v[c] = Elem<T>::from_f(acc[j][c] * inv);
+    if (V == 1 || a.out_wide) {
+      *reinterpret_cast<Out*>(o) = y;
+    } else {
+#pragma unroll
+      for (int c = 0; c < V; ++c) o[c] = y.v[c];
+    }
   }
 }
-__host__ __device__ constexpr int join_bytes(int groups) { return groups * (kJoinChunk * 12 + 12); }
+template <typename T>
+__device__ __forceinline__ void join_rows(const Args& a, int b, int hk, int n_local, const float* local_ml,
+                                          const float* local_o, int local_rows, int o_stride, float* smem) {
+  if ((a.head_dim & 3) == 0) join_rows_v<T, 4>(a, b, hk, n_local, local_ml, local_o, local_rows, o_stride, smem);
+  else join_rows_v<T, 1>(a, b, hk, n_local, local_ml, local_o, local_rows, o_stride, smem);
+}
+__host__ __device__ constexpr int join_bytes(int groups) { return groups * (kJoinChunk * 8 + 12); }
 
 // ---------------------------------------------------------------------------
 // CUDA cores: any type and shape, float32 throughout
@@ -408,8 +455,8 @@ __global__ void __launch_bounds__(kGThreads) shared_generic_kernel(Args a) {
   if (!read_item(a, blockIdx.x, it)) return;
   const int D = a.head_dim, P = generic_pitch(D), tid = threadIdx.x, r = tid >> 2, part = tid & 3;
   const int rows = min(it.slab1 >= 0 ? 2 * kSlabRows : kSlabRows, it.n_rows - it.row0);
-  for (int r0 = 0; r0 < rows; r0 += kGRows) {
-    __syncthreads();
+  const int r0 = int(blockIdx.y) * kGRows;
+  if (r0 < rows) {
     for (int i = tid >> 5; i < kGRows; i += kGThreads / 32) {
       const char* src = r0 + i < rows ? query_row(a, it, it.row0 + r0 + i) : nullptr;
       for (int d = tid & 31; d < D; d += 32)
@@ -479,7 +526,10 @@ __global__ void __launch_bounds__(kGThreads) own_generic_kernel(Args a) {
 // a few rows wide, so they run transposed: S^T = K Q^T and O^T = V^T P^T put the
 // tokens (and dims) on the 16 mma rows and the query heads of the group on
 // the 8 columns. Each of four warps stages 32 tokens of K and V at a time
-// (cp.async, two buffers) and keeps its own running softmax; the CTA joins
+// (cp.async; the next K is fetched behind the scores, the next V behind P V)
+// and keeps its own running softmax. One buffer each rather than two: what
+// hides the latency is the CTAs beside it (3 an SM at head_dim 128, 5 at 64),
+// which also cover each other's starts and joins. The CTA joins
 // the warps, the run's slabs and (for long own parts) the other CTAs' parts,
 // whose last arrival writes the output (it joins them in their order, so the
 // result does not depend on the order of arrival). Bound by HBM: K and V rows are read once.
@@ -511,14 +561,14 @@ template <int D>
 struct OwnCfg {
   static constexpr int kRow = D * 2 + 16;  // padded: ldmatrix rows hit distinct banks
   static constexpr int kTile = kOwnTok * kRow;
-  static constexpr int kBufs = 2;
-  static constexpr int kPipe = kOwnWarps * kBufs * 2 * kTile;
+  static constexpr int kPipe = kOwnWarps * 2 * kTile;
+  static constexpr int kCtas = D == 64 ? 5 : 3;  // resident per SM: 37 or 70 KB each
 };
 // warps' parts [4][heads][2] and [4][heads][D] over the stages, then the join's memory
 __host__ __device__ constexpr int own_parts_bytes(int D, int heads) { return kOwnWarps * heads * (D + 2) * 4; }
 
 template <typename T, int D, int NG>
-__global__ void __launch_bounds__(kOwnThreads) own_mma_kernel(Args a) {
+__global__ void __launch_bounds__(kOwnThreads, OwnCfg<D>::kCtas) own_mma_kernel(Args a) {
   using CF = OwnCfg<D>;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ int last_flag;
@@ -535,24 +585,27 @@ __global__ void __launch_bounds__(kOwnThreads) own_mma_kernel(Args a) {
     last = min(last, first + cut);
   }
   const int n_st = (last - first + kOwnTok - 1) / kOwnTok;
-  unsigned char* mine = smem + warp * CF::kBufs * 2 * CF::kTile;
-  const uint32_t mine_s = smem_u32(mine);
+  const uint32_t ks_ = smem_u32(smem) + warp * 2 * CF::kTile, vs_ = ks_ + CF::kTile;
 
   constexpr int CH = D / 8;  // 16-byte pieces of a row
-  auto load_stage = [&](int st, int buf) {
+  auto row_of = [&](int st) -> int64_t {  // this lane's row of stage st
     const int pos = first + st * kOwnTok + lane;
-    const int64_t off = pos < last ? own_row(a, b, hk, pos) : -1;
+    return pos < last ? own_row(a, b, hk, pos) : -1;
+  };
+  auto fetch = [&](const char* pool, uint32_t dst, int64_t off) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int row = i * (32 / CH) + lane / CH, c = lane % CH;
       const int64_t o = __shfl_sync(0xffffffffu, off, row);
-      const uint32_t dst = mine_s + buf * 2 * CF::kTile + row * CF::kRow + c * 16;
-      cp_async16(dst, a.k + (o >= 0 ? o + c * 16 : 0), o >= 0 ? 16 : 0);
-      cp_async16(dst + CF::kTile, a.v + (o >= 0 ? o + c * 16 : 0), o >= 0 ? 16 : 0);
+      cp_async16(dst + row * CF::kRow + c * 16, pool + (o >= 0 ? o + c * 16 : 0), o >= 0 ? 16 : 0);
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  if (warp < n_st) load_stage(warp, 0);
-  asm volatile("cp.async.commit_group;" ::: "memory");
+  if (warp < n_st) {
+    const int64_t off = row_of(warp);
+    fetch(a.k, ks_, off);
+    fetch(a.v, vs_, off);
+  }
 
   uint32_t qb[NG][D / 16][2];
 #pragma unroll
@@ -574,13 +627,11 @@ __global__ void __launch_bounds__(kOwnThreads) own_mma_kernel(Args a) {
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) o[n][d][0] = o[n][d][1] = o[n][d][2] = o[n][d][3] = 0.f;
   }
-  int buf = 0;
-  for (int st = warp; st < n_st; st += kOwnWarps, buf ^= 1) {
-    if (st + kOwnWarps < n_st) load_stage(st + kOwnWarps, buf ^ 1);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    asm volatile("cp.async.wait_group 1;" ::: "memory");
+  for (int st = warp; st < n_st; st += kOwnWarps) {
+    const bool more = st + kOwnWarps < n_st;
+    const int64_t next = more ? row_of(st + kOwnWarps) : -1;
+    asm volatile("cp.async.wait_group 1;" ::: "memory");  // K
     __syncwarp();
-    const uint32_t ks_ = mine_s + buf * 2 * CF::kTile, vs_ = ks_ + CF::kTile;
     float s[2][NG][4];
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt)
@@ -596,6 +647,8 @@ __global__ void __launch_bounds__(kOwnThreads) own_mma_kernel(Args a) {
         for (int n = 0; n < NG; ++n) Elem<T>::mma(s[mt][n], ka, qb[n][ks][0], qb[n][ks][1]);
       }
     }
+    __syncwarp();
+    if (more) fetch(a.k, ks_, next);
     const int left = last - first - st * kOwnTok;  // tokens of this stage
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
@@ -646,6 +699,9 @@ __global__ void __launch_bounds__(kOwnThreads) own_mma_kernel(Args a) {
         pb[mt][n][0] = transpose8(Elem<T>::pack(s[mt][n][0], s[mt][n][1]));
         pb[mt][n][1] = transpose8(Elem<T>::pack(s[mt][n][2], s[mt][n][3]));
       }
+    if (more) asm volatile("cp.async.wait_group 1;" ::: "memory");  // V; the next K may still be on its way
+    else asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncwarp();
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
@@ -657,9 +713,9 @@ __global__ void __launch_bounds__(kOwnThreads) own_mma_kernel(Args a) {
         for (int n = 0; n < NG; ++n) Elem<T>::mma(o[n][d], va, pb[mt][n][0], pb[mt][n][1]);
       }
     }
-    __syncwarp();  // every lane is done with this buffer before it is filled again
+    __syncwarp();
+    if (more) fetch(a.v, vs_, next);
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
   float* part_ml = reinterpret_cast<float*>(smem);  // [4][H][2]
   float* part_o = part_ml + kOwnWarps * H * 2;      // [4][H][D]
@@ -1284,7 +1340,7 @@ int run_generic(const Args& a, cudaStream_t st) {
   if (a.n_items > 0) {
     const int rc = allow_smem(reinterpret_cast<const void*>(shared_generic_kernel<T>), shared, done_s, "shared_generic_kernel");
     if (rc != AUGUR_KV_OK) return rc;
-    shared_generic_kernel<T><<<unsigned(a.n_items), kGThreads, size_t(shared), st>>>(a);
+    shared_generic_kernel<T><<<dim3(unsigned(a.n_items), 2 * kSlabRows / kGRows), kGThreads, size_t(shared), st>>>(a);
     const int lc = augur_kv_dev::check_launch("shared_generic_kernel");
     if (lc != AUGUR_KV_OK) return lc;
   }
@@ -1378,6 +1434,7 @@ AUGUR_KV_EXPORT int augur_kv_shared_prefix_attention(const augur_kv_shared_prefi
   a.out = static_cast<char*>(out);
   a.out_stride_b = p->out_strides[0] * es;
   a.out_stride_h = p->out_strides[1] * es;
+  a.out_wide = ((reinterpret_cast<uintptr_t>(out) | uintptr_t(a.out_stride_b) | uintptr_t(a.out_stride_h)) & uintptr_t(4 * es - 1)) == 0;
   a.items = reinterpret_cast<const Item*>(p->items);
   a.n_items = p->n_items;
   a.members = p->members;
@@ -1411,7 +1468,7 @@ AUGUR_KV_EXPORT int augur_kv_shared_prefix_attention(const augur_kv_shared_prefi
   const bool tensor = tensor_ok && p->flags != AUGUR_KV_ATTN_GENERIC;
   const int64_t units = int64_t(a.batch) * a.hkv;
   a.n_split = tensor ? own_split(units, p->max_own_len) : 1;
-  {  // scratch: slab sums, slab rows, then the parts'
+  {  // scratch: output rows of the slabs and of the parts, then their maxima and sums
     const int64_t slab_rows = int64_t(a.n_slabs) * kSlabRows;
     const int64_t part_rows = a.n_split > 1 ? units * a.n_split * a.groups : 0;
     if ((slab_rows + part_rows) * (a.head_dim + 2) * 4 + 64 > p->scratch_bytes && slab_rows + part_rows > 0)
@@ -1421,11 +1478,12 @@ AUGUR_KV_EXPORT int augur_kv_shared_prefix_attention(const augur_kv_shared_prefi
     float* f = static_cast<float*>(p->scratch);
     a.slab_o = f;
     f += slab_rows * a.head_dim;
-    a.slab_ml = f;
+    a.split_o = f;
+    f += part_rows * a.head_dim;
+    a.slab_ml = f;  // an even number of floats behind an aligned start: pairs are aligned
     f += slab_rows * 2;
     a.split_ml = f;
-    f += part_rows * 2;
-    a.split_o = f;
+    if (slab_rows + part_rows > 0x7fffffff) return fail(AUGUR_KV_EINVAL, "shared_prefix_attention: too many partial rows");
     a.counters = p->counters;
   }
   if (units * a.n_split > 0x7fffffff) return fail(AUGUR_KV_EINVAL, "shared_prefix_attention: too many sequences");
