@@ -90,11 +90,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "augur_kv_decode_layer": (ctypes.c_int, [_P, _I32, _P, _P, _P, _P, _P]),
     "augur_kv_shared_prefix_attention": (ctypes.c_int, [_P, _I32, _P, _P, _P]),
     "augur_kv_shared_prefix_workspace": (ctypes.c_int, [_I32, _I32, _I32, _I32, _I32, _I32, _I64P, _I64P]),
-    "augur_kv_rope_axes_scatter": (
-        ctypes.c_int,
-        [_P, _I64P, _P, _I64P, _I32, _P, _I64P, _P, _I64P, _I32, _P, _P, _I64P, _I64, _I32, _P, _I64, _P, _I64P,
-         _I32, _P, _P, _I64, _I32, _I32, _P, _P],
-    ),
+    "augur_kv_rope_axes_scatter": (ctypes.c_int, [_P, _I32, _P, _P, _P, _P, _P, _P, _P]),
     "augur_kv_sample": (
         ctypes.c_int,
         [_P, _I64, _I32, _I32, _I32, _P, _P, ctypes.c_float, _P, _I32, _P, ctypes.c_float, _P, ctypes.c_float,
@@ -182,6 +178,35 @@ class SharedPrefixArgs(ctypes.Structure):
         ("scratch_bytes", ctypes.c_int64),
         ("counters", ctypes.c_void_p),
         ("counters_bytes", ctypes.c_int64),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class RopeAxesArgs(ctypes.Structure):
+    """augur_kv_rope_axes_args: what the layers of a several-axis RoPE write share (field for field)."""
+
+    _fields_ = [
+        ("k_pool", ctypes.c_void_p),
+        ("v_pool", ctypes.c_void_p),
+        ("pool_strides", ctypes.c_int64 * 4),
+        ("num_blocks", ctypes.c_int64),
+        ("block_size", ctypes.c_int32),
+        ("n_layers", ctypes.c_int32),
+        ("n_q_heads", ctypes.c_int32),
+        ("n_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("n_tokens", ctypes.c_int64),
+        ("q_strides", ctypes.c_int64 * 2),
+        ("k_strides", ctypes.c_int64 * 2),
+        ("v_strides", ctypes.c_int64 * 2),
+        ("q_out_strides", ctypes.c_int64 * 2),
+        ("slot_stride", ctypes.c_int64),
+        ("position_strides", ctypes.c_int64 * 2),
+        ("inv_freq", ctypes.c_void_p),
+        ("axis_of_frequency", ctypes.c_void_p),
+        ("n_axes", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
         ("status", ctypes.c_void_p),
     ]
 

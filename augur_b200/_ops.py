@@ -95,6 +95,13 @@ class _DeviceGuard:
             torch.cuda.set_device(self.prev)
 
 
+# The current device, and the handle of the current stream on a device, without torch.cuda's
+# lazy-init check and stream object: for callers that already hold tensors on it.
+current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+current_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _ptr(t: Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 

@@ -555,11 +555,6 @@ def _shared_workspace(lib, device: torch.device, st: torch.cuda.Stream, sizes: t
     return cnt, scr
 
 
-_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
-    lambda index: torch.cuda.current_stream(index).cuda_stream)
-
-
 def paged_shared_prefix_attention(
     q: Tensor,
     cache: PagedKVCache,
@@ -587,8 +582,8 @@ def paged_shared_prefix_attention(
     if (fast is not None and out is None and stream is None and kernel == "auto" and fast[0] is cache
             and q.shape == fast[1] and q.stride() == fast[2] and q.dtype is fast[3] and q.get_device() == fast[4]
             and cache.keys.data_ptr() == fast[5] and 0 <= layer_idx < fast[6]
-            and _current_device() == fast[4]):
-        st_raw = _raw_stream(fast[4])
+            and _ops.current_device() == fast[4]):
+        st_raw = _ops.current_raw_stream(fast[4])
         if st_raw == fast[7]:
             res = torch.empty_like(q, memory_format=torch.contiguous_format)
             code = fast[9](fast[8], layer_idx, q.data_ptr(), res.data_ptr(), st_raw)

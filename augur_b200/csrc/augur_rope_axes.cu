@@ -189,68 +189,67 @@ int launch(AxesArgs a, cudaStream_t st) {
 
 #define AUGUR_KV_EXPORT extern "C" __attribute__((visibility("default")))
 
-AUGUR_KV_EXPORT int augur_kv_rope_axes_scatter(
-    const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides, int32_t n_q_heads,
-    const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, int32_t dtype, void* k_pool,
-    void* v_pool, const int64_t* pool_strides, int64_t num_blocks, int32_t block_size, const int64_t* slots,
-    int64_t slot_stride, const int64_t* positions, const int64_t* position_strides, int32_t n_axes,
-    const float* inv_freq, const int32_t* axis_of_frequency, int64_t n_tokens, int32_t n_kv_heads, int32_t head_dim,
-    int32_t* status, void* stream) {
+AUGUR_KV_EXPORT int augur_kv_rope_axes_scatter(const augur_kv_rope_axes_args* p, int32_t layer, const void* q,
+                                               const void* k, const void* v, void* q_out, const int64_t* slots,
+                                               const int64_t* positions, void* stream) {
   using namespace augur_kv_axes;
   using augur_kv_dev::fail;
   augur_kv_dev::g_last_error[0] = '\0';
-  const int es = augur_kv_dev::elem_size(dtype);
-  if (es == 0) return fail(AUGUR_KV_EINVAL, "rope_axes_scatter: unknown dtype %d", dtype);
-  if (n_tokens < 0) return fail(AUGUR_KV_EINVAL, "rope_axes_scatter: negative sizes");
-  if (n_tokens == 0) return AUGUR_KV_OK;
-  if (q == nullptr || q_out == nullptr || k == nullptr || v == nullptr || k_pool == nullptr || v_pool == nullptr ||
-      q_strides == nullptr || q_out_strides == nullptr || k_strides == nullptr || v_strides == nullptr ||
-      pool_strides == nullptr || slots == nullptr || positions == nullptr || position_strides == nullptr ||
-      inv_freq == nullptr || axis_of_frequency == nullptr)
+  if (p == nullptr) return fail(AUGUR_KV_EINVAL, "rope_axes_scatter: null args");
+  if (layer < 0 || layer >= p->n_layers)
+    return fail(AUGUR_KV_EINVAL, "rope_axes_scatter: layer %d outside [0, %d)", layer, p->n_layers);
+  const int es = augur_kv_dev::elem_size(p->dtype);
+  if (es == 0) return fail(AUGUR_KV_EINVAL, "rope_axes_scatter: unknown dtype %d", p->dtype);
+  if (p->n_tokens < 0) return fail(AUGUR_KV_EINVAL, "rope_axes_scatter: negative sizes");
+  if (p->n_tokens == 0) return AUGUR_KV_OK;
+  if (q == nullptr || q_out == nullptr || k == nullptr || v == nullptr || p->k_pool == nullptr ||
+      p->v_pool == nullptr || slots == nullptr || positions == nullptr || p->inv_freq == nullptr ||
+      p->axis_of_frequency == nullptr)
     return fail(AUGUR_KV_EINVAL, "rope_axes_scatter: null pointer argument");
-  if (n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads > 65536 || n_kv_heads > 65536 || head_dim <= 0 ||
-      head_dim % 2 != 0 || head_dim > 1024 || block_size <= 0 || num_blocks <= 0 || n_axes <= 0)
+  if (p->n_q_heads <= 0 || p->n_kv_heads <= 0 || p->n_q_heads > 65536 || p->n_kv_heads > 65536 || p->head_dim <= 0 ||
+      p->head_dim % 2 != 0 || p->head_dim > 1024 || p->block_size <= 0 || p->num_blocks <= 0 || p->n_axes <= 0)
     return fail(AUGUR_KV_EINVAL, "rope_axes_scatter: bad sizes (head_dim even and at most 1024)");
   AxesArgs a;
   memset(&a, 0, sizeof(a));
+  const int64_t layer_bytes = int64_t(layer) * p->pool_strides[0] * es;
   a.q = static_cast<const char*>(q);
   a.q_out = static_cast<char*>(q_out);
   a.k = static_cast<const char*>(k);
   a.v = static_cast<const char*>(v);
-  a.k_pool = static_cast<char*>(k_pool);
-  a.v_pool = static_cast<char*>(v_pool);
+  a.k_pool = static_cast<char*>(p->k_pool) + layer_bytes;
+  a.v_pool = static_cast<char*>(p->v_pool) + layer_bytes;
   uintptr_t bits = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(k) |
-                   reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(k_pool) |
-                   reinterpret_cast<uintptr_t>(v_pool) | uintptr_t(head_dim / 2 * es);
+                   reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(a.k_pool) |
+                   reinterpret_cast<uintptr_t>(a.v_pool) | uintptr_t(p->head_dim / 2 * es);
   for (int i = 0; i < 2; ++i) {
-    a.q_stride[i] = q_strides[i] * es;
-    a.q_out_stride[i] = q_out_strides[i] * es;
-    a.k_stride[i] = k_strides[i] * es;
-    a.v_stride[i] = v_strides[i] * es;
-    a.pos_stride[i] = position_strides[i];
+    a.q_stride[i] = p->q_strides[i] * es;
+    a.q_out_stride[i] = p->q_out_strides[i] * es;
+    a.k_stride[i] = p->k_strides[i] * es;
+    a.v_stride[i] = p->v_strides[i] * es;
+    a.pos_stride[i] = p->position_strides[i];
     bits |= uintptr_t(a.q_stride[i]) | uintptr_t(a.q_out_stride[i]) | uintptr_t(a.k_stride[i]) | uintptr_t(a.v_stride[i]);
   }
   for (int i = 0; i < 3; ++i) {
-    a.pool_stride[i] = pool_strides[i] * es;
+    a.pool_stride[i] = p->pool_strides[i + 1] * es;
     bits |= uintptr_t(a.pool_stride[i]);
   }
   if ((bits & uintptr_t(es - 1)) != 0) return fail(AUGUR_KV_EINVAL, "rope_axes_scatter: pointers must be aligned to the type");
-  a.num_slots = num_blocks * block_size;
-  a.block_size = block_size;
+  a.num_slots = p->num_blocks * p->block_size;
+  a.block_size = p->block_size;
   a.slots = slots;
-  a.slot_stride = slot_stride;
+  a.slot_stride = p->slot_stride;
   a.positions = positions;
-  a.inv_freq = inv_freq;
-  a.axis = axis_of_frequency;
-  a.n_axes = n_axes;
-  a.hq = n_q_heads;
-  a.hkv = n_kv_heads;
-  a.half = head_dim / 2;
-  a.n_tokens = n_tokens;
-  a.status = status;
+  a.inv_freq = p->inv_freq;
+  a.axis = p->axis_of_frequency;
+  a.n_axes = p->n_axes;
+  a.hq = p->n_q_heads;
+  a.hkv = p->n_kv_heads;
+  a.half = p->head_dim / 2;
+  a.n_tokens = p->n_tokens;
+  a.status = p->status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool wide = (bits & 15u) == 0;  // every piece of 16 bytes is aligned; else one element a piece
-  if (dtype == AUGUR_KV_F32) return wide ? launch<float, 4>(a, st) : launch<float, 1>(a, st);
-  if (dtype == AUGUR_KV_F16) return wide ? launch<__half, 8>(a, st) : launch<__half, 1>(a, st);
+  if (p->dtype == AUGUR_KV_F32) return wide ? launch<float, 4>(a, st) : launch<float, 1>(a, st);
+  if (p->dtype == AUGUR_KV_F16) return wide ? launch<__half, 8>(a, st) : launch<__half, 1>(a, st);
   return wide ? launch<__nv_bfloat16, 8>(a, st) : launch<__nv_bfloat16, 1>(a, st);
 }

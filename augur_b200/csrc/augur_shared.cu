@@ -81,11 +81,13 @@ struct Args {
   const int32_t* ref_starts;  // [batch + 1] into refs
   const int4* refs;           // first slab of the run, key ranges, sequence's place in the run, row tiles
   int32_t n_refs, n_slabs;
+  int32_t quads;   // head_dim / 4, rounded up
   float* slab_ml;  // [n_slabs][128][2]
-  float* slab_o;   // [n_slabs][128][head_dim]
+  // [n_slabs][quads][128][4]: a warp's 32 rows of four dims are 512 bytes in a row, written and read whole
+  float* slab_o;
   int32_t n_split;     // parts of a sequence's own keys
   float* split_ml;     // [batch * hkv][n_split][groups][2]
-  float* split_o;      // [batch * hkv][n_split][groups][head_dim]
+  float* split_o;      // [batch * hkv][n_split][groups][4 quads]
   int32_t* counters;   // [batch * hkv], zero between launches
   int32_t* status;
 };
@@ -220,29 +222,28 @@ constexpr int kJoinChunk = 64;  // sources joined at a time
 
 // Joins row parts of `groups` rows and writes the output rows. local_ml / local_o: the
 // n_local own parts, [part][local_rows][2] and [part][local_rows][o_stride] (shared or global
-// memory, stride in floats, rows 16-byte aligned with V = 4). smem: join_bytes. All threads call it.
-// A warp takes a row's factors, lanes its sources; then a thread takes V neighbouring dims of a row.
-template <typename T, int V>
-__device__ void join_rows_v(const Args& a, int b, int hk, int n_local, const float* local_ml, const float* local_o,
-                            int local_rows, int o_stride, float* smem) {
-  const int G = a.groups, D = a.head_dim, n_thr = blockDim.x, tid = threadIdx.x, lane = tid & 31;
+// memory, stride in floats, rows 16-byte aligned and padded to four). smem: join_bytes. All
+// threads call it. A warp takes a row's factors, lanes its sources; then a thread takes four
+// dims of a row (rows fastest, as the slabs lie).
+template <typename T>
+__device__ void join_rows(const Args& a, int b, int hk, int n_local, const float* local_ml, const float* local_o,
+                          int local_rows, int o_stride, float* smem) {
+  const int G = a.groups, n_thr = blockDim.x, tid = threadIdx.x, lane = tid & 31;
   const int n_src = n_local + slab_sources(a, b);
-  float* fac = smem;                                               // [G][kJoinChunk]
-  int32_t* rows = reinterpret_cast<int32_t*>(fac + G * kJoinChunk);  // [G][kJoinChunk] rows of the source's array
-  float* run_m = reinterpret_cast<float*>(rows + G * kJoinChunk);  // [G] running reference
-  float* run_l = run_m + G;                                        // [G]
-  float* run_s = run_l + G;                                        // [G] scale of what is joined so far
+  float* fac = smem;                                                 // [G][kJoinChunk]
+  int32_t* rows = reinterpret_cast<int32_t*>(fac + G * kJoinChunk);  // [G][kJoinChunk] the part's first quad
+  float* run_m = reinterpret_cast<float*>(rows + G * kJoinChunk);    // [G] running reference
+  float* run_l = run_m + G;                                          // [G]
+  float* run_s = run_l + G;                                          // [G] scale of what is joined so far
   for (int h = tid; h < G; h += n_thr) {
     run_m[h] = kNegInf;
     run_l[h] = 0.f;
   }
-  constexpr int kMaxVal = 32 / V;  // V-wide values a thread holds: groups * head_dim <= 32 * threads
-  float acc[kMaxVal][V];
+  constexpr int kMaxVal = 8;  // quads a thread holds: groups * quads <= 8 * threads
+  float4 acc[kMaxVal];
 #pragma unroll
-  for (int i = 0; i < kMaxVal; ++i)
-#pragma unroll
-    for (int c = 0; c < V; ++c) acc[i][c] = 0.f;
-  const int dv = D / V, tasks = G * dv;
+  for (int i = 0; i < kMaxVal; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int tasks = G * a.quads;
   for (int s0 = 0; s0 < n_src; s0 += kJoinChunk) {
     const int ns = min(kJoinChunk, n_src - s0);
     __syncthreads();
@@ -263,7 +264,7 @@ __device__ void join_rows_v(const Args& a, int b, int hk, int n_local, const flo
             at = int32_t(row);
           } else if (slab_row(a, b, hk, h, s0 + s - n_local, row)) {
             ml[i] = *reinterpret_cast<const float2*>(a.slab_ml + row * 2);
-            at = int32_t(row);
+            at = int32_t((row / kSlabRows) * a.quads * kSlabRows + row % kSlabRows);
           }
           rows[h * kJoinChunk + s] = at;
         }
@@ -293,29 +294,27 @@ __device__ void join_rows_v(const Args& a, int b, int hk, int n_local, const flo
     for (int j = 0; j < kMaxVal; ++j) {
       const int i = tid + j * n_thr;
       if (i >= tasks) break;
-      const int h = i / dv, d = (i - h * dv) * V;
+      const int d = i / G, h = i - d * G;
       const float* f = fac + h * kJoinChunk;
       const int32_t* r = rows + h * kJoinChunk;
-      float x[V];
-#pragma unroll
-      for (int c = 0; c < V; ++c) x[c] = acc[j][c] * run_s[h];
-      const int nl = max(0, min(ns, n_local - s0));
+      float4 x = acc[j];
+      x.x *= run_s[h];
+      x.y *= run_s[h];
+      x.z *= run_s[h];
+      x.w *= run_s[h];
       auto add = [&](const float* o, float w) {
-        if constexpr (V == 4) {
-          const float4 y = *reinterpret_cast<const float4*>(o);
-          x[0] = fmaf(w, y.x, x[0]);
-          x[1] = fmaf(w, y.y, x[1]);
-          x[2] = fmaf(w, y.z, x[2]);
-          x[3] = fmaf(w, y.w, x[3]);
-        } else {
-          x[0] = fmaf(w, *o, x[0]);
-        }
+        const float4 y = *reinterpret_cast<const float4*>(o);
+        x.x = fmaf(w, y.x, x.x);
+        x.y = fmaf(w, y.y, x.y);
+        x.z = fmaf(w, y.z, x.z);
+        x.w = fmaf(w, y.w, x.w);
       };
-      for (int s = 0; s < nl; ++s) add(local_o + int64_t(r[s]) * o_stride + d, f[s]);
+      const int nl = max(0, min(ns, n_local - s0));
+      for (int s = 0; s < nl; ++s) add(local_o + int64_t(r[s]) * o_stride + 4 * d, f[s]);
+      const float* slab = a.slab_o + int64_t(d) * (kSlabRows * 4);
 #pragma unroll 8
-      for (int s = nl; s < ns; ++s) add(a.slab_o + int64_t(r[s]) * D + d, f[s]);
-#pragma unroll
-      for (int c = 0; c < V; ++c) acc[j][c] = x[c];
+      for (int s = nl; s < ns; ++s) add(slab + int64_t(r[s]) * 4, f[s]);
+      acc[j] = x;
     }
   }
   __syncthreads();
@@ -323,28 +322,25 @@ __device__ void join_rows_v(const Args& a, int b, int hk, int n_local, const flo
   for (int j = 0; j < kMaxVal; ++j) {
     const int i = tid + j * n_thr;
     if (i >= tasks) break;
-    const int h = i / dv, d = (i - h * dv) * V;
+    const int d = i / G, h = i - d * G;
     const float l = n_src > 0 ? run_l[h] : 0.f;
     const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;  // no key at all: zero; NaN stays
-    T* o = reinterpret_cast<T*>(a.out + int64_t(b) * a.out_stride_b + int64_t(hk * G + h) * a.out_stride_h) + d;
-    struct alignas(V * sizeof(T)) Out {
-      T v[V];
+    T* o = reinterpret_cast<T*>(a.out + int64_t(b) * a.out_stride_b + int64_t(hk * G + h) * a.out_stride_h) + 4 * d;
+    struct alignas(4 * sizeof(T)) Out {
+      T v[4];
     } y;
-#pragma unroll
-    for (int c = 0; c < V; ++c) y.v[c] = Elem<T>::from_f(acc[j][c] * inv);
-    if (V == 1 || a.out_wide) {
+    y.v[0] = Elem<T>::from_f(acc[j].x * inv);
+    y.v[1] = Elem<T>::from_f(acc[j].y * inv);
+    y.v[2] = Elem<T>::from_f(acc[j].z * inv);
+    y.v[3] = Elem<T>::from_f(acc[j].w * inv);
+    if (a.out_wide) {
       *reinterpret_cast<Out*>(o) = y;
     } else {
 #pragma unroll
-      for (int c = 0; c < V; ++c) o[c] = y.v[c];
+      for (int c = 0; c < 4; ++c)
+        if (4 * d + c < a.head_dim) o[c] = y.v[c];
     }
   }
-}
-template <typename T>
-__device__ __forceinline__ void join_rows(const Args& a, int b, int hk, int n_local, const float* local_ml,
-                                          const float* local_o, int local_rows, int o_stride, float* smem) {
-  if ((a.head_dim & 3) == 0) join_rows_v<T, 4>(a, b, hk, n_local, local_ml, local_o, local_rows, o_stride, smem);
-  else join_rows_v<T, 1>(a, b, hk, n_local, local_ml, local_o, local_rows, o_stride, smem);
 }
 __host__ __device__ constexpr int join_bytes(int groups) { return groups * (kJoinChunk * 8 + 12); }
 
@@ -478,11 +474,12 @@ __global__ void __launch_bounds__(kGThreads) shared_generic_kernel(Args a) {
     if (row < rows) {
       const int64_t at = int64_t(row < kSlabRows ? it.slab0 : it.slab1) * kSlabRows + (row & (kSlabRows - 1));
       if (part == 0) *reinterpret_cast<float2*>(a.slab_ml + at * 2) = make_float2(m, l);
+      const int64_t quad = (at / kSlabRows) * a.quads * kSlabRows + at % kSlabRows;
 #pragma unroll
       for (int i = 0; i < kGMaxDim / 16; ++i)
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if (16 * i + 4 * part + c < D) a.slab_o[at * D + 16 * i + 4 * part + c] = o[4 * i + c];
+        if (4 * i + part < a.quads)
+          *reinterpret_cast<float4*>(a.slab_o + (quad + int64_t(4 * i + part) * kSlabRows) * 4) =
+              make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
     }
   }
 }
@@ -510,9 +507,9 @@ __global__ void __launch_bounds__(kGThreads) own_generic_kernel(Args a) {
     }
 #pragma unroll
     for (int i = 0; i < kGMaxDim / 16; ++i)
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (16 * i + 4 * part + c < D) gsm[r * P + 16 * i + 4 * part + c] = o[4 * i + c];
+      if (4 * i + part < a.quads)
+        *reinterpret_cast<float4*>(gsm + r * P + 16 * i + 4 * part) =
+            make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
   }
   wait_prerequisites();  // the shared launch's slabs
   join_rows<T>(a, b, hk, 1, ml, gsm, kGRows, P, ml + 2 * kGRows);
@@ -564,8 +561,8 @@ struct OwnCfg {
   static constexpr int kPipe = kOwnWarps * 2 * kTile;
   static constexpr int kCtas = D == 64 ? 5 : 3;  // resident per SM: 37 or 70 KB each
 };
-// warps' parts [4][heads][2] and [4][heads][D] over the stages, then the join's memory
-__host__ __device__ constexpr int own_parts_bytes(int D, int heads) { return kOwnWarps * heads * (D + 2) * 4; }
+// warps' parts [4][heads][2] and [4][heads][D + 4] over the stages, then the join's memory
+__host__ __device__ constexpr int own_parts_bytes(int D, int heads) { return kOwnWarps * heads * (D + 6) * 4; }
 
 template <typename T, int D, int NG>
 __global__ void __launch_bounds__(kOwnThreads, OwnCfg<D>::kCtas) own_mma_kernel(Args a) {
@@ -718,7 +715,8 @@ __global__ void __launch_bounds__(kOwnThreads, OwnCfg<D>::kCtas) own_mma_kernel(
   }
   __syncthreads();
   float* part_ml = reinterpret_cast<float*>(smem);  // [4][H][2]
-  float* part_o = part_ml + kOwnWarps * H * 2;      // [4][H][D]
+  float* part_o = part_ml + kOwnWarps * H * 2;      // [4][H][P]
+  constexpr int P = D + 4;  // neighbouring rows start four banks apart
 #pragma unroll
   for (int n = 0; n < NG; ++n) {
 #pragma unroll
@@ -734,16 +732,16 @@ __global__ void __launch_bounds__(kOwnThreads, OwnCfg<D>::kCtas) own_mma_kernel(
       }
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) {
-        part_o[(warp * H + h) * D + d * 16 + g] = o[n][d][c];
-        part_o[(warp * H + h) * D + d * 16 + g + 8] = o[n][d][c + 2];
+        part_o[(warp * H + h) * P + d * 16 + g] = o[n][d][c];
+        part_o[(warp * H + h) * P + d * 16 + g + 8] = o[n][d][c + 2];
       }
     }
   }
-  float* join_mem = part_o + kOwnWarps * H * D;
+  float* join_mem = part_o + kOwnWarps * H * P;
   __syncthreads();
   if (a.n_split == 1) {
     wait_prerequisites();  // the shared launch's slabs
-    join_rows<T>(a, b, hk, kOwnWarps, part_ml, part_o, H, D, join_mem);
+    join_rows<T>(a, b, hk, kOwnWarps, part_ml, part_o, H, P, join_mem);
     return;
   }
   // this CTA's part to scratch; the last CTA of the unit to arrive joins them all
@@ -757,7 +755,7 @@ __global__ void __launch_bounds__(kOwnThreads, OwnCfg<D>::kCtas) own_mma_kernel(
     for (int w = 0; w < kOwnWarps; ++w) {
       const float f = m == kNegInf ? 0.f : ex2(part_ml[(w * H + h) * 2] - m);
       l += f * part_ml[(w * H + h) * 2 + 1];
-      x += f * part_o[(w * H + h) * D + d];
+      x += f * part_o[(w * H + h) * P + d];
     }
     a.split_o[(base + h) * D + d] = x;
     if (d == 0) *reinterpret_cast<float2*>(a.split_ml + (base + h) * 2) = make_float2(m, l);
@@ -786,20 +784,24 @@ __global__ void __launch_bounds__(kOwnThreads, OwnCfg<D>::kCtas) own_mma_kernel(
 // (TMA, one box per block and 64 dims, 128-byte swizzle; keys past the range
 // and bad block ids take an out-of-range block coordinate, which TMA fills
 // with zeros), warp 9 issues the products. Per tile: S = Q K^T into tensor
-// memory (M = N = 128), each thread loads its row of S, takes the running
-// maximum, writes P = 2^(x - m) in the cache type over S, and O += P V takes
-// P as the operand in tensor memory and accumulates there. O is rescaled only
-// when a row's maximum has grown by more than 2^8 over the reference its
-// exponents use (P then stays below 2^8, and the float32 sums do not care),
-// so most tiles touch it not at all. The groups work on the same keys with
-// different rows (`pair`: a run with over 128 rows reads its keys once for
-// 256), or on the same rows with even and odd key tiles, whose results are
-// joined in shared memory. While one group's softmax runs, the tensor core
-// works for the other.
+// memory (M = N = 128); each thread takes its row of S 32 columns at a time,
+// P = 2^(x - m) in the cache type goes back to tensor memory 64 keys at a time, and
+// O += P V takes P as its operand there and accumulates in tensor memory.
+// m is a reference, not the maximum: the exponentials of 64 keys are taken with
+// the reference so far while their maximum is looked for, and only where that
+// has passed the reference by more than 2^8 are they taken again with a new
+// one, and O and the sum rescaled (P stays below 2^8, and the float32 sums do
+// not care). The groups work on the same keys with different rows (`pair`: a
+// run with over 128 rows reads its keys once for 256), or on the same rows
+// with even and odd key tiles, whose results are joined in shared memory.
+// While one group's softmax runs, the tensor core works for the other. At
+// head_dim 64 P has columns of its own, so the next tile's S is computed
+// while this tile's exponentials are; at 128 P lies over S.
 //
 // Bound by the 16 exponentials a clock an SM has: a 256 x 128 tile needs 2,048
-// clocks of them, its products 1,024 (head_dim 64) or 2,048 (128). With few
-// rows it is bound by HBM instead.
+// clocks of them, its products 1,024 (head_dim 64) or 2,048 (128). So every
+// second pair (head_dim 64), or every fourth (128), is computed on the FMA
+// pipes instead (exp2_poly2). With few rows it is bound by HBM.
 //
 // Every wait is bounded (2 s of %globaltimer); on expiry the CTA records
 // AUGUR_KV_ETIMEOUT, drains its copies and products, frees its tensor memory and returns.
@@ -818,7 +820,10 @@ struct ShCfg {
   static constexpr int kV = kK + kKBufs * kTileBytes;
   static constexpr int kBar = kV + kVBufs * kTileBytes;
   static constexpr int kBytes = kBar + 256 + 1024;  // and the alignment of the first tile
-  static constexpr uint32_t kS = 0, kO = 256, kCols = 512;  // tensor memory: S0, S1 (P over them), O0, O1
+  // tensor memory: S0, S1, then O0, O1 (and P0, P1; at head_dim 128 P lies over S)
+  static constexpr bool kOwnP = D == 64;
+  static constexpr uint32_t kS = 0, kO = 256, kP = kOwnP ? 256 + 2 * D : 0, kPStep = kOwnP ? 64 : 128, kCols = 512;
+  static constexpr int kPolyEvery = D == 64 ? 2 : 4;  // of so many pairs, one goes to the FMA pipes
 };
 
 __device__ __forceinline__ uint64_t global_ns() {
@@ -919,8 +924,53 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// The wait names the registers of the load it waits for, so that nothing that reads them moves ahead of it.
+__device__ __forceinline__ void tmem_wait_ld32(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Two float32 operations at a time.
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// 2^x and 2^y on the FMA pipes, for arguments at most 127 (below -126: 2^-126, a weight of nothing):
+// 2^x = 2^n 2^f with n = round(x) (the low bits of x + 1.5 2^23) and f in [-1/2, 1/2], and for 2^f the
+// polynomial of degree 4 whose largest relative error there is smallest (2.6e-6; found by exchange).
+__device__ __forceinline__ uint64_t exp2_poly2(float x, float y) {
+  const uint64_t v = pack2(fmaxf(x, -126.f), fmaxf(y, -126.f));
+  const uint64_t t = add2(v, pack2(12582912.f, 12582912.f));
+  const uint64_t n = add2(t, pack2(-12582912.f, -12582912.f));
+  const uint64_t f = fma2(n, pack2(-1.f, -1.f), v);
+  uint64_t p = fma2(f, pack2(0.009570102207362652f, 0.009570102207362652f), pack2(0.05591785907745361f, 0.05591785907745361f));
+  p = fma2(p, f, pack2(0.240247443318367f, 0.240247443318367f));
+  p = fma2(p, f, pack2(0.6931217908859253f, 0.6931217908859253f));
+  p = fma2(p, f, pack2(0.9999992847442627f, 0.9999992847442627f));
+  float p0, p1, t0, t1;
+  unpack2(p, p0, p1);
+  unpack2(t, t0, t1);
+  return pack2(__uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23)),
+               __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23)));
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kShThreads, 1)
@@ -945,28 +995,69 @@ __global__ void __launch_bounds__(kShThreads, 1)
   auto v_empty = [&](int i) { return bars + 8u * uint32_t(2 * CF::kKBufs + CF::kVBufs + i); };
   const uint32_t rest = bars + 8u * uint32_t(2 * CF::kKBufs + 2 * CF::kVBufs);
   auto s_full = [&](int i) { return rest + 8u * uint32_t(i); };
-  auto p_full = [&](int i) { return rest + 16u + 8u * uint32_t(i); };
-  auto o_done = [&](int i) { return rest + 32u + 8u * uint32_t(i); };
-  const uint32_t drain = rest + 48u;
-  static_assert(8 * (2 * CF::kKBufs + 2 * CF::kVBufs + 7) <= 256, "barriers");
+  auto s_free = [&](int i) { return rest + 16u + 8u * uint32_t(i); };
+  // a barrier for each half of a tile: neither side is ever more than a phase ahead of the other's look at it
+  auto p_full = [&](int i, int half) { return rest + 32u + 16u * uint32_t(i) + 8u * uint32_t(half); };
+  auto o_done = [&](int i, int half) { return rest + 64u + 16u * uint32_t(i) + 8u * uint32_t(half); };
+  const uint32_t drain = rest + 96u;
+  static_assert(8 * (2 * CF::kKBufs + 2 * CF::kVBufs + 13) <= 256, "barriers");
 
-  if (tid == 0) {
-    for (int i = 0; i < CF::kKBufs; ++i) {
-      mbar_init(k_full(i), 1);
-      mbar_init(k_empty(i), 1);
+  // ---- K and V tiles: one box a lane
+  const int bs = a.block_size;
+  const int box = bs < kTileKeys ? bs : kTileKeys;  // rows of a TMA box
+  const int boxes = kTileKeys / box * CF::kHalves;  // boxes of a K or V tile: at most 32
+  auto fetch = [&](int t, bool v) {                 // warp 8; the buffer is free
+    const int j = lane / CF::kHalves, half = lane - j * CF::kHalves;
+    const int pos = it.key0 + t * kTileKeys + j * box;
+    int blk = -1, row = 0;
+    if (lane < boxes && pos < it.key1) {
+      const int lb = pos / bs;
+      row = pos - lb * bs;
+      blk = __ldg(a.run_blocks + it.block0 + lb);
+      if (blk < 0 || blk >= a.num_blocks) {
+        record_status(a.status, AUGUR_KV_EBOUNDS);
+        blk = -1;
+      }
     }
-    for (int i = 0; i < CF::kVBufs; ++i) {
-      mbar_init(v_full(i), 1);
-      mbar_init(v_empty(i), 1);
+    const int at = blk >= 0 ? blk : int(a.num_blocks);  // past the pool: zeros
+    const int buf = t % (v ? CF::kVBufs : CF::kKBufs);
+    const uint32_t full = v ? v_full(buf) : k_full(buf);
+    if (lane == 0) mbar_expect(full, CF::kTileBytes);
+    __syncwarp();
+    if (lane < boxes)
+      tma_box(sb + (v ? CF::kV : CF::kK) + uint32_t(buf) * CF::kTileBytes + uint32_t(half) * (kTileKeys * 128) +
+                  uint32_t(j) * uint32_t(box) * 128u,
+              v ? &v_map : &k_map, full, half * 64, row, it.kv_head, at);
+  };
+  int n_k = min(n_tiles, CF::kKBufs), n_v = min(n_tiles, CF::kVBufs);  // tiles under way (warp 8)
+  if (warp == 8) {
+    if (lane == 0) {
+      for (int i = 0; i < CF::kKBufs; ++i) {
+        mbar_init(k_full(i), 1);
+        mbar_init(k_empty(i), 1);
+      }
+      for (int i = 0; i < CF::kVBufs; ++i) {
+        mbar_init(v_full(i), 1);
+        mbar_init(v_empty(i), 1);
+      }
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(s_full(i), 1);
+        mbar_init(s_free(i), 128);
+        mbar_init(p_full(i, 0), 128);
+        mbar_init(p_full(i, 1), 128);
+        mbar_init(o_done(i, 0), 1);
+        mbar_init(o_done(i, 1), 1);
+      }
+      mbar_init(drain, 1);
+      gave_up = 0;
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(s_full(i), 1);
-      mbar_init(p_full(i), 128);
-      mbar_init(o_done(i), 1);
+    __syncwarp();
+    for (int t = 0; t < max(n_k, n_v); ++t) {  // the rings' first tiles, beside the rest of the start
+      if (t < n_k) fetch(t, false);
+      if (t < n_v) fetch(t, true);
     }
-    mbar_init(drain, 1);
-    gave_up = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
@@ -975,16 +1066,24 @@ __global__ void __launch_bounds__(kShThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (warp < 8) {  // the query rows, K-major with the 128-byte swizzle; rows past the run are zero
-    constexpr int CH = D / 8;
+    constexpr int CH = D / 8, kBatch = 8;
     const int n_q = pair ? 256 : 128;
-    for (int p = tid; p < n_q * CH; p += 256) {
-      const int r = p / CH, c = p - r * CH;
-      const char* src = query_row(a, it, it.row0 + r);
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (src != nullptr) x = *reinterpret_cast<const uint4*>(src + c * 16);
-      const int rr = r & 127;
-      *reinterpret_cast<uint4*>(smem + CF::kQ + (r >> 7) * CF::kTileBytes + (c >> 3) * (kTileKeys * 128) + rr * 128 +
-                                (((c & 7) ^ (rr & 7)) << 4)) = x;
+    for (int p0 = tid; p0 < n_q * CH; p0 += 256 * kBatch) {
+      uint4 x[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int p = p0 + i * 256, r = p / CH, c = p - r * CH;
+        const char* src = r < n_q ? query_row(a, it, it.row0 + r) : nullptr;
+        x[i] = make_uint4(0, 0, 0, 0);
+        if (src != nullptr) x[i] = __ldg(reinterpret_cast<const uint4*>(src + c * 16));
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int p = p0 + i * 256, r = p / CH, c = p - r * CH, rr = r & 127;
+        if (r < n_q)
+          *reinterpret_cast<uint4*>(smem + CF::kQ + (r >> 7) * CF::kTileBytes + (c >> 3) * (kTileKeys * 128) + rr * 128 +
+                                    (((c & 7) ^ (rr & 7)) << 4)) = x[i];
+      }
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -994,41 +1093,17 @@ __global__ void __launch_bounds__(kShThreads, 1)
   const uint32_t tmem = tmem_slot;
 
   if (warp == 8) {
-    // ---- K and V tiles
-    const int bs = a.block_size;
-    const int box = bs < kTileKeys ? bs : kTileKeys;     // rows of a TMA box
-    const int boxes = kTileKeys / box * CF::kHalves;     // boxes of a K or V tile
-    int n_k = 0, n_v = 0;
     bool ok = true;
-    for (int t = 0; t < n_tiles && ok; ++t) {
-      // this lane's boxes: lane, lane + 32 (128 keys of 8-token blocks at head_dim 128 make 32)
-      const int j = lane / CF::kHalves, half = lane - j * CF::kHalves;
-      const int pos = it.key0 + t * kTileKeys + j * box;
-      int blk = -1, row = 0;
-      if (lane < boxes && pos < it.key1) {
-        const int lb = pos / bs;
-        row = pos - lb * bs;
-        blk = __ldg(a.run_blocks + it.block0 + lb);
-        if (blk < 0 || blk >= a.num_blocks) {
-          record_status(a.status, AUGUR_KV_EBOUNDS);
-          blk = -1;
-        }
-      }
-      const int at = blk >= 0 ? blk : int(a.num_blocks);  // past the pool: zeros
-      const uint32_t off = uint32_t(half) * (kTileKeys * 128) + uint32_t(j) * uint32_t(box) * 128u;
+    for (int t = min(CF::kKBufs, CF::kVBufs); t < n_tiles && ok; ++t) {
 #pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        const int bufs = kv ? CF::kVBufs : CF::kKBufs, buf = t % bufs, use = t / bufs;
-        const uint32_t full = kv ? v_full(buf) : k_full(buf), empty = kv ? v_empty(buf) : k_empty(buf);
-        if (use > 0) ok = mbar_wait(empty, uint32_t(use - 1) & 1u, &gave_up);
+      for (int v = 0; v < 2; ++v) {
+        const int bufs = v ? CF::kVBufs : CF::kKBufs;
+        if (t < bufs) continue;
+        ok = mbar_wait(v ? v_empty(t % bufs) : k_empty(t % bufs), uint32_t(t / bufs - 1) & 1u, &gave_up);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        if (lane == 0) mbar_expect(full, CF::kTileBytes);
-        __syncwarp();
-        if (lane < boxes)
-          tma_box(sb + (kv ? CF::kV : CF::kK) + uint32_t(buf) * CF::kTileBytes + off, kv ? &v_map : &k_map, full,
-                  half * 64, row, it.kv_head, at);
-        if (kv) n_v = t + 1;
+        fetch(t, v != 0);
+        if (v) n_v = t + 1;
         else n_k = t + 1;
       }
     }
@@ -1055,15 +1130,15 @@ __global__ void __launch_bounds__(kShThreads, 1)
         mma_commit(s_full(i));
         if (!pair || i == 1) mma_commit(k_empty(t % CF::kKBufs));
       };
-      auto issue_o = [&](int i, int t, bool acc) {
+      auto issue_o = [&](int i, int t, int half, bool acc) {  // 64 keys
         const uint32_t v = sb + CF::kV + uint32_t(t % CF::kVBufs) * CF::kTileBytes;
-        const uint32_t p = tmem + CF::kS + uint32_t(i) * 128u;
+        const uint32_t p = tmem + CF::kP + uint32_t(i) * CF::kPStep;
 #pragma unroll
-        for (int s = 0; s < kTileKeys / 16; ++s)
-          mma_ts(tmem + CF::kO + uint32_t(i) * 128u, p + uint32_t(s) * 8u,
+        for (int s = half * 4; s < half * 4 + 4; ++s)
+          mma_ts(tmem + CF::kO + uint32_t(i) * uint32_t(D), p + uint32_t(s) * 8u,
                  sw128_desc(v + uint32_t(s) * 2048u, kTileKeys * 128), idesc_o, acc || s > 0);
-        mma_commit(o_done(i));
-        if (!pair || i == 1) mma_commit(v_empty(t % CF::kVBufs));
+        mma_commit(o_done(i, half));
+        if (half == 1 && (!pair || i == 1)) mma_commit(v_empty(t % CF::kVBufs));
       };
       auto wait_k = [&](int t) { return mbar_wait(k_full(t % CF::kKBufs), uint32_t(t / CF::kKBufs) & 1u, &gave_up); };
       auto wait_v = [&](int t) { return mbar_wait(v_full(t % CF::kVBufs), uint32_t(t / CF::kVBufs) & 1u, &gave_up); };
@@ -1088,11 +1163,21 @@ __global__ void __launch_bounds__(kShThreads, 1)
             ok = wait_v(t);
             if (ok && next < n_tiles) ok = wait_k(next);
           }
-          if (ok) ok = mbar_wait(p_full(i), uint32_t(u) & 1u, &gave_up);
+          if (ok) ok = mbar_wait(p_full(i, 0), uint32_t(u) & 1u, &gave_up);
           if (!ok) break;
           tc_after();
-          issue_o(i, t, u > 0);
-          if (next < n_tiles) issue_s(i, next);  // in order behind the product that reads P from there
+          issue_o(i, t, 0, u > 0);
+          if (CF::kOwnP && next < n_tiles) {
+            ok = mbar_wait(s_free(i), uint32_t(u) & 1u, &gave_up);
+            if (!ok) break;
+            tc_after();
+            issue_s(i, next);
+          }
+          ok = mbar_wait(p_full(i, 1), uint32_t(u) & 1u, &gave_up);
+          if (!ok) break;
+          tc_after();
+          issue_o(i, t, 1, true);
+          if (!CF::kOwnP && next < n_tiles) issue_s(i, next);  // in order behind the product that reads P from there
         }
         if (!any) break;
       }
@@ -1107,96 +1192,150 @@ __global__ void __launch_bounds__(kShThreads, 1)
     // ---- softmax: group i, one row a thread
     const int i = warp >> 2, r = tid & 127;
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
-    const uint32_t t_s = tmem + CF::kS + uint32_t(i) * 128u + lanes, t_o = tmem + CF::kO + uint32_t(i) * 128u + lanes;
+    const uint32_t t_s = tmem + CF::kS + uint32_t(i) * 128u + lanes, t_o = tmem + CF::kO + uint32_t(i) * uint32_t(D) + lanes;
+    const uint32_t t_p = tmem + CF::kP + uint32_t(i) * CF::kPStep + lanes;
     const int n_mine = pair ? n_tiles : (n_tiles - i + 1) / 2;
+    const uint64_t scale2 = pack2(a.scale, a.scale);
     float m = kNegInf, l = 0.f;
     bool ok = true;
+    // 32 columns of S of which `left` are keys: the rest counts as -inf
+    auto mask = [&](uint32_t* s, int left) {
+      if (left < 32) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (j >= left) s[j] = 0xff800000u;
+      }
+    };
+    auto max32 = [&](const uint32_t* s, float mx) {
+      float m0 = mx, m1 = kNegInf, m2 = kNegInf, m3 = kNegInf;
+#pragma unroll
+      for (int j = 0; j < 32; j += 8) {
+        m0 = fmaxf(m0, fmaxf(__uint_as_float(s[j]), __uint_as_float(s[j + 1])));
+        m1 = fmaxf(m1, fmaxf(__uint_as_float(s[j + 2]), __uint_as_float(s[j + 3])));
+        m2 = fmaxf(m2, fmaxf(__uint_as_float(s[j + 4]), __uint_as_float(s[j + 5])));
+        m3 = fmaxf(m3, fmaxf(__uint_as_float(s[j + 6]), __uint_as_float(s[j + 7])));
+      }
+      return fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+    };
+    // P of 32 columns, and their sum
+    auto exps = [&](const uint32_t* s, uint32_t* p, uint64_t& sum) {
+      // scores of -inf only so far: their exponentials are 0; an infinite score makes the row NaN, as softmax does
+      const float neg = m == kNegInf ? 0.f : m == INFINITY ? NAN : -m;
+      const uint64_t neg2 = pack2(neg, neg);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        float x, y;
+        unpack2(fma2(pack2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), scale2, neg2), x, y);
+        uint64_t e;
+        if (j % CF::kPolyEvery == CF::kPolyEvery - 1) {
+          e = exp2_poly2(x, y);
+          unpack2(e, x, y);
+        } else {
+          x = ex2(x);
+          y = ex2(y);
+          e = pack2(x, y);
+        }
+        sum = add2(sum, e);  // the sum takes the unrounded values; P V takes them rounded to the cache type
+        p[j] = Elem<T>::pack(x, y);
+      }
+    };
     for (int u = 0; u < n_mine && ok; ++u) {
-      const int t = pair ? u : 2 * u + i;
+      const int t = pair ? u : 2 * u + i, left = n_keys - t * kTileKeys;
       ok = mbar_wait(s_full(i), uint32_t(u) & 1u, &gave_up);
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
         break;
       }
       tc_after();
-      uint32_t s[128];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, s + c * 32);
-      tmem_wait_ld();
-      const int left = n_keys - t * kTileKeys;
-      if (left < kTileKeys) {
+      for (int half = 0; half < 2; ++half) {
+        uint32_t s0[32], s1[32], p[32];
+        float mx = kNegInf;
+        if (u == 0 && half == 0) {  // no reference yet
+          tmem_ld32(t_s, s0);
+          tmem_ld32(t_s + 32, s1);
+          tmem_wait_ld32(s0);
+          tmem_wait_ld32(s1);
+          mask(s0, left);
+          mask(s1, left - 32);
+          m = max32(s1, max32(s0, kNegInf)) * a.scale;
+        }
+        uint64_t sum;
+        for (;;) {
+          tmem_ld32(t_s + half * 64, s0);
+          tmem_wait_ld32(s0);
+          tmem_ld32(t_s + half * 64 + 32, s1);
+          mask(s0, left - half * 64);
+          sum = 0;
+          exps(s0, p, sum);
+          mx = max32(s0, kNegInf);
+          tmem_wait_ld32(s1);
+          mask(s1, left - half * 64 - 32);
+          exps(s1, p + 16, sum);
+          mx = max32(s1, mx) * a.scale;
+          const bool grow = mx > m + 8.f;
+          if (!__any_sync(0xffffffffu, grow)) break;
+          const float mn = grow ? mx : m;
+          if (u > 0 || half > 0) {  // the last product into O: this tile's first half, or the last tile's second
+            ok = mbar_wait(o_done(i, half ^ 1), uint32_t(half ? u : u - 1) & 1u, &gave_up);
+            if (!__all_sync(0xffffffffu, ok)) {
+              ok = false;
+              break;
+            }
+            tc_after();
+            const float alpha = m == kNegInf ? 0.f : ex2(m - mn);
+            l *= alpha;
 #pragma unroll
-        for (int j = 0; j < 128; ++j)
-          if (j >= left) s[j] = 0xff800000u;  // -inf
-      }
-      float mx0 = kNegInf, mx1 = kNegInf;
+            for (int c = 0; c < D / 32; ++c) {
+              tmem_ld32(t_o + c * 32, s0);
+              tmem_wait_ld32(s0);
 #pragma unroll
-      for (int j = 0; j < 128; j += 2) {
-        mx0 = fmaxf(mx0, __uint_as_float(s[j]));
-        mx1 = fmaxf(mx1, __uint_as_float(s[j + 1]));
-      }
-      const float mx = fmaxf(mx0, mx1) * a.scale;
-      const bool grow = mx > m + 8.f;  // the first tile, and rarely later
-      if (__any_sync(0xffffffffu, grow)) {
-        const float mn = grow ? mx : m;
-        if (u > 0) {
-          ok = mbar_wait(o_done(i), uint32_t(u - 1) & 1u, &gave_up);
+              for (int j = 0; j < 32; ++j) s0[j] = __float_as_uint(__uint_as_float(s0[j]) * alpha);
+              tmem_st32(t_o + c * 32, s0);
+            }
+            tmem_wait_st();
+          }
+          m = mn;
+        }
+        if (!ok) break;
+        if (CF::kOwnP && half == 1) {  // S is read: the next tile's may take its place
+          tc_before();
+          mbar_arrive(s_free(i));
+        }
+        float x, y;
+        unpack2(sum, x, y);
+        l += x + y;
+        // P's place: its last reader was done before this tile's S was, but for the second half of a P of its own
+        if (CF::kOwnP && half == 1 && u > 0) {
+          ok = mbar_wait(o_done(i, 1), uint32_t(u - 1) & 1u, &gave_up);
           if (!__all_sync(0xffffffffu, ok)) {
             ok = false;
             break;
           }
           tc_after();
-          const float alpha = ex2(m - mn);
-          l *= alpha;
-#pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t x[32];
-            tmem_ld32(t_o + c * 32, x);
-            tmem_wait_ld();
-#pragma unroll
-            for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * alpha);
-            tmem_st32(t_o + c * 32, x);
-          }
-          tmem_wait_st();
         }
-        m = mn;
+        tmem_st32(t_p + half * 32, p);
+        tmem_wait_st();
+        tc_before();
+        mbar_arrive(p_full(i, half));
       }
-      const float neg = m == kNegInf ? 0.f : -m;  // scores of -inf only so far: their exponentials are 0
-      float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t p[32];
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const float x = ex2(fmaf(__uint_as_float(s[c * 64 + 2 * j]), a.scale, neg));
-          const float y = ex2(fmaf(__uint_as_float(s[c * 64 + 2 * j + 1]), a.scale, neg));
-          l0 += x;  // the sum takes the unrounded values; P V takes them rounded to the cache type
-          l1 += y;
-          p[j] = Elem<T>::pack(x, y);
-        }
-        tmem_st32(t_s + c * 32, p);
-      }
-      l += l0 + l1;
-      tmem_wait_st();
-      tc_before();
-      mbar_arrive(p_full(i));
     }
-    if (ok && n_mine > 0) ok = mbar_wait(o_done(i), uint32_t(n_mine - 1) & 1u, &gave_up);
+    if (ok && n_mine > 0) ok = mbar_wait(o_done(i, 1), uint32_t(n_mine - 1) & 1u, &gave_up);
     ok = __all_sync(0xffffffffu, ok);
     tc_after();
     const int row = it.row0 + (pair ? i * 128 : 0) + r;
-    const int64_t at = int64_t(pair && i ? it.slab1 : it.slab0) * kSlabRows + r;
+    const int64_t slab = pair && i ? it.slab1 : it.slab0;
     float* other = reinterpret_cast<float*>(smem + CF::kK);  // [D][128] then m, l: the rings are idle by then
     static_assert((D + 2) * 512 <= (CF::kKBufs + CF::kVBufs) * CF::kTileBytes, "the join fits the rings");
-    if (!pair) {
+    if (!pair && n_tiles > 1) {
       asm volatile("bar.sync 1, 256;" ::: "memory");  // both groups' products have read the rings
       if (i == 1) {
-        if (ok && n_mine > 0) {
+        if (ok) {
 #pragma unroll
           for (int c = 0; c < D / 32; ++c) {
             uint32_t x[32];
             tmem_ld32(t_o + c * 32, x);
-            tmem_wait_ld();
+            tmem_wait_ld32(x);
 #pragma unroll
             for (int j = 0; j < 32; ++j) other[(c * 32 + j) * 128 + r] = __uint_as_float(x[j]);
           }
@@ -1207,33 +1346,34 @@ __global__ void __launch_bounds__(kShThreads, 1)
       asm volatile("bar.sync 1, 256;" ::: "memory");
     }
     if (ok && (pair || i == 0)) {
+      const bool joined = !pair && n_tiles > 1;
       float f0 = 1.f, f1 = 0.f;
-      if (!pair) {
+      if (joined) {
         const float m1 = other[D * 128 + r], l1 = other[(D + 1) * 128 + r];
         const float mn = fmaxf(m, m1);
-        f0 = ex2(m - mn);
+        f0 = m == kNegInf ? 0.f : ex2(m - mn);
         f1 = m1 == kNegInf ? 0.f : ex2(m1 - mn);
         l = l * f0 + l1 * f1;
         m = mn;
       }
-      const bool joined = !pair && n_tiles > 1;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         uint32_t x[32];
         tmem_ld32(t_o + c * 32, x);
-        tmem_wait_ld();
+        tmem_wait_ld32(x);
         if (joined) {
 #pragma unroll
           for (int j = 0; j < 32; ++j)
             x[j] = __float_as_uint(__uint_as_float(x[j]) * f0 + other[(c * 32 + j) * 128 + r] * f1);
         }
         if (row < it.n_rows) {
+          float* dst = a.slab_o + ((slab * (D / 4) + c * 8) * kSlabRows + r) * 4;
 #pragma unroll
           for (int j = 0; j < 32; j += 4)
-            *reinterpret_cast<uint4*>(a.slab_o + at * D + c * 32 + j) = make_uint4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+            *reinterpret_cast<uint4*>(dst + j * kSlabRows) = make_uint4(x[j], x[j + 1], x[j + 2], x[j + 3]);
         }
       }
-      if (row < it.n_rows) *reinterpret_cast<float2*>(a.slab_ml + at * 2) = make_float2(m, l);
+      if (row < it.n_rows) *reinterpret_cast<float2*>(a.slab_ml + (slab * kSlabRows + r) * 2) = make_float2(m, l);
     }
   }
   tc_before();
@@ -1375,7 +1515,7 @@ AUGUR_KV_EXPORT int augur_kv_shared_prefix_workspace(int32_t n_slabs, int32_t ba
   const int split = own_split(units, max_own_len);
   const int64_t rows = int64_t(n_slabs) * kSlabRows + (split > 1 ? units * split * (n_q_heads / n_kv_heads) : 0);
   *counters_bytes = split > 1 ? units * 4 : 0;
-  *scratch_bytes = rows * (int64_t(head_dim) + 2) * 4 + 64;
+  *scratch_bytes = rows * (int64_t((head_dim + 3) / 4 * 4) + 2) * 4 + 64;
   return AUGUR_KV_OK;
 }
 
@@ -1406,7 +1546,7 @@ AUGUR_KV_EXPORT int augur_kv_shared_prefix_attention(const augur_kv_shared_prefi
   Args a;
   memset(&a, 0, sizeof(a));
   a.groups = p->n_q_heads / p->n_kv_heads;
-  if (a.groups > kGRows || p->head_dim > kGMaxDim || a.groups * p->head_dim > 32 * kGThreads)
+  if (a.groups > kGRows || p->head_dim > kGMaxDim || a.groups * ((p->head_dim + 3) / 4) > 8 * kGThreads)
     return fail(AUGUR_KV_EINVAL,
                 "shared_prefix_attention: at most %d query heads per KV head, head_dim %d, and %d values of both together",
                 kGRows, kGMaxDim, 32 * kGThreads);
@@ -1434,7 +1574,8 @@ AUGUR_KV_EXPORT int augur_kv_shared_prefix_attention(const augur_kv_shared_prefi
   a.out = static_cast<char*>(out);
   a.out_stride_b = p->out_strides[0] * es;
   a.out_stride_h = p->out_strides[1] * es;
-  a.out_wide = ((reinterpret_cast<uintptr_t>(out) | uintptr_t(a.out_stride_b) | uintptr_t(a.out_stride_h)) & uintptr_t(4 * es - 1)) == 0;
+  a.quads = (p->head_dim + 3) / 4;
+  a.out_wide = p->head_dim % 4 == 0 && ((reinterpret_cast<uintptr_t>(out) | uintptr_t(a.out_stride_b) | uintptr_t(a.out_stride_h)) & uintptr_t(4 * es - 1)) == 0;
   a.items = reinterpret_cast<const Item*>(p->items);
   a.n_items = p->n_items;
   a.members = p->members;
@@ -1471,19 +1612,20 @@ AUGUR_KV_EXPORT int augur_kv_shared_prefix_attention(const augur_kv_shared_prefi
   {  // scratch: output rows of the slabs and of the parts, then their maxima and sums
     const int64_t slab_rows = int64_t(a.n_slabs) * kSlabRows;
     const int64_t part_rows = a.n_split > 1 ? units * a.n_split * a.groups : 0;
-    if ((slab_rows + part_rows) * (a.head_dim + 2) * 4 + 64 > p->scratch_bytes && slab_rows + part_rows > 0)
+    const int width = 4 * a.quads;
+    if ((slab_rows + part_rows) * (width + 2) * 4 + 64 > p->scratch_bytes && slab_rows + part_rows > 0)
       return fail(AUGUR_KV_EINVAL, "shared_prefix_attention: the scratch is too small");
     if (a.n_split > 1 && (p->counters == nullptr || p->counters_bytes < units * 4))
       return fail(AUGUR_KV_EINVAL, "shared_prefix_attention: the counters are too small");
     float* f = static_cast<float*>(p->scratch);
     a.slab_o = f;
-    f += slab_rows * a.head_dim;
+    f += slab_rows * width;
     a.split_o = f;
-    f += part_rows * a.head_dim;
+    f += part_rows * width;
     a.slab_ml = f;  // an even number of floats behind an aligned start: pairs are aligned
     f += slab_rows * 2;
     a.split_ml = f;
-    if (slab_rows + part_rows > 0x7fffffff) return fail(AUGUR_KV_EINVAL, "shared_prefix_attention: too many partial rows");
+    if ((slab_rows + part_rows) * a.quads > 0x7fffffff) return fail(AUGUR_KV_EINVAL, "shared_prefix_attention: too many partial rows");
     a.counters = p->counters;
   }
   if (units * a.n_split > 0x7fffffff) return fail(AUGUR_KV_EINVAL, "shared_prefix_attention: too many sequences");

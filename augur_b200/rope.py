@@ -17,6 +17,7 @@ largest position does it, or rope_tables()).
 
 from __future__ import annotations
 
+import ctypes
 from collections.abc import Sequence
 
 import numpy as np
@@ -349,6 +350,9 @@ class RopeAxes:
         self.half = len(axes)
         self.inv_freq = inv_freq.contiguous()
         self.axis = torch.tensor(axes, dtype=torch.int32).to(inv_freq.device)
+        # the last call's layout and argument block: the layers of a step, and steps of one batch
+        # size, differ in nothing but their tensors' addresses
+        self._prepared: tuple | None = None
 
     @staticmethod
     def frequencies(head_dim: int, rope_theta: float, device: torch.device) -> Tensor:
@@ -392,50 +396,86 @@ def write_paged_kv_batch_rope_axes(
     once to the cache dtype. There is no table of positions: nothing to build or to grow, no host
     sync, and any call can be captured in a CUDA graph.
     """
+    kc, vc = cache.keys, cache.values
+    layout = (kc.shape, kc.stride(), kc.dtype, kc.get_device(),
+              q.shape, q.stride(), q.dtype, q.get_device(), key.shape, key.stride(), key.dtype, key.get_device(),
+              value.shape, value.stride(), value.dtype, value.get_device(), slot_mapping.shape, slot_mapping.stride(),
+              slot_mapping.dtype, slot_mapping.get_device(), positions.shape, positions.stride(), positions.dtype,
+              positions.get_device(), vc.shape, vc.stride(), vc.dtype)
+    ready = axes._prepared
+    if ready is None or ready[0] != layout:
+        _check_rope_axes(cache, q, key, value, slot_mapping, positions, axes)
+    if not 0 <= layer_idx < kc.shape[0]:
+        raise ValueError("layer_idx is outside the cache layer range")
+    if ready is None or ready[0] != layout:
+        plain = (q.stride(2) == key.stride(2) == value.stride(2) == 1
+                 and slot_mapping.dtype == positions.dtype == torch.int64)
+        if not plain:  # what the kernel takes: head_dim contiguous, int64 indices
+            q, key, value = (_last_dim_contiguous(t) for t in (q, key, value))
+            slot_mapping, positions = slot_mapping.to(torch.int64), positions.to(torch.int64)
+        ready = (layout if plain else None, _rope_axes_args(cache, q, key, value, slot_mapping, positions, axes))
+        if plain:
+            axes._prepared = ready
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if q.shape[0] == 0 or q.shape[1] == 0:
+        return q_out
+    index = kc.get_device()
+    raw = stream.cuda_stream if stream is not None else _ops.current_raw_stream(index)
+    args, at = ready[1]
+    args.k_pool, args.v_pool = kc.data_ptr(), vc.data_ptr()
+    call = (at, layer_idx, q.data_ptr(), key.data_ptr(), value.data_ptr(), q_out.data_ptr(),
+            slot_mapping.data_ptr(), positions.data_ptr(), raw)
+    if _ops.current_device() == index:
+        code = _lib.load().augur_kv_rope_axes_scatter(*call)
+    else:
+        with _ops._DeviceGuard(kc.device):
+            code = _lib.load().augur_kv_rope_axes_scatter(*call)
+    if code != _lib.OK:
+        _lib.check(code, "augur_kv_rope_axes_scatter")
+    _ops.launch_count += 1
+    if stream is not None:
+        _ops.keep_until_done(stream, q, key, value, q_out, slot_mapping, positions, axes.inv_freq, axes.axis)
+    return q_out
+
+
+def _check_rope_axes(cache: PagedKVCache, q: Tensor, key: Tensor, value: Tensor, slot_mapping: Tensor,
+                     positions: Tensor, axes: RopeAxes) -> None:
     if key.shape != value.shape or key.dim() != 3 or q.dim() != 3 or q.shape[0] != key.shape[0]:
         raise ValueError("q [tokens, heads, D], key/value [tokens, kv_heads, D] expected")
-    L, NB, Hkv, bs, D = cache.keys.shape
-    if not 0 <= layer_idx < L:
-        raise ValueError("layer_idx is outside the cache layer range")
+    kc, vc = cache.keys, cache.values
     n_tokens, num_heads, head_dim = key.shape
-    if (num_heads, head_dim) != (Hkv, D) or q.shape[2] != D:
+    if (num_heads, head_dim) != (kc.shape[2], kc.shape[4]) or q.shape[2] != head_dim:
         raise ValueError("key/value shape does not match cache shape")
-    if axes.half * 2 != D:
+    if axes.half * 2 != head_dim:
         raise ValueError("axes must have head_dim / 2 frequencies")
     if slot_mapping.shape != (n_tokens,):
         raise ValueError("slot_mapping must have shape [tokens]")
     if positions.dim() != 2 or positions.shape[0] < axes.n_axes or positions.shape[1] != n_tokens:
         raise ValueError("positions must have shape [axes, tokens]")
-    kc, vc = cache.keys, cache.values
-    dt = kc.dtype
-    if q.dtype != dt or key.dtype != dt or value.dtype != dt or vc.dtype != dt:
+    if not (q.dtype == key.dtype == value.dtype == vc.dtype == kc.dtype):
         raise ValueError("q, key, value and the cache must share one dtype")
-    if kc.stride() != vc.stride() or kc.stride(4) != 1:
+    if kc.shape != vc.shape or kc.stride() != vc.stride() or kc.stride(4) != 1:
         raise ValueError("keys and values must share one layout, head_dim contiguous")
-    device = kc.device
     _ops.require_cuda("write_paged_kv_batch_rope_axes", kc, vc, q, key, value, slot_mapping, positions, axes.inv_freq)
     if not (q.device == key.device == value.device == vc.device == slot_mapping.device == positions.device
-            == axes.inv_freq.device == device):
+            == axes.inv_freq.device == kc.device):
         raise ValueError("all tensors must be on the cache's device")
-    q, key, value = (_last_dim_contiguous(t) for t in (q, key, value))
-    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    if n_tokens == 0 or q.shape[1] == 0:
-        return q_out
-    slots = slot_mapping if slot_mapping.dtype == torch.int64 else slot_mapping.to(torch.int64)
-    pos = positions if positions.dtype == torch.int64 else positions.to(torch.int64)
-    st = stream if stream is not None else torch.cuda.current_stream(device)
-    es = kc.element_size()
-    off = layer_idx * kc.stride(0) * es
-    with _ops._DeviceGuard(device):
-        code = _lib.load().augur_kv_rope_axes_scatter(
-            q.data_ptr(), _lib.i64_array(q.stride()[:2]), q_out.data_ptr(), _lib.i64_array(q_out.stride()[:2]), q.shape[1],
-            key.data_ptr(), _lib.i64_array(key.stride()[:2]), value.data_ptr(), _lib.i64_array(value.stride()[:2]),
-            _ops.dtype_code(kc), kc.data_ptr() + off, vc.data_ptr() + off, _lib.i64_array(kc.stride()[1:4]), NB, bs,
-            slots.data_ptr(), slots.stride(0), pos.data_ptr(), _lib.i64_array(pos.stride()), pos.shape[0],
-            axes.inv_freq.data_ptr(), axes.axis.data_ptr(), n_tokens, Hkv, D,
-            _ops.status_word(device).data_ptr(), st.cuda_stream)
-    _lib.check(code, "augur_kv_rope_axes_scatter")
-    _ops.launch_count += 1
-    if stream is not None:
-        _ops.keep_until_done(st, q, key, value, q_out, slots, pos, axes.inv_freq, axes.axis)
-    return q_out
+
+
+def _rope_axes_args(cache: PagedKVCache, q: Tensor, key: Tensor, value: Tensor, slot_mapping: Tensor,
+                    positions: Tensor, axes: RopeAxes) -> tuple[_lib.RopeAxesArgs, int]:
+    """The argument block of a call with tensors laid out like these, and its address."""
+    kc = cache.keys
+    L, NB, Hkv, bs, D = kc.shape
+    a = _lib.RopeAxesArgs()
+    a.pool_strides[:] = kc.stride()[:4]
+    a.num_blocks, a.block_size, a.n_layers = NB, bs, L
+    a.n_q_heads, a.n_kv_heads, a.head_dim, a.dtype = q.shape[1], Hkv, D, _ops.dtype_code(kc)
+    a.n_tokens = q.shape[0]
+    a.q_strides[:], a.k_strides[:], a.v_strides[:] = q.stride()[:2], key.stride()[:2], value.stride()[:2]
+    a.q_out_strides[:] = (q.shape[1] * D, D)
+    a.slot_stride = slot_mapping.stride(0)
+    a.position_strides[:] = positions.stride()
+    a.inv_freq, a.axis_of_frequency, a.n_axes = axes.inv_freq.data_ptr(), axes.axis.data_ptr(), positions.shape[0]
+    a.status = _ops.status_word(kc.device).data_ptr()
+    return a, ctypes.addressof(a)

@@ -17,14 +17,14 @@ from . import _lib, _ops
 _MAX_VOCAB = 1 << 21
 
 
-def _setting(name: str, value: float | int | Tensor, rows: int, dtype: torch.dtype, device: torch.device):
+def _setting(name: str, value: float | int | Tensor, rows: int, dtype: torch.dtype, index: int):
     """(per-row tensor or None, scalar) of a sampling setting."""
     if isinstance(value, Tensor):
         if value.shape != (rows,):
             raise ValueError(f"{name} must be a number or a tensor of shape [rows]")
-        if value.device != device:
+        if value.get_device() != index:
             raise ValueError(f"{name} must be on the logits' device")
-        if value.dtype != dtype:
+        if value.dtype is not dtype:
             value = value.to(dtype)
         return value if value.is_contiguous() else value.contiguous(), 0
     return None, value
@@ -58,36 +58,43 @@ def sample_tokens(
     if logits.dim() != 2:
         raise ValueError("logits must be [rows, vocab]")
     rows, vocab = logits.shape
-    _ops.require_cuda("sample_tokens", logits, uniform)
+    if not (logits.is_cuda and uniform.is_cuda):
+        _ops.require_cuda("sample_tokens", logits, uniform)
     if not 0 < vocab <= _MAX_VOCAB:
         raise ValueError(f"vocab must be between 1 and {_MAX_VOCAB}")
-    if uniform.shape != (rows,) or uniform.dtype != torch.float32 or uniform.device != logits.device:
+    index = logits.get_device()
+    if uniform.shape != (rows,) or uniform.dtype is not torch.float32 or uniform.get_device() != index:
         raise ValueError("uniform must be a float32 tensor of shape [rows] on the logits' device")
     dtype = _ops._DTYPE_CODES.get(logits.dtype)
     if dtype is None:
         raise ValueError(f"unsupported logits dtype {logits.dtype}; use float32, float16 or bfloat16")
-    device = logits.device
-    if logits.stride(1) != 1 and vocab > 1:
+    row_stride, step = logits.stride()
+    if step != 1 and vocab > 1:
         logits = logits.contiguous()
+        row_stride = vocab
     if not uniform.is_contiguous():
         uniform = uniform.contiguous()
-    t, t_all = _setting("temperature", temperature, rows, torch.float32, device)
-    k, k_all = _setting("top_k", top_k, rows, torch.int32, device)
-    p, p_all = _setting("top_p", top_p, rows, torch.float32, device)
-    m, m_all = _setting("min_p", min_p, rows, torch.float32, device)
+    t, t_all = _setting("temperature", temperature, rows, torch.float32, index)
+    k, k_all = _setting("top_k", top_k, rows, torch.int32, index)
+    p, p_all = _setting("top_p", top_p, rows, torch.float32, index)
+    m, m_all = _setting("min_p", min_p, rows, torch.float32, index)
     tokens = torch.empty_like(uniform, dtype=torch.int64)
     logprobs = torch.empty_like(uniform)
     if rows == 0:
         return tokens, logprobs
-    st = stream if stream is not None else torch.cuda.current_stream(device)
-    with _ops._DeviceGuard(device):
-        code = _lib.load().augur_kv_sample(
-            logits.data_ptr(), logits.stride(0), rows, vocab, dtype, uniform.data_ptr(),
+    call = (logits.data_ptr(), row_stride, rows, vocab, dtype, uniform.data_ptr(),
             None if t is None else t.data_ptr(), t_all, None if k is None else k.data_ptr(), k_all,
             None if p is None else p.data_ptr(), p_all, None if m is None else m.data_ptr(), m_all,
-            tokens.data_ptr(), logprobs.data_ptr(), st.cuda_stream)
-    _lib.check(code, "augur_kv_sample")
+            tokens.data_ptr(), logprobs.data_ptr(),
+            stream.cuda_stream if stream is not None else _ops.current_raw_stream(index))
+    if _ops.current_device() == index:
+        code = _lib.load().augur_kv_sample(*call)
+    else:
+        with _ops._DeviceGuard(logits.device):
+            code = _lib.load().augur_kv_sample(*call)
+    if code != _lib.OK:
+        _lib.check(code, "augur_kv_sample")
     _ops.launch_count += 1
     if stream is not None:
-        _ops.keep_until_done(st, logits, uniform, t, k, p, m, tokens, logprobs)
+        _ops.keep_until_done(stream, logits, uniform, t, k, p, m, tokens, logprobs)
     return tokens, logprobs

@@ -535,28 +535,45 @@ int augur_kv_shared_prefix_workspace(int32_t n_slabs, int32_t batch, int32_t n_q
  * height, width for images and video), fused with the append of keys and
  * values to a paged pool layer.
  *
- * Token t has position positions[axis*S[0] + t*S[1]] on each of n_axes axes
- * (S = position_strides). Frequency j (0 <= j < head_dim/2) turns elements j
- * and j + head_dim/2 of every q and k row by
+ * args holds what the layers of a call share. Token t has position
+ * positions[axis*S[0] + t*S[1]] on each of n_axes axes (S = position_strides).
+ * Frequency j (0 <= j < head_dim/2) turns elements j and j + head_dim/2 of
+ * every q and k row by
  *   angle = float(position on axis axis_of_frequency[j]) * inv_freq[j]
  * in float32, rounded once to the dtype. q goes to q_out, k and v to slot
- * slots[t*slot_stride] of the pool (block = slot / block_size); a negative
+ * slots[t*slot_stride] of the pools' layer (block = slot / block_size); a negative
  * slot writes no k and v. A slot outside the pool, or an axis outside
  * [0, n_axes), records AUGUR_KV_EBOUNDS (the row is not written; the frequency
- * turns nothing). Positions are exact up to 2^24.
- * All strides are in elements: q, q_out, k, v: token, head; pool: block, kv
- * head, row; head_dim elements are contiguous. k and v pools share strides.
+ * turns nothing). Positions are exact up to 2^24. head_dim elements are
+ * contiguous everywhere; k and v pools share strides.
  */
-int augur_kv_rope_axes_scatter(const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides,
-                               int32_t n_q_heads, const void* k, const int64_t* k_strides, const void* v,
-                               const int64_t* v_strides, int32_t dtype, void* k_pool, void* v_pool,
-                               const int64_t* pool_strides, int64_t num_blocks, int32_t block_size,
-                               const int64_t* slots, int64_t slot_stride, const int64_t* positions,
-                               const int64_t* position_strides, int32_t n_axes,
-                               const float* inv_freq,            /* device [head_dim/2] */
-                               const int32_t* axis_of_frequency, /* device [head_dim/2] */
-                               int64_t n_tokens, int32_t n_kv_heads, int32_t head_dim,
-                               int32_t* status, /* device int32 or NULL */
+typedef struct augur_kv_rope_axes_args {
+  void* k_pool; /* layer 0 of the pools */
+  void* v_pool;
+  int64_t pool_strides[4]; /* elements: layer, block, kv head, row */
+  int64_t num_blocks;
+  int32_t block_size;
+  int32_t n_layers;
+  int32_t n_q_heads;
+  int32_t n_kv_heads;
+  int32_t head_dim;
+  int32_t dtype;
+  int64_t n_tokens;
+  int64_t q_strides[2]; /* elements: token, head */
+  int64_t k_strides[2];
+  int64_t v_strides[2];
+  int64_t q_out_strides[2];
+  int64_t slot_stride;
+  int64_t position_strides[2]; /* elements: axis, token */
+  const float* inv_freq;            /* device [head_dim/2] */
+  const int32_t* axis_of_frequency; /* device [head_dim/2] */
+  int32_t n_axes;
+  int32_t reserved;
+  int32_t* status; /* device int32 or NULL */
+} augur_kv_rope_axes_args;
+
+int augur_kv_rope_axes_scatter(const augur_kv_rope_axes_args* args, int32_t layer, const void* q, const void* k,
+                               const void* v, void* q_out, const int64_t* slots, const int64_t* positions,
                                void* stream);
 
 /*
