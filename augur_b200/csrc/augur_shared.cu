@@ -972,6 +972,17 @@ __device__ __forceinline__ uint64_t exp2_poly2(float x, float y) {
                __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23)));
 }
 
+// A value that is the same in all lanes, in a form the compiler knows to be.
+__device__ __forceinline__ int warp_uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(one)::"memory");
+  return one != 0;
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kShThreads, 1)
     shared_umma_kernel(const __grid_constant__ Args a, const __grid_constant__ CUtensorMap k_map,
@@ -982,12 +993,12 @@ __global__ void __launch_bounds__(kShThreads, 1)
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int gave_up;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = warp_uniform(tid >> 5), lane = tid & 31;
   launch_dependents();
   Item it;
   if (!read_item(a, blockIdx.x, it)) return;
-  const bool pair = it.slab1 >= 0;
-  const int n_keys = it.key1 - it.key0, n_tiles = (n_keys + kTileKeys - 1) / kTileKeys;
+  const bool pair = warp_uniform(it.slab1 >= 0) != 0;
+  const int n_keys = warp_uniform(it.key1 - it.key0), n_tiles = (n_keys + kTileKeys - 1) / kTileKeys;
   const uint32_t sb = smem_u32(smem), bars = sb + CF::kBar;
   auto k_full = [&](int i) { return bars + 8u * uint32_t(i); };
   auto k_empty = [&](int i) { return bars + 8u * uint32_t(CF::kKBufs + i); };
@@ -1090,7 +1101,7 @@ __global__ void __launch_bounds__(kShThreads, 1)
   tc_before();
   __syncthreads();
   tc_after();
-  const uint32_t tmem = tmem_slot;
+  const uint32_t tmem = uint32_t(warp_uniform(int(tmem_slot)));
 
   if (warp == 8) {
     bool ok = true;
@@ -1115,77 +1126,88 @@ __global__ void __launch_bounds__(kShThreads, 1)
         mbar_wait(v_full(i % CF::kVBufs), uint32_t(i / CF::kVBufs) & 1u, &ignore);
     }
   } else if (warp == 9) {
-    // ---- the products: one thread issues. Group i's tiles are i, i + 2, .. (pair: all of them)
-    if (lane == 0) {
-      constexpr uint32_t idesc_s = mma_desc<T>(kTileKeys, false), idesc_o = mma_desc<T>(D, true);
-      const int step = pair ? 1 : 2;
-      auto issue_s = [&](int i, int t) {
-        const uint32_t q = sb + CF::kQ + (pair ? uint32_t(i) * CF::kTileBytes : 0u);
-        const uint32_t k = sb + CF::kK + uint32_t(t % CF::kKBufs) * CF::kTileBytes;
+    // ---- the products. Group i's tiles are i, i + 2, .. (pair: all of them). The whole warp keeps step, so that
+    // what the instructions take is uniform; one lane issues.
+    constexpr uint32_t idesc_s = mma_desc<T>(kTileKeys, false), idesc_o = mma_desc<T>(D, true);
+    const int step = pair ? 1 : 2;
+    const uint64_t q_desc = sw128_desc(sb + CF::kQ, 16), k_desc = sw128_desc(sb + CF::kK, 16);
+    const uint64_t v_desc = sw128_desc(sb + CF::kV, kTileKeys * 128);
+    auto issue_s = [&](int i, int t) {
+      const uint64_t q = q_desc + (pair ? uint32_t(i) * (CF::kTileBytes >> 4) : 0u);
+      const uint64_t k = k_desc + uint32_t(t % CF::kKBufs) * (CF::kTileBytes >> 4);
+      if (elect_one()) {
 #pragma unroll
         for (int s = 0; s < D / 16; ++s) {
-          const uint32_t o = uint32_t(s >> 2) * (kTileKeys * 128) + uint32_t(s & 3) * 32u;
-          mma_ss(tmem + CF::kS + uint32_t(i) * 128u, sw128_desc(q + o, 16), sw128_desc(k + o, 16), idesc_s, s > 0);
+          const uint32_t o = (uint32_t(s >> 2) * (kTileKeys * 128) + uint32_t(s & 3) * 32u) >> 4;
+          mma_ss(tmem + CF::kS + uint32_t(i) * 128u, q + o, k + o, idesc_s, s > 0);
         }
         mma_commit(s_full(i));
         if (!pair || i == 1) mma_commit(k_empty(t % CF::kKBufs));
-      };
-      auto issue_o = [&](int i, int t, int half, bool acc) {  // 64 keys
-        const uint32_t v = sb + CF::kV + uint32_t(t % CF::kVBufs) * CF::kTileBytes;
-        const uint32_t p = tmem + CF::kP + uint32_t(i) * CF::kPStep;
+      }
+      __syncwarp();
+    };
+    auto issue_o = [&](int i, int t, int half, bool acc) {  // 64 keys
+      const uint64_t v = v_desc + uint32_t(t % CF::kVBufs) * (CF::kTileBytes >> 4);
+      const uint32_t p = tmem + CF::kP + uint32_t(i) * CF::kPStep;
+      if (elect_one()) {
 #pragma unroll
         for (int s = half * 4; s < half * 4 + 4; ++s)
-          mma_ts(tmem + CF::kO + uint32_t(i) * uint32_t(D), p + uint32_t(s) * 8u,
-                 sw128_desc(v + uint32_t(s) * 2048u, kTileKeys * 128), idesc_o, acc || s > 0);
+          mma_ts(tmem + CF::kO + uint32_t(i) * uint32_t(D), p + uint32_t(s) * 8u, v + uint32_t(s) * (2048u >> 4), idesc_o,
+                 acc || s > 0);
         mma_commit(o_done(i, half));
         if (half == 1 && (!pair || i == 1)) mma_commit(v_empty(t % CF::kVBufs));
-      };
-      auto wait_k = [&](int t) { return mbar_wait(k_full(t % CF::kKBufs), uint32_t(t / CF::kKBufs) & 1u, &gave_up); };
-      auto wait_v = [&](int t) { return mbar_wait(v_full(t % CF::kVBufs), uint32_t(t / CF::kVBufs) & 1u, &gave_up); };
-      bool ok = true;
-      for (int i = 0; i < 2 && ok; ++i) {
-        const int t = pair ? 0 : i;
-        if (t >= n_tiles) break;
-        if (i == 0 || !pair) ok = wait_k(t);
-        if (ok) {
-          tc_after();
-          issue_s(i, t);
-        }
       }
-      for (int u = 0; ok; ++u) {
-        bool any = false;
-        for (int i = 0; i < 2 && ok; ++i) {
-          const int t = pair ? u : 2 * u + i;
-          if (t >= n_tiles) break;
-          any = true;
-          const int next = t + step;
-          if (i == 0 || !pair) {
-            ok = wait_v(t);
-            if (ok && next < n_tiles) ok = wait_k(next);
-          }
-          if (ok) ok = mbar_wait(p_full(i, 0), uint32_t(u) & 1u, &gave_up);
+      __syncwarp();
+    };
+    auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, &gave_up));
+    };
+    auto wait_k = [&](int t) { return wait(k_full(t % CF::kKBufs), uint32_t(t / CF::kKBufs) & 1u); };
+    auto wait_v = [&](int t) { return wait(v_full(t % CF::kVBufs), uint32_t(t / CF::kVBufs) & 1u); };
+    bool ok = true;
+    for (int i = 0; i < 2 && ok; ++i) {
+      const int t = pair ? 0 : i;
+      if (t >= n_tiles) break;
+      if (i == 0 || !pair) ok = wait_k(t);
+      if (ok) {
+        tc_after();
+        issue_s(i, t);
+      }
+    }
+    for (int u = 0; ok; ++u) {
+      bool any = false;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int t = pair ? u : 2 * u + i;
+        if (!ok || t >= n_tiles) break;
+        any = true;
+        const int next = t + step;
+        if (i == 0 || !pair) {
+          ok = wait_v(t);
+          if (ok && next < n_tiles) ok = wait_k(next);
+        }
+        if (ok) ok = wait(p_full(i, 0), uint32_t(u) & 1u);
+        if (!ok) break;
+        tc_after();
+        issue_o(i, t, 0, u > 0);
+        if (CF::kOwnP && next < n_tiles) {
+          ok = wait(s_free(i), uint32_t(u) & 1u);
           if (!ok) break;
           tc_after();
-          issue_o(i, t, 0, u > 0);
-          if (CF::kOwnP && next < n_tiles) {
-            ok = mbar_wait(s_free(i), uint32_t(u) & 1u, &gave_up);
-            if (!ok) break;
-            tc_after();
-            issue_s(i, next);
-          }
-          ok = mbar_wait(p_full(i, 1), uint32_t(u) & 1u, &gave_up);
-          if (!ok) break;
-          tc_after();
-          issue_o(i, t, 1, true);
-          if (!CF::kOwnP && next < n_tiles) issue_s(i, next);  // in order behind the product that reads P from there
+          issue_s(i, next);
         }
-        if (!any) break;
+        ok = wait(p_full(i, 1), uint32_t(u) & 1u);
+        if (!ok) break;
+        tc_after();
+        issue_o(i, t, 1, true);
+        if (!CF::kOwnP && next < n_tiles) issue_s(i, next);  // in order behind the product that reads P from there
       }
-      if (!ok) {  // no product may be in flight when tensor memory is freed
-        volatile int ignore = 0;
-        mma_commit(drain);
-        mbar_wait(drain, 0, &ignore);
-      }
+      if (!any) break;
+    }
+    if (!ok && lane == 0) {  // no product may be in flight when tensor memory is freed
+      volatile int ignore = 0;
+      mma_commit(drain);
+      mbar_wait(drain, 0, &ignore);
     }
     __syncwarp();
   } else {
