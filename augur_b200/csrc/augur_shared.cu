@@ -779,11 +779,13 @@ __global__ void __launch_bounds__(kOwnThreads, OwnCfg<D>::kCtas) own_mma_kernel(
 // Tensor cores: the shared runs (tcgen05, accumulators in tensor memory)
 // ---------------------------------------------------------------------------
 //
-// One CTA per item: ten warps. Two groups of four warps each own a tile of
-// 128 query rows, one row a thread; warp 8 fetches K and V tiles of 128 keys
-// (TMA, one box per block and 64 dims, 128-byte swizzle; keys past the range
-// and bad block ids take an out-of-range block coordinate, which TMA fills
-// with zeros), warp 9 issues the products. Per tile: S = Q K^T into tensor
+// One CTA per item: 11 warps. Two groups of four warps each own a tile of
+// 128 query rows, one row a thread; warp 8 fetches K tiles of 128 keys and
+// warp 9 V tiles (TMA, one box a lane: a block's rows of 64 dims, with the
+// 128-byte swizzle; keys past the range and bad block ids take an out-of-range
+// block coordinate, which TMA fills with zeros), warp 10 issues the products.
+// (cp.async in TMA's place, by four warps, measured 133 against 107 us on 64 questions over
+// 98,304 tokens.) Per tile: S = Q K^T into tensor
 // memory (M = N = 128); each thread takes its row of S 32 columns at a time,
 // P = 2^(x - m) in the cache type goes back to tensor memory 64 keys at a time, and
 // O += P V takes P as its operand there and accumulates in tensor memory.
@@ -806,7 +808,7 @@ __global__ void __launch_bounds__(kOwnThreads, OwnCfg<D>::kCtas) own_mma_kernel(
 // Every wait is bounded (2 s of %globaltimer); on expiry the CTA records
 // AUGUR_KV_ETIMEOUT, drains its copies and products, frees its tensor memory and returns.
 
-constexpr int kShThreads = 320;
+constexpr int kShThreads = 352;
 constexpr int kTileKeys = 128;
 
 template <int D>
@@ -1013,36 +1015,8 @@ __global__ void __launch_bounds__(kShThreads, 1)
   const uint32_t drain = rest + 96u;
   static_assert(8 * (2 * CF::kKBufs + 2 * CF::kVBufs + 13) <= 256, "barriers");
 
-  // ---- K and V tiles: one box a lane
-  const int bs = a.block_size;
-  const int box = bs < kTileKeys ? bs : kTileKeys;  // rows of a TMA box
-  const int boxes = kTileKeys / box * CF::kHalves;  // boxes of a K or V tile: at most 32
-  auto fetch = [&](int t, bool v) {                 // warp 8; the buffer is free
-    const int j = lane / CF::kHalves, half = lane - j * CF::kHalves;
-    const int pos = it.key0 + t * kTileKeys + j * box;
-    int blk = -1, row = 0;
-    if (lane < boxes && pos < it.key1) {
-      const int lb = pos / bs;
-      row = pos - lb * bs;
-      blk = __ldg(a.run_blocks + it.block0 + lb);
-      if (blk < 0 || blk >= a.num_blocks) {
-        record_status(a.status, AUGUR_KV_EBOUNDS);
-        blk = -1;
-      }
-    }
-    const int at = blk >= 0 ? blk : int(a.num_blocks);  // past the pool: zeros
-    const int buf = t % (v ? CF::kVBufs : CF::kKBufs);
-    const uint32_t full = v ? v_full(buf) : k_full(buf);
-    if (lane == 0) mbar_expect(full, CF::kTileBytes);
-    __syncwarp();
-    if (lane < boxes)
-      tma_box(sb + (v ? CF::kV : CF::kK) + uint32_t(buf) * CF::kTileBytes + uint32_t(half) * (kTileKeys * 128) +
-                  uint32_t(j) * uint32_t(box) * 128u,
-              v ? &v_map : &k_map, full, half * 64, row, it.kv_head, at);
-  };
-  int n_k = min(n_tiles, CF::kKBufs), n_v = min(n_tiles, CF::kVBufs);  // tiles under way (warp 8)
-  if (warp == 8) {
-    if (lane == 0) {
+  if (warp == 10) {
+    if (elect_one()) {
       for (int i = 0; i < CF::kKBufs; ++i) {
         mbar_init(k_full(i), 1);
         mbar_init(k_empty(i), 1);
@@ -1065,67 +1039,76 @@ __global__ void __launch_bounds__(kShThreads, 1)
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     __syncwarp();
-    for (int t = 0; t < max(n_k, n_v); ++t) {  // the rings' first tiles, beside the rest of the start
-      if (t < n_k) fetch(t, false);
-      if (t < n_v) fetch(t, true);
-    }
-  }
-  if (warp == 9) {
+    asm volatile("bar.arrive 3, 96;" ::: "memory");  // the barriers are there: warps 8 and 9 may begin
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
                  "r"(CF::kCols)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  if (warp < 8) {  // the query rows, K-major with the 128-byte swizzle; rows past the run are zero
-    constexpr int CH = D / 8, kBatch = 8;
-    const int n_q = pair ? 256 : 128;
-    for (int p0 = tid; p0 < n_q * CH; p0 += 256 * kBatch) {
-      uint4 x[kBatch];
+  constexpr int CH = D / 8;  // 16-byte pieces of a row
+  // piece c of row r of a K, V or Q tile: 128-byte swizzle, 64 dims after 64 dims
+  auto place = [](int r, int c) { return uint32_t((c >> 3) * (kTileKeys * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)); };
+  if (warp < 8) {  // the query rows, K-major; rows past the run are zero
+    const char* mine = tid < (pair ? 256 : 128) ? query_row(a, it, it.row0 + tid) : nullptr;
+    const int64_t off = mine != nullptr ? mine - a.q : -1;
+    if (warp < (pair ? 8 : 4)) {
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const int p = p0 + i * 256, r = p / CH, c = p - r * CH;
-        const char* src = r < n_q ? query_row(a, it, it.row0 + r) : nullptr;
-        x[i] = make_uint4(0, 0, 0, 0);
-        if (src != nullptr) x[i] = __ldg(reinterpret_cast<const uint4*>(src + c * 16));
+      for (int j = 0; j < CH; ++j) {  // this warp's 32 rows, 32 / CH a step
+        const int rr = j * (32 / CH) + lane / CH, c = lane % CH;
+        const int64_t o = __shfl_sync(0xffffffffu, off, rr);
+        cp_async16(sb + CF::kQ + uint32_t(warp >> 2) * CF::kTileBytes + place((warp & 3) * 32 + rr, c),
+                   a.q + (o >= 0 ? o + c * 16 : 0), o >= 0 ? 16 : 0);
       }
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const int p = p0 + i * 256, r = p / CH, c = p - r * CH, rr = r & 127;
-        if (r < n_q)
-          *reinterpret_cast<uint4*>(smem + CF::kQ + (r >> 7) * CF::kTileBytes + (c >> 3) * (kTileKeys * 128) + rr * 128 +
-                                    (((c & 7) ^ (rr & 7)) << 4)) = x[i];
-      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   tc_before();
-  __syncthreads();
+  // the fetching warps need nothing of the others but the barriers, and do not wait here
+  if (warp == 8 || warp == 9) asm volatile("bar.sync 3, 96;" ::: "memory");
+  else asm volatile("bar.sync 2, 288;" ::: "memory");
   tc_after();
-  const uint32_t tmem = uint32_t(warp_uniform(int(tmem_slot)));
+  const uint32_t tmem = warp == 8 || warp == 9 ? 0u : uint32_t(warp_uniform(int(tmem_slot)));
 
-  if (warp == 8) {
+  if (warp == 8 || warp == 9) {
+    // ---- K tiles (warp 8) and V tiles (warp 9)
+    const bool v = warp == 9;
+    const CUtensorMap* map = v ? &v_map : &k_map;
+    const int bs = a.block_size, box = bs < kTileKeys ? bs : kTileKeys;  // rows of a box
+    const int boxes = kTileKeys / box * CF::kHalves;                     // of a tile: at most 32
+    const int my_box = lane / CF::kHalves, my_half = lane - my_box * CF::kHalves;
+    const int bufs = v ? CF::kVBufs : CF::kKBufs;
+    const uint32_t dst = sb + (v ? CF::kV : CF::kK) + uint32_t(my_half) * (kTileKeys * 128) + uint32_t(my_box) * uint32_t(box) * 128u;
+    auto full = [&](int i) { return v ? v_full(i) : k_full(i); };
+    auto block_of = [&](int t) -> int {  // this lane's block of tile t; past the keys or outside the pool: past the pool
+      const int pos = it.key0 + t * kTileKeys + my_box * box;
+      if (lane >= boxes || pos >= it.key1) return int(a.num_blocks);
+      const int blk = __ldg(a.run_blocks + it.block0 + pos / bs);
+      if (blk >= 0 && blk < a.num_blocks) return blk;
+      record_status(a.status, AUGUR_KV_EBOUNDS);
+      return int(a.num_blocks);
+    };
     bool ok = true;
-    for (int t = min(CF::kKBufs, CF::kVBufs); t < n_tiles && ok; ++t) {
-#pragma unroll
-      for (int v = 0; v < 2; ++v) {
-        const int bufs = v ? CF::kVBufs : CF::kKBufs;
-        if (t < bufs) continue;
-        ok = mbar_wait(v ? v_empty(t % bufs) : k_empty(t % bufs), uint32_t(t / bufs - 1) & 1u, &gave_up);
-        ok = __all_sync(0xffffffffu, ok);
+    int n = 0, next = block_of(0);
+    for (int t = 0; t < n_tiles; ++t) {
+      const int buf = t % bufs, blk = next;
+      if (t + 1 < n_tiles) next = block_of(t + 1);  // on its way while this tile waits for its place
+      if (t >= bufs) {
+        ok = __all_sync(0xffffffffu, mbar_wait(v ? v_empty(buf) : k_empty(buf), uint32_t(t / bufs - 1) & 1u, &gave_up));
         if (!ok) break;
-        fetch(t, v != 0);
-        if (v) n_v = t + 1;
-        else n_k = t + 1;
       }
+      if (elect_one()) mbar_expect(full(buf), CF::kTileBytes);
+      __syncwarp();
+      if (lane < boxes)
+        tma_box(dst + uint32_t(buf) * CF::kTileBytes, map, full(buf), my_half * 64,
+                bs > kTileKeys ? (it.key0 + t * kTileKeys) % bs : 0, it.kv_head, blk);
+      n = t + 1;
     }
     if (!ok) {  // no copy may be in flight when the CTA ends
       volatile int ignore = 0;
-      for (int i = max(0, n_k - CF::kKBufs); i < n_k; ++i)
-        mbar_wait(k_full(i % CF::kKBufs), uint32_t(i / CF::kKBufs) & 1u, &ignore);
-      for (int i = max(0, n_v - CF::kVBufs); i < n_v; ++i)
-        mbar_wait(v_full(i % CF::kVBufs), uint32_t(i / CF::kVBufs) & 1u, &ignore);
+      for (int i = max(0, n - bufs); i < n; ++i) mbar_wait(full(i % bufs), uint32_t(i / bufs) & 1u, &ignore);
     }
-  } else if (warp == 9) {
+  } else if (warp == 10) {
     // ---- the products. Group i's tiles are i, i + 2, .. (pair: all of them). The whole warp keeps step, so that
     // what the instructions take is uniform; one lane issues.
     constexpr uint32_t idesc_s = mma_desc<T>(kTileKeys, false), idesc_o = mma_desc<T>(D, true);
@@ -1182,16 +1165,14 @@ __global__ void __launch_bounds__(kShThreads, 1)
         if (!ok || t >= n_tiles) break;
         any = true;
         const int next = t + step;
-        if (i == 0 || !pair) {
-          ok = wait_v(t);
-          if (ok && next < n_tiles) ok = wait_k(next);
-        }
+        const bool first = i == 0 || !pair;  // to use the tiles
+        if (first) ok = wait_v(t);
         if (ok) ok = wait(p_full(i, 0), uint32_t(u) & 1u);
         if (!ok) break;
         tc_after();
         issue_o(i, t, 0, u > 0);
         if (CF::kOwnP && next < n_tiles) {
-          ok = wait(s_free(i), uint32_t(u) & 1u);
+          ok = wait(s_free(i), uint32_t(u) & 1u) && (!first || wait_k(next));
           if (!ok) break;
           tc_after();
           issue_s(i, next);
@@ -1200,7 +1181,12 @@ __global__ void __launch_bounds__(kShThreads, 1)
         if (!ok) break;
         tc_after();
         issue_o(i, t, 1, true);
-        if (!CF::kOwnP && next < n_tiles) issue_s(i, next);  // in order behind the product that reads P from there
+        if (!CF::kOwnP && next < n_tiles) {  // in order behind the product that reads P from there
+          ok = !first || wait_k(next);
+          if (!ok) break;
+          tc_after();
+          issue_s(i, next);
+        }
       }
       if (!any) break;
     }
@@ -1402,7 +1388,7 @@ __global__ void __launch_bounds__(kShThreads, 1)
   __syncthreads();
   tc_after();
   if (tid == 0 && gave_up) record_status(a.status, AUGUR_KV_ETIMEOUT);
-  if (warp == 9)
+  if (warp == 10)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(CF::kCols) : "memory");
 }
 
