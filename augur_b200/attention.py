@@ -355,8 +355,15 @@ def paged_attention(
 _ITEM_FIELDS = 12
 _TILE_ROWS = 128
 _TILE_KEYS = 128
-# A run is worth a pass of its own when the sequences would otherwise re-read this many positions
+# A run is worth items of its own when the sequences would otherwise re-read this many positions,
+# and a plan the launch that takes them when its runs spare this much reading (bytes of one layer's
+# K and V). Measured on 2 to 64 samples of 1 or 8 prompts of 256 to 16,384 positions, 14 query / 2
+# KV heads of 64 and 32 / 8 of 128: sparing 25 MB or less the one launch was the faster (10 against
+# 12 to 15 us for the shortest), from 63 MB on the two (15 against 17 us, 98 against 739 at the most)
 _MIN_SAVED_TOKENS = 256
+_MIN_SAVED_BYTES = 40_000_000
+# A work item's start and end, in steps of its loop (128 keys for up to 256 rows): about 10 us against 1.9 us
+_ITEM_STEPS = 5.0
 
 
 def _shared_runs(rows: np.ndarray, full: np.ndarray, min_saved: int) -> tuple[list[tuple[np.ndarray, int, int]], np.ndarray]:
@@ -396,17 +403,26 @@ def _shared_runs(rows: np.ndarray, full: np.ndarray, min_saved: int) -> tuple[li
     return runs, covered
 
 
-def _ranges(tiles: Sequence[int], units: Sequence[int], ctas: int, least: int) -> list[int]:
-    """Into how many key ranges each run's tiles are cut: tiles[i] key tiles, each range an
-    item for each of units[i] (row tiles x KV heads). The ranges are as short as one wave of
-    CTAs (one an SM) allows, but `least` tiles; where the runs alone exceed a wave, as long as
-    three waves make them, so that the last wave's waste is small."""
-    total = sum(t * u for t, u in zip(tiles, units))
-    waves = 1 if sum(units) <= ctas else 3
-    per = max(least, -(-total // (ctas * waves)))
-    while waves == 1 and sum(-(-t // per) * u for t, u in zip(tiles, units)) > ctas:
-        per += max(1, per // 16)
-    return [-(-t // per) for t in tiles]
+def _ranges(tiles: Sequence[int], units: Sequence[int], steps: Sequence[float], ctas: int, least: int) -> list[int]:
+    """Into how many key ranges each run's tiles are cut: tiles[i] key tiles, each range an item
+    for each of units[i] (row tiles x KV heads), steps[i] of a CTA's steps a tile.
+
+    An item costs its steps and a start and an end worth about _ITEM_STEPS more. With c items'
+    cost a CTA: one wave takes its longest item; several take their average and half an item.
+    The range length that this makes cheapest is taken, `least` tiles or more."""
+    if not tiles:
+        return []
+    best, longest = None, max(tiles)
+    lengths = sorted({max(least, -(-longest // n)) for n in (*range(1, 33), 40, 48, 64, 80, 96, 112, 128, ctas)}, reverse=True)
+    for per in lengths:
+        ranges = [-(-t // per) for t in tiles]
+        items = sum(n * u for n, u in zip(ranges, units))
+        most = max(-(-t // n) * s for t, n, s in zip(tiles, ranges, steps)) + _ITEM_STEPS
+        total = items * _ITEM_STEPS + sum(t * u * s for t, u, s in zip(tiles, units, steps))
+        cost = most if items <= ctas else total / ctas + most / 2
+        if best is None or cost < best[0]:
+            best = (cost, ranges)
+    return best[1]
 
 
 class SharedPrefixTables:
@@ -420,9 +436,12 @@ class SharedPrefixTables:
     """
 
     def __init__(self, cache: PagedKVCache, tables: Sequence[SequenceBlockTable], n_q_heads: int,
-                 seq_lens: Sequence[int] | None = None, stream: torch.cuda.Stream | None = None) -> None:
+                 seq_lens: Sequence[int] | None = None, stream: torch.cuda.Stream | None = None,
+                 min_saved_bytes: int | None = None) -> None:
         """stream: the stream the copy is ordered on (the current one by default); launches on
-        another stream wait for it."""
+        another stream wait for it. min_saved_bytes: how much reading (bytes of one layer) the
+        runs must spare to be taken apart; where they spare less, each sequence reads them
+        itself, which is then faster (None: the measured threshold)."""
         L, NB, Hkv, bs, D = cache.keys.shape
         if n_q_heads <= 0 or n_q_heads % Hkv != 0:
             raise ValueError("n_q_heads must be a positive multiple of the cache's KV heads")
@@ -437,6 +456,9 @@ class SharedPrefixTables:
         rows = packed[: B * width].reshape(B, width)
         lens_np = np.asarray(lens, dtype=np.int64)
         runs, covered = _shared_runs(rows, lens_np // bs, -(-_MIN_SAVED_TOKENS // bs))
+        spared = sum((m.size - 1) * (end - start) for m, start, end in runs) * bs
+        if spared * Hkv * D * 2 * cache.keys.element_size() < (_MIN_SAVED_BYTES if min_saved_bytes is None else min_saved_bytes):
+            runs, covered = [], np.zeros_like(covered)
         self.batch, self.n_q_heads, self.block_size = B, n_q_heads, bs
         self.max_seq_len = max(lens, default=0)
         self.shared_lens = covered * bs
@@ -445,8 +467,10 @@ class SharedPrefixTables:
         ctas = _sm_count(device)
         row_tiles = [-(-m.size * groups // _TILE_ROWS) for m, _, _ in runs]
         tiles = [-(-(end - start) * bs // _TILE_KEYS) for _, start, end in runs]
-        # a tensor-core item works on two key tiles at a time; the float32 kernel is slower a tile
-        ranges = _ranges(tiles, [-(-rt // 2) * Hkv for rt in row_tiles], ctas, 1 if cache.keys.dtype == torch.float32 else 2)
+        # a tensor-core item of one row tile works on two key tiles at a time; the float32 kernel is slower a tile
+        wide = cache.keys.dtype != torch.float32
+        ranges = _ranges(tiles, [-(-rt // 2) * Hkv for rt in row_tiles],
+                         [(0.5 if rt == 1 else 1.0) if wide else 8.0 for rt in row_tiles], ctas, 2 if wide else 1)
         items: list[tuple[int, ...]] = []
         refs: list[list[tuple[int, ...]]] = [[] for _ in range(B)]
         member0 = block0 = slab = 0

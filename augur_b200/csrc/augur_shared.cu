@@ -484,35 +484,133 @@ __global__ void __launch_bounds__(kGThreads) shared_generic_kernel(Args a) {
   }
 }
 
+// A unit's CTA (sequence, KV head, part): the part [first, last) of the sequence's own keys.
+__device__ __forceinline__ void part_range(const Args& a, int part, int step, int& first, int& last) {
+  const int steps = (last - first + step - 1) / step;
+  const int cut = (steps + a.n_split - 1) / a.n_split * step;
+  first = min(last, first + part * cut);
+  last = min(last, first + cut);
+}
+// A CTA whose part is in scratch arrives; true in the last one of its unit, which sees all the others'
+// parts (and leaves the counter zero). All threads call it.
+__device__ __forceinline__ bool last_to_arrive(const Args& a, int unit) {
+  __shared__ int is_last;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    is_last = atomicAdd(a.counters + unit, 1) == a.n_split - 1;
+    if (is_last) a.counters[unit] = 0;
+    __threadfence();
+  }
+  __syncthreads();
+  return is_last != 0;
+}
+
+// A sequence's own keys on CUDA cores. Eight warps share 32 keys in shared
+// memory; a warp takes query heads w, w + 8, ..: for the scores its lanes are the
+// keys, for P V the dims. Bound by the shared-memory reads, 2 D + D / 4 words a lane,
+// key and head.
 template <typename T>
 __global__ void __launch_bounds__(kGThreads) own_generic_kernel(Args a) {
   extern __shared__ __align__(16) float gsm[];
-  const int b = blockIdx.x / a.hkv, hk = blockIdx.x - b * a.hkv;
-  const int D = a.head_dim, P = generic_pitch(D), tid = threadIdx.x, r = tid >> 2, part = tid & 3;
+  constexpr int kHeads = kGRows / 8, kDims = kGMaxDim / 32;  // of a warp; of a lane
+  const int unit = blockIdx.x / a.n_split, part = blockIdx.x - unit * a.n_split;
+  const int b = unit / a.hkv, hk = unit - b * a.hkv;
+  const int D = a.head_dim, P = generic_pitch(D), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.groups;
+  float* sk = gsm + kGRows * P;
+  float* sv = sk + kGKeys * P;
+  float* ml = gsm + generic_floats(D);  // [64][2]; the queries' place takes the output rows
   int first, last;
   own_range(a, b, first, last);
-  for (int i = tid >> 5; i < kGRows; i += kGThreads / 32) {
-    const char* src = a.q + int64_t(b) * a.q_stride_b + int64_t(hk * a.groups + i) * a.q_stride_h;
-    for (int d = tid & 31; d < D; d += 32)
-      gsm[i * P + d] = i < a.groups ? Elem<T>::to_f(reinterpret_cast<const T*>(src)[d]) : 0.f;
+  part_range(a, part, kGKeys, first, last);
+  for (int i = warp; i < G; i += 8) {
+    const char* src = a.q + int64_t(b) * a.q_stride_b + int64_t(hk * G + i) * a.q_stride_h;
+    for (int d = lane; d < a.quads * 4; d += 32) gsm[i * P + d] = d < D ? Elem<T>::to_f(reinterpret_cast<const T*>(src)[d]) : 0.f;
   }
-  float m, l, o[kGMaxDim / 4];
-  generic_attend<T>(a, gsm, last - first, [&](int j) { return own_row(a, b, hk, first + j); }, m, l, o);
+  float m[kHeads], l[kHeads], o[kHeads][kDims];
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h) {
+    m[h] = kNegInf;
+    l[h] = 0.f;
+#pragma unroll
+    for (int c = 0; c < kDims; ++c) o[h][c] = 0.f;
+  }
+  for (int k0 = first; k0 < last; k0 += kGKeys) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kGKeys / 8; ++i) {  // a warp takes four keys' rows
+      const int key = warp * (kGKeys / 8) + i;
+      const int64_t off = k0 + key < last ? own_row(a, b, hk, k0 + key) : -1;
+      for (int d = lane; d < a.quads * 4; d += 32) {
+        const bool in = off >= 0 && d < D;
+        sk[key * P + d] = in ? Elem<T>::to_f(reinterpret_cast<const T*>(a.k + off)[d]) : 0.f;
+        sv[key * P + d] = in ? Elem<T>::to_f(reinterpret_cast<const T*>(a.v + off)[d]) : 0.f;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h) {
+      const int head = warp + 8 * h;
+      if (head >= G) break;
+      float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+      for (int d = 0; d < a.quads * 4; d += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(gsm + head * P + d);
+        const float4 y = *reinterpret_cast<const float4*>(sk + lane * P + d);
+        s0 = fmaf(x.x, y.x, s0);
+        s1 = fmaf(x.y, y.y, s1);
+        s2 = fmaf(x.z, y.z, s2);
+        s3 = fmaf(x.w, y.w, s3);
+      }
+      const float s = k0 + lane < last ? ((s0 + s1) + (s2 + s3)) * a.scale : kNegInf;
+      float mn = s;
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, x));
+      mn = fmaxf(mn, m[h]);
+      const float alpha = mn == kNegInf ? 1.f : ex2(m[h] - mn);
+      const float p = mn == kNegInf ? 0.f : ex2(s - mn);
+      m[h] = mn;
+      l[h] = l[h] * alpha + p;
+#pragma unroll
+      for (int c = 0; c < kDims; ++c) o[h][c] *= alpha;
+#pragma unroll 8
+      for (int j = 0; j < kGKeys; ++j) {
+        const float pj = __shfl_sync(0xffffffffu, p, j);
+#pragma unroll
+        for (int c = 0; c < kDims; ++c)
+          if (c * 32 < D) o[h][c] = fmaf(pj, sv[j * P + min(c * 32 + lane, D - 1)], o[h][c]);
+      }
+    }
+  }
   __syncthreads();
-  float* ml = gsm + generic_floats(D);  // [64][2]; the queries' place takes the output rows
-  if (r < a.groups) {
-    if (part == 0) {
-      ml[2 * r] = m;
-      ml[2 * r + 1] = l;
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h) {
+    const int head = warp + 8 * h;
+    if (head >= G) break;
+    float sum = l[h];
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    if (lane == 0) {
+      ml[2 * head] = m[h];
+      ml[2 * head + 1] = sum;
     }
 #pragma unroll
-    for (int i = 0; i < kGMaxDim / 16; ++i)
-      if (4 * i + part < a.quads)
-        *reinterpret_cast<float4*>(gsm + r * P + 16 * i + 4 * part) =
-            make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+    for (int c = 0; c < kDims; ++c)
+      if (c * 32 + lane < a.quads * 4) gsm[head * P + c * 32 + lane] = o[h][c];
   }
-  wait_prerequisites();  // the shared launch's slabs
-  join_rows<T>(a, b, hk, 1, ml, gsm, kGRows, P, ml + 2 * kGRows);
+  __syncthreads();
+  if (a.n_split == 1) {
+    wait_prerequisites();  // the shared launch's slabs
+    join_rows<T>(a, b, hk, 1, ml, gsm, kGRows, P, ml + 2 * kGRows);
+    return;
+  }
+  const int width = 4 * a.quads;
+  const int64_t base = (int64_t(unit) * a.n_split + part) * G;
+  for (int i = tid; i < G * width; i += kGThreads) a.split_o[base * width + i] = gsm[i / width * P + i % width];
+  for (int i = tid; i < 2 * G; i += kGThreads) a.split_ml[base * 2 + i] = ml[i];
+  if (!last_to_arrive(a, unit)) return;
+  wait_prerequisites();
+  const int64_t unit0 = int64_t(unit) * a.n_split * G;
+  join_rows<T>(a, b, hk, a.n_split, a.split_ml + unit0 * 2, a.split_o + unit0 * width, G, width, ml + 2 * kGRows);
 }
 
 // ---------------------------------------------------------------------------
@@ -568,19 +666,13 @@ template <typename T, int D, int NG>
 __global__ void __launch_bounds__(kOwnThreads, OwnCfg<D>::kCtas) own_mma_kernel(Args a) {
   using CF = OwnCfg<D>;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ int last_flag;
   constexpr int H = NG * 8;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int unit = blockIdx.x / a.n_split, part = blockIdx.x - unit * a.n_split;
   const int b = unit / a.hkv, hk = unit - b * a.hkv;
   int first, last;
   own_range(a, b, first, last);
-  {
-    const int stages = (last - first + kOwnTok - 1) / kOwnTok;
-    const int cut = (stages + a.n_split - 1) / a.n_split * kOwnTok;
-    first = min(last, first + part * cut);
-    last = min(last, first + cut);
-  }
+  part_range(a, part, kOwnTok, first, last);
   const int n_st = (last - first + kOwnTok - 1) / kOwnTok;
   const uint32_t ks_ = smem_u32(smem) + warp * 2 * CF::kTile, vs_ = ks_ + CF::kTile;
 
@@ -760,16 +852,7 @@ __global__ void __launch_bounds__(kOwnThreads, OwnCfg<D>::kCtas) own_mma_kernel(
     a.split_o[(base + h) * D + d] = x;
     if (d == 0) *reinterpret_cast<float2*>(a.split_ml + (base + h) * 2) = make_float2(m, l);
   }
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    const int seen = atomicAdd(a.counters + unit, 1);
-    last_flag = seen == a.n_split - 1;
-    if (last_flag) a.counters[unit] = 0;
-    __threadfence();
-  }
-  __syncthreads();
-  if (!last_flag) return;
+  if (!last_to_arrive(a, unit)) return;
   wait_prerequisites();
   const int64_t unit0 = int64_t(unit) * a.n_split * a.groups;
   join_rows<T>(a, b, hk, a.n_split, a.split_ml + unit0 * 2, a.split_o + unit0 * D, a.groups, D, join_mem);
@@ -800,10 +883,11 @@ __global__ void __launch_bounds__(kOwnThreads, OwnCfg<D>::kCtas) own_mma_kernel(
 // head_dim 64 P has columns of its own, so the next tile's S is computed
 // while this tile's exponentials are; at 128 P lies over S.
 //
-// Bound by the 16 exponentials a clock an SM has: a 256 x 128 tile needs 2,048
-// clocks of them, its products 1,024 (head_dim 64) or 2,048 (128). So every
-// second pair (head_dim 64), or every fourth (128), is computed on the FMA
-// pipes instead (exp2_poly2). With few rows it is bound by HBM.
+// A 256 x 128 tile needs 2,048 clocks of exponentials (16 a clock and SM), its
+// products 1,024 (head_dim 64) or 2,048 (128); it takes about 3,500, in which each
+// group spends 2,000 on its softmax and 1,400 waiting for its next S. (A
+// quarter or a half of the exponentials on the FMA pipes changed nothing, nor
+// did rows that lie in L2.) With few rows it is bound by HBM.
 //
 // Every wait is bounded (2 s of %globaltimer); on expiry the CTA records
 // AUGUR_KV_ETIMEOUT, drains its copies and products, frees its tensor memory and returns.
@@ -825,7 +909,6 @@ struct ShCfg {
   // tensor memory: S0, S1, then O0, O1 (and P0, P1; at head_dim 128 P lies over S)
   static constexpr bool kOwnP = D == 64;
   static constexpr uint32_t kS = 0, kO = 256, kP = kOwnP ? 256 + 2 * D : 0, kPStep = kOwnP ? 64 : 128, kCols = 512;
-  static constexpr int kPolyEvery = D == 64 ? 2 : 4;  // of so many pairs, one goes to the FMA pipes
 };
 
 __device__ __forceinline__ uint64_t global_ns() {
@@ -955,25 +1038,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-// 2^x and 2^y on the FMA pipes, for arguments at most 127 (below -126: 2^-126, a weight of nothing):
-// 2^x = 2^n 2^f with n = round(x) (the low bits of x + 1.5 2^23) and f in [-1/2, 1/2], and for 2^f the
-// polynomial of degree 4 whose largest relative error there is smallest (2.6e-6; found by exchange).
-__device__ __forceinline__ uint64_t exp2_poly2(float x, float y) {
-  const uint64_t v = pack2(fmaxf(x, -126.f), fmaxf(y, -126.f));
-  const uint64_t t = add2(v, pack2(12582912.f, 12582912.f));
-  const uint64_t n = add2(t, pack2(-12582912.f, -12582912.f));
-  const uint64_t f = fma2(n, pack2(-1.f, -1.f), v);
-  uint64_t p = fma2(f, pack2(0.009570102207362652f, 0.009570102207362652f), pack2(0.05591785907745361f, 0.05591785907745361f));
-  p = fma2(p, f, pack2(0.240247443318367f, 0.240247443318367f));
-  p = fma2(p, f, pack2(0.6931217908859253f, 0.6931217908859253f));
-  p = fma2(p, f, pack2(0.9999992847442627f, 0.9999992847442627f));
-  float p0, p1, t0, t1;
-  unpack2(p, p0, p1);
-  unpack2(t, t0, t1);
-  return pack2(__uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23)),
-               __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23)));
-}
-
 // A value that is the same in all lanes, in a form the compiler knows to be.
 __device__ __forceinline__ int warp_uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 // True in one lane of a converged warp.
@@ -1234,16 +1298,9 @@ __global__ void __launch_bounds__(kShThreads, 1)
       for (int j = 0; j < 16; ++j) {
         float x, y;
         unpack2(fma2(pack2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), scale2, neg2), x, y);
-        uint64_t e;
-        if (j % CF::kPolyEvery == CF::kPolyEvery - 1) {
-          e = exp2_poly2(x, y);
-          unpack2(e, x, y);
-        } else {
-          x = ex2(x);
-          y = ex2(y);
-          e = pack2(x, y);
-        }
-        sum = add2(sum, e);  // the sum takes the unrounded values; P V takes them rounded to the cache type
+        x = ex2(x);
+        y = ex2(y);
+        sum = add2(sum, pack2(x, y));  // the sum takes the unrounded values; P V takes them rounded to the cache type
         p[j] = Elem<T>::pack(x, y);
       }
     };
@@ -1494,7 +1551,7 @@ int run_generic(const Args& a, cudaStream_t st) {
   }
   const int rc = allow_smem(reinterpret_cast<const void*>(own_generic_kernel<T>), smem, done_o, "own_generic_kernel");
   if (rc != AUGUR_KV_OK) return rc;
-  return launch_own(own_generic_kernel<T>, a, a.batch * a.hkv, kGThreads, size_t(smem), a.n_items > 0, st, "own_generic_kernel");
+  return launch_own(own_generic_kernel<T>, a, a.batch * a.hkv * a.n_split, kGThreads, size_t(smem), a.n_items > 0, st, "own_generic_kernel");
 }
 
 // Parts of a sequence's own keys: enough CTAs for the GPU, and at least 128 keys a part.
@@ -1616,7 +1673,7 @@ AUGUR_KV_EXPORT int augur_kv_shared_prefix_attention(const augur_kv_shared_prefi
                 "KV head, 16-byte aligned rows and blocks of 8, 16, 32, 64 or a multiple of 128 tokens");
   const bool tensor = tensor_ok && p->flags != AUGUR_KV_ATTN_GENERIC;
   const int64_t units = int64_t(a.batch) * a.hkv;
-  a.n_split = tensor ? own_split(units, p->max_own_len) : 1;
+  a.n_split = own_split(units, p->max_own_len);
   {  // scratch: output rows of the slabs and of the parts, then their maxima and sums
     const int64_t slab_rows = int64_t(a.n_slabs) * kSlabRows;
     const int64_t part_rows = a.n_split > 1 ? units * a.n_split * a.groups : 0;

@@ -17,13 +17,19 @@ import pytest
 import torch
 
 import augur_b200 as ab
-from augur_b200 import _lib, _ops
+from augur_b200 import _lib, _ops, attention
 from augur_b200.attention import SharedPrefixTables, paged_decode_attention, paged_shared_prefix_attention
 from tests.conftest import poison_
 
 pytestmark = pytest.mark.gpu
 
 _UNIT = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+
+
+@pytest.fixture(autouse=True)
+def every_run_counts(monkeypatch):
+    """Runs are taken apart however little reading they spare, so that small cases reach the shared kernels."""
+    monkeypatch.setattr(attention, "_MIN_SAVED_BYTES", 0)
 
 
 class Case:
@@ -243,3 +249,15 @@ def test_refusals(cuda):
         paged_shared_prefix_attention(wide.q, wide.pool, wide.layer, wide.tables)
     empty = paged_shared_prefix_attention(case.q[:0], case.pool, case.layer, [])
     assert empty.shape == (0, 14, 1, 64)
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim", [(torch.bfloat16, 14, 2, 64), (torch.float16, 32, 8, 128), (torch.float32, 14, 2, 64),
+                                                      (torch.float32, 20, 4, 36), (torch.bfloat16, 64, 1, 80)])
+@pytest.mark.parametrize("name", _BATCHES)
+def test_runs_that_spare_little_are_read_by_each_sequence(cuda, monkeypatch, name, dtype, heads, kv_heads, dim):
+    """The plan without runs: every key is a sequence's own, long ones in several parts."""
+    monkeypatch.setattr(attention, "_MIN_SAVED_BYTES", 1 << 62)
+    case = Case(cuda, dtype, heads, kv_heads, dim, 16, _BATCHES[name], seed=4)
+    plan = SharedPrefixTables(case.pool, case.tables, heads)
+    assert plan.n_items == 0 and not plan.runs
+    case.check(paged_shared_prefix_attention(case.q, case.pool, case.layer, plan))

@@ -10,7 +10,14 @@ import pytest
 import torch
 
 import augur_b200 as ab
+from augur_b200 import attention
 from augur_b200.attention import SharedPrefixTables, paged_shared_prefix_attention
+
+
+@pytest.fixture(autouse=True)
+def every_run_counts(monkeypatch):
+    """Runs are taken apart however little reading they spare, so that small cases reach the shared kernels."""
+    monkeypatch.setattr(attention, "_MIN_SAVED_BYTES", 0)
 
 
 def _pool(bs, num_blocks, kv_heads=2, dim=64):
@@ -142,3 +149,14 @@ def test_refusals():
         paged_shared_prefix_attention(torch.zeros(1, 14, 2, 64), pool, 0, tables)
     with pytest.raises(ValueError, match="kernel must be"):
         paged_shared_prefix_attention(torch.zeros(1, 14, 64), pool, 0, tables, kernel="mma")
+
+
+def test_runs_must_spare_enough_reading():
+    pool = _pool(16, 200)
+    common = list(range(40))
+    tables = _tables(16, [(common + [100 + i], 641 + i) for i in range(5)])
+    spared = 4 * 640 * 2 * 64 * 2 * 4  # sequences, positions, KV heads, dims, K and V, bytes
+    assert SharedPrefixTables(pool, tables, 14, min_saved_bytes=spared).runs == [([0, 1, 2, 3, 4], 0, 640)]
+    plan = SharedPrefixTables(pool, tables, 14, min_saved_bytes=spared + 1)
+    assert plan.runs == [] and not plan.shared_lens.any() and plan.max_own_len == 645
+    _covered_keys(plan, pool, tables, 14)
