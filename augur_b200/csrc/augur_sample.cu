@@ -137,6 +137,15 @@ template <> struct Logit<__half> {
 
 __device__ __forceinline__ float no_nan(float x) { return x == x ? x : kNegInf; }  // a NaN is never drawn
 
+// floats as unsigned integers of the same order
+__device__ __forceinline__ uint32_t ordered(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float from_ordered(uint32_t o) {
+  return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
+}
+
 // The row's scale: z of an entry, its weight, and its key (bits of |z|: rising
 // keys are falling z; kDead for entries that can never be drawn).
 struct Scale {
@@ -192,8 +201,7 @@ __device__ __forceinline__ uint32_t bin_edge(int b) {
   return lo;
 }
 
-// The first position of CTA-wide running sums: found = the thread whose inclusive sum `incl` is the
-// first to reach goal (kBins if none does).
+// CTA-wide running sums, inclusive.
 __device__ __forceinline__ void scan_pair(Shared& sh, uint32_t n, unsigned long long m, uint32_t& cum_n,
                                           unsigned long long& cum_m) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -204,10 +212,9 @@ __device__ __forceinline__ void scan_pair(Shared& sh, uint32_t n, unsigned long 
     sh.warp_mass[warp] = cum_m;
   }
   __syncthreads();
-  for (int w = 0; w < warp; ++w) {
-    cum_n += sh.warp_count[w];
-    cum_m += sh.warp_mass[w];
-  }
+  const bool before = lane < warp;
+  cum_n += __reduce_add_sync(0xffffffffu, before ? sh.warp_count[lane] : 0u);
+  cum_m += warp_sum(before ? sh.warp_mass[lane] : 0ull);
   __syncthreads();
 }
 
@@ -245,6 +252,19 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
   const int C = int(cluster.num_blocks()), rank = int(cluster.block_rank());
   const int row = int(blockIdx.x) / C;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  // every CTA's value of one field, a lane each (lanes past the cluster: `none`): one exchange's latency, not C of them
+  auto of_lane = [&](auto field, auto none) { return lane < C ? field(*cluster.map_shared_rank(&sh, lane)) : none; };
+  // the sum over the cluster of one field for each thread: the loads go out together
+  auto cluster_sum = [&](auto field) {
+    decltype(field(sh)) v[kMaxCluster];
+#pragma unroll
+    for (int c = 0; c < kMaxCluster; ++c) v[c] = c < C ? field(*cluster.map_shared_rank(&sh, c)) : 0;
+    auto sum = v[0];
+#pragma unroll
+    for (int c = 1; c < kMaxCluster; ++c) sum += v[c];
+    return sum;
+  };
 
   // the part of the row this CTA holds, in 16-byte granules of memory: slot s is entry first + s
   const char* base = a.logits + int64_t(row) * a.row_stride;
@@ -312,8 +332,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
   }
   cluster.sync();
   Scale sc;
-  sc.m = kNegInf;
-  for (int c = 0; c < C; ++c) sc.m = fmaxf(sc.m, cluster.map_shared_rank(&sh, c)->cta_max);
+  sc.m = of_lane([](const Shared& o) { return o.cta_max; }, kNegInf);
+#pragma unroll
+  for (int o = kMaxCluster / 2; o > 0; o >>= 1) sc.m = fmaxf(sc.m, __shfl_xor_sync(0xffffffffu, sc.m, o));
+  sc.m = __shfl_sync(0xffffffffu, sc.m, 0);
   sc.greedy = !(temperature > 0.f);
   sc.inv = sc.greedy ? 0.f : 1.f / temperature;
   sc.plain = !sc.greedy && fabsf(sc.m) < INFINITY && sc.inv > 0.f && sc.inv < INFINITY;
@@ -360,10 +382,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
       sh.first = best;
     }
     cluster.sync();
-    if (rank == 0 && tid == 0) {
-      for (int c = 1; c < C; ++c) best = min(best, cluster.map_shared_rank(&sh, c)->first);
-      a.tokens[row] = int64_t(best);
-      if (a.logprobs) a.logprobs[row] = 0.f;
+    if (rank == 0 && warp == 0) {
+      best = __reduce_min_sync(0xffffffffu, of_lane([](const Shared& o) { return o.first; }, 0xffffffffu));
+      if (lane == 0) {
+        a.tokens[row] = int64_t(best);
+        if (a.logprobs) a.logprobs[row] = 0.f;
+      }
     }
     cluster.sync();
     return;
@@ -376,8 +400,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
     const float b = bin_of(sc.z(tmax));
     if (b < float(kBins)) atomicAdd(&sh.bin_count[int(b)], 1u);
     cluster.sync();
-    uint32_t n = 0;
-    for (int c = 0; c < C; ++c) n += cluster.map_shared_rank(&sh, c)->bin_count[tid];
+    const uint32_t n = cluster_sum([&](const Shared& o) { return o.bin_count[tid]; });
     if (tid == 0) sh.found = kBins;
     uint32_t cum_n;
     unsigned long long cum_m;
@@ -388,25 +411,23 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
     else cluster.sync();  // everyone has read the bins
   }
 
-  // Entries that `in` picks, into CTA 0's list in index order. Returns how many there are in the
+  // Entries with x in [low, high) (a high of NaN bounds nothing), into CTA 0's list in index order. Returns how many there are in the
   // cluster; only where they fit (kList) is the list filled, and only in CTA 0.
-  auto collect = [&](auto in) -> uint32_t {
+  auto collect = [&](float low, float high) -> uint32_t {
     uint32_t mine = 0;
     for (int s = w0 + lane * VEC; s < w1; s += kStep) {
       float f[VEC];
       load(s, f);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) mine += in(sc.z(f[j])) ? 1u : 0u;
+      for (int j = 0; j < VEC; ++j) mine += f[j] >= low && !(f[j] >= high) ? 1u : 0u;
     }
     mine = __reduce_add_sync(0xffffffffu, mine);
     if (lane == 0) sh.warp_count[warp] = mine;
     __syncthreads();
-    uint32_t before = 0, here_all = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      const uint32_t n = sh.warp_count[w];
-      before += w < warp ? n : 0;
-      here_all += n;
-    }
+    uint32_t before = lane < kWarps ? sh.warp_count[lane] : 0;
+    const uint32_t upto = warp_scan(before, lane);
+    const uint32_t here_all = __shfl_sync(0xffffffffu, upto, kWarps - 1);
+    before = __shfl_sync(0xffffffffu, upto, warp) - mine;
     if (tid == 0) sh.count = here_all;
     if (mine != 0 && here_all <= uint32_t(kList)) {
       for (int s0 = w0; s0 < w1; s0 += kStep) {
@@ -414,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
         load(s0 + lane * VEC, f);
         uint32_t bits = 0;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) bits |= in(sc.z(f[j])) ? 1u << j : 0u;
+        for (int j = 0; j < VEC; ++j) bits |= f[j] >= low && !(f[j] >= high) ? 1u << j : 0u;
         if (__ballot_sync(0xffffffffu, bits != 0) == 0) continue;
         const uint32_t incl = warp_scan(uint32_t(__popc(bits)), lane);
         uint32_t at = before + incl - __popc(bits);
@@ -427,19 +448,37 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
       }
     }
     cluster.sync();
-    uint32_t n_all = 0;
-    for (int c = 0; c < C; ++c) n_all += cluster.map_shared_rank(&sh, c)->count;
+    const uint32_t theirs = of_lane([](const Shared& o) { return o.count; }, 0u);
+    const uint32_t ends = warp_scan(theirs, lane);  // of the CTAs' entries, in the list
+    const uint32_t n_all = __shfl_sync(0xffffffffu, ends, kMaxCluster - 1);
     if (n_all <= uint32_t(kList) && rank == 0) {
-      uint32_t at = sh.count;
-      for (int c = 1; c < C; ++c) {
-        const uint32_t n = cluster.map_shared_rank(&sh, c)->count;
-        const unsigned long long* from = cluster.map_shared_rank(list, c);
-        for (uint32_t i = tid; i < n; i += kThreads) list[at + i] = from[i];
-        at += n;
+      for (uint32_t i0 = here_all; i0 < n_all; i0 += kThreads) {
+        const uint32_t i = i0 + tid;
+        int c = 0;
+        uint32_t start = 0;
+#pragma unroll
+        for (int x = 0; x < kMaxCluster - 1; ++x) {
+          const uint32_t end = __shfl_sync(0xffffffffu, ends, x);
+          if (i >= end && x < C - 1) {
+            c = x + 1;
+            start = end;
+          }
+        }
+        if (i < n_all) list[i] = cluster.map_shared_rank(list, c)[i - start];
       }
     }
     cluster.sync();
     return n_all;
+  };
+  // The smallest x whose entry has a key below `key` > 0 (up to the maximum, keys fall as x rises).
+  auto x_below = [&](uint32_t key) -> float {
+    uint32_t lo = ordered(kNegInf), hi = ordered(sc.m);  // the maximum's key is 0
+    while (lo < hi) {
+      const uint32_t mid = lo + (hi - lo) / 2;
+      if (key_of(sc.z(from_ordered(mid))) < key) hi = mid;
+      else lo = mid + 1;
+    }
+    return from_ordered(lo);
   };
   // CTA 0: the first n list entries sorted into `to`, padded to a power of two (returned).
   auto sort_list = [&](unsigned long long* to, int n) -> int {
@@ -506,9 +545,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
       }
     }
   };
+  // entries up to and with x = m (which may be infinite: the upper bound is left out)
+  auto collect_below = [&](uint32_t key) { return collect(x_below(key), NAN); };
   auto list_up_to = [&](int bin) -> bool {  // true: the row is done
-    const float end = float(bin + 1);
-    const uint32_t n = collect([&](float z) { return bin_of(z) < end; });
+    const uint32_t n = collect_below(bin_edge(bin + 1));
     if (n > uint32_t(kList)) return false;
     if (rank == 0) draw_from_list(int(n));  // from CTA 0's memory alone
     return true;
@@ -542,13 +582,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
         }
       }
       cluster.sync();
-      n = 0;
-      m = 0;
-      for (int c = 0; c < C; ++c) {
-        const Shared* o = cluster.map_shared_rank(&sh, c);
-        n += o->bin_count[tid];
-        m += (unsigned long long)o->bin_lo[tid] + ((unsigned long long)o->bin_hi[tid] << (kResident ? 16 : 32));
-      }
+      n = cluster_sum([&](const Shared& o) { return o.bin_count[tid]; });
+      m = cluster_sum([&](const Shared& o) {
+        return (unsigned long long)o.bin_lo[tid] + ((unsigned long long)o.bin_hi[tid] << (kResident ? 16 : 32));
+      });
       scan_pair(sh, n, m, cum_n, cum_m);
       cluster.sync();  // everyone has read the bins
     };
@@ -595,10 +632,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
         cut_ties = uint32_t(ties);
         return below_m + w * ties;
       }
-      collect([&](float z) {
-        const uint32_t key = key_of(z);
-        return key >= lo && key < hi;
-      });
+      collect(x_below(hi), lo == 0 ? NAN : x_below(lo));
       if (rank == 0) {  // sorted in place: the part is still needed
         int np = 32;
         while (np < int(in_n)) np <<= 1;
@@ -691,8 +725,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
       sh.ties = n;
     }
     cluster.sync();
-    for (int c = 0; c < rank; ++c) tie0 += cluster.map_shared_rank(&sh, c)->ties;
-    for (int w = 0; w < warp; ++w) tie0 += sh.warp_count[w];
+    const uint32_t theirs = of_lane([](const Shared& o) { return o.ties; }, 0u);
+    tie0 = __reduce_add_sync(0xffffffffu, lane < rank ? theirs : 0u) +
+           __reduce_add_sync(0xffffffffu, lane < warp ? sh.warp_count[lane] : 0u);
   }
   // the kept weights of this lane's slots (an entry without weight is never kept); advances the warp's tie count
   auto kept = [&](int s, uint32_t& ties, uint32_t* w) -> unsigned long long {
@@ -749,14 +784,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
     sh.mass = m;
   }
   cluster.sync();
-  unsigned long long whole = 0, before = 0;
-  for (int c = 0; c < C; ++c) {
-    const unsigned long long m = cluster.map_shared_rank(&sh, c)->mass;
-    before += c < rank ? m : 0;
-    whole += m;
-  }
-  const unsigned long long target = draw_target(u, whole);
-  for (int w = 0; w < warp; ++w) before += sh.warp_mass[w];
+  const unsigned long long theirs = of_lane([](const Shared& o) { return o.mass; }, 0ull);
+  const unsigned long long whole = warp_sum(theirs), target = draw_target(u, whole);
+  unsigned long long before = warp_sum((lane < rank ? theirs : 0ull) + (lane < warp ? sh.warp_mass[lane] : 0ull));
   if (before <= target && target < before + sh.warp_mass[warp]) {
     uint32_t ties = tie0;
     for (int s0 = w0; s0 < w1; s0 += kStep) {

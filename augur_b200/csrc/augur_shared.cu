@@ -508,12 +508,13 @@ __device__ __forceinline__ bool last_to_arrive(const Args& a, int unit) {
 
 // A sequence's own keys on CUDA cores. Eight warps share 32 keys in shared
 // memory; a warp takes query heads w, w + 8, ..: for the scores its lanes are the
-// keys, for P V the dims. Bound by the shared-memory reads, 2 D + D / 4 words a lane,
-// key and head.
-template <typename T>
+// keys, for P V the dims (kDims = head_dim / 32 of them a lane, rounded up to 2, 4 or 8).
+// The next 32 keys' rows are on their way to registers meanwhile. Bound by the
+// latency of those loads with few heads, by shared-memory reads with many.
+template <typename T, int kDims>
 __global__ void __launch_bounds__(kGThreads) own_generic_kernel(Args a) {
   extern __shared__ __align__(16) float gsm[];
-  constexpr int kHeads = kGRows / 8, kDims = kGMaxDim / 32;  // of a warp; of a lane
+  constexpr int kHeads = kDims == 8 ? 4 : 8;  // of a warp: heads x dims at most 8,192
   const int unit = blockIdx.x / a.n_split, part = blockIdx.x - unit * a.n_split;
   const int b = unit / a.hkv, hk = unit - b * a.hkv;
   const int D = a.head_dim, P = generic_pitch(D), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.groups;
@@ -535,18 +536,41 @@ __global__ void __launch_bounds__(kGThreads) own_generic_kernel(Args a) {
 #pragma unroll
     for (int c = 0; c < kDims; ++c) o[h][c] = 0.f;
   }
+  constexpr int kKeys = kGKeys / 8;  // a warp fetches four keys' rows
+  T kr[kKeys][kDims], vr[kKeys][kDims];
+  bool there[kKeys];
+  auto fetch = [&](int k0) {
+    const int key = k0 + warp * kKeys + lane;
+    const int64_t mine = lane < kKeys && key < last ? own_row(a, b, hk, key) : -1;
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i) {
+      const int64_t off = __shfl_sync(0xffffffffu, mine, i);
+      there[i] = off >= 0;
+#pragma unroll
+      for (int c = 0; c < kDims; ++c) {
+        const int d = min(c * 32 + lane, D - 1);  // in the row even where it is not used
+        kr[i][c] = reinterpret_cast<const T*>(a.k + max(off, int64_t(0)))[d];
+        vr[i][c] = reinterpret_cast<const T*>(a.v + max(off, int64_t(0)))[d];
+      }
+    }
+  };
+  if (first < last) fetch(first);
   for (int k0 = first; k0 < last; k0 += kGKeys) {
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kGKeys / 8; ++i) {  // a warp takes four keys' rows
-      const int key = warp * (kGKeys / 8) + i;
-      const int64_t off = k0 + key < last ? own_row(a, b, hk, k0 + key) : -1;
-      for (int d = lane; d < a.quads * 4; d += 32) {
-        const bool in = off >= 0 && d < D;
-        sk[key * P + d] = in ? Elem<T>::to_f(reinterpret_cast<const T*>(a.k + off)[d]) : 0.f;
-        sv[key * P + d] = in ? Elem<T>::to_f(reinterpret_cast<const T*>(a.v + off)[d]) : 0.f;
+    for (int i = 0; i < kKeys; ++i) {
+      const int key = warp * kKeys + i;
+#pragma unroll
+      for (int c = 0; c < kDims; ++c) {
+        const int d = c * 32 + lane;
+        const bool in = there[i] && d < D;
+        if (d < a.quads * 4) {
+          sk[key * P + d] = in ? Elem<T>::to_f(kr[i][c]) : 0.f;
+          sv[key * P + d] = in ? Elem<T>::to_f(vr[i][c]) : 0.f;
+        }
       }
     }
+    if (k0 + kGKeys < last) fetch(k0 + kGKeys);
     __syncthreads();
 #pragma unroll
     for (int h = 0; h < kHeads; ++h) {
@@ -577,7 +601,7 @@ __global__ void __launch_bounds__(kGThreads) own_generic_kernel(Args a) {
         const float pj = __shfl_sync(0xffffffffu, p, j);
 #pragma unroll
         for (int c = 0; c < kDims; ++c)
-          if (c * 32 < D) o[h][c] = fmaf(pj, sv[j * P + min(c * 32 + lane, D - 1)], o[h][c]);
+          o[h][c] = fmaf(pj, sv[j * P + min(c * 32 + lane, D - 1)], o[h][c]);
       }
     }
   }
@@ -1541,7 +1565,7 @@ template <typename T>
 int run_generic(const Args& a, cudaStream_t st) {
   const int shared = generic_floats(a.head_dim) * 4;
   const int smem = shared + 2 * kGRows * 4 + join_bytes(a.groups);
-  static int done_s[augur_kv_dev::kMaxDevices] = {0}, done_o[augur_kv_dev::kMaxDevices] = {0};
+  static int done_s[augur_kv_dev::kMaxDevices] = {0}, done_o[3][augur_kv_dev::kMaxDevices] = {{0}};
   if (a.n_items > 0) {
     const int rc = allow_smem(reinterpret_cast<const void*>(shared_generic_kernel<T>), shared, done_s, "shared_generic_kernel");
     if (rc != AUGUR_KV_OK) return rc;
@@ -1549,16 +1573,23 @@ int run_generic(const Args& a, cudaStream_t st) {
     const int lc = augur_kv_dev::check_launch("shared_generic_kernel");
     if (lc != AUGUR_KV_OK) return lc;
   }
-  const int rc = allow_smem(reinterpret_cast<const void*>(own_generic_kernel<T>), smem, done_o, "own_generic_kernel");
-  if (rc != AUGUR_KV_OK) return rc;
-  return launch_own(own_generic_kernel<T>, a, a.batch * a.hkv * a.n_split, kGThreads, size_t(smem), a.n_items > 0, st, "own_generic_kernel");
+  auto own = [&](auto kernel, int (&done)[augur_kv_dev::kMaxDevices]) {
+    const int rc = allow_smem(reinterpret_cast<const void*>(kernel), smem, done, "own_generic_kernel");
+    if (rc != AUGUR_KV_OK) return rc;
+    return launch_own(kernel, a, a.batch * a.hkv * a.n_split, kGThreads, size_t(smem), a.n_items > 0, st, "own_generic_kernel");
+  };
+  if (a.head_dim <= 64) return own(own_generic_kernel<T, 2>, done_o[0]);
+  if (a.head_dim <= 128) return own(own_generic_kernel<T, 4>, done_o[1]);
+  return own(own_generic_kernel<T, 8>, done_o[2]);
 }
 
-// Parts of a sequence's own keys: enough CTAs for the GPU, and at least 128 keys a part.
-int own_split(int64_t units, int64_t max_own) {
+// Parts of a sequence's own keys: enough CTAs for the GPU, and at least `least` keys a part
+// (a stage of each warp on the tensor cores; two tiles on CUDA cores).
+constexpr int kLeastTensor = kOwnWarps * kOwnTok, kLeastGeneric = 2 * kGKeys;
+int own_split(int64_t units, int64_t max_own, int least) {
   const int64_t slots = int64_t(augur_kv_dev::sm_count()) * 2;
   int64_t n = units > 0 ? slots / units : 1;
-  const int64_t most = max_own / 128;
+  const int64_t most = max_own / least;
   if (n > most) n = most;
   if (n > 32) n = 32;
   return int(n < 1 ? 1 : n);
@@ -1577,7 +1608,7 @@ AUGUR_KV_EXPORT int augur_kv_shared_prefix_workspace(int32_t n_slabs, int32_t ba
       max_own_len < 0 || counters_bytes == nullptr || scratch_bytes == nullptr)
     return augur_kv_dev::fail(AUGUR_KV_EINVAL, "shared_prefix_workspace: bad arguments");
   const int64_t units = int64_t(batch) * n_kv_heads;
-  const int split = own_split(units, max_own_len);
+  const int split = own_split(units, max_own_len, kLeastGeneric);  // at least what either path takes
   const int64_t rows = int64_t(n_slabs) * kSlabRows + (split > 1 ? units * split * (n_q_heads / n_kv_heads) : 0);
   *counters_bytes = split > 1 ? units * 4 : 0;
   *scratch_bytes = rows * (int64_t((head_dim + 3) / 4 * 4) + 2) * 4 + 64;
@@ -1673,7 +1704,7 @@ AUGUR_KV_EXPORT int augur_kv_shared_prefix_attention(const augur_kv_shared_prefi
                 "KV head, 16-byte aligned rows and blocks of 8, 16, 32, 64 or a multiple of 128 tokens");
   const bool tensor = tensor_ok && p->flags != AUGUR_KV_ATTN_GENERIC;
   const int64_t units = int64_t(a.batch) * a.hkv;
-  a.n_split = own_split(units, p->max_own_len);
+  a.n_split = own_split(units, p->max_own_len, tensor ? kLeastTensor : kLeastGeneric);
   {  // scratch: output rows of the slabs and of the parts, then their maxima and sums
     const int64_t slab_rows = int64_t(a.n_slabs) * kSlabRows;
     const int64_t part_rows = a.n_split > 1 ? units * a.n_split * a.groups : 0;
