@@ -84,6 +84,7 @@ struct Shared {
   unsigned long long warp_mass[kWarps];
   // histogram; masses in halves of 16 bits (a part has at most 65,536 entries), or whole where it has more
   uint32_t bin_count[kBins], bin_lo[kBins], bin_hi[kBins];
+  unsigned long long depth_mass[kWarps][4], cta_depth_mass[4];  // within some depths of the maximum, and in all
   // results of a step, written by one thread; cut: by CTA 0 for the cluster
   uint32_t found, found_n;
   unsigned long long found_m, found_bin_m;
@@ -190,15 +191,25 @@ __device__ __forceinline__ unsigned long long draw_target(float u, unsigned long
 }
 
 __device__ __forceinline__ float bin_of(float z) { return fabsf(z) * kBinScale; }
+// The smallest value in [lo, hi) for which `pred`, which turns true once, holds (hi if none). A warp
+// tries 32 values a step.
+template <typename F>
+__device__ __forceinline__ uint32_t first_true(uint32_t lo, uint32_t hi, F pred) {
+  const uint32_t lane = threadIdx.x & 31;
+  while (lo < hi) {
+    const uint32_t step = (hi - lo + 31) / 32, at = lo + lane * step;  // lane 0 tries lo, the last ones may pass hi
+    const uint32_t yes = __ballot_sync(0xffffffffu, at >= hi || at < lo || pred(at));
+    const uint32_t f = yes ? uint32_t(__ffs(yes)) - 1 : 32u;
+    if (f == 0) return lo;
+    const uint32_t below = lo + (f - 1) * step;  // false there
+    if (f < 32 && below < hi - step) hi = lo + f * step;  // true there
+    lo = below + 1;
+  }
+  return hi;
+}
 // The smallest key whose bin is b or above.
 __device__ __forceinline__ uint32_t bin_edge(int b) {
-  uint32_t lo = 0, hi = kDead;  // the key of an infinite |z| is past every bin
-  while (lo < hi) {
-    const uint32_t mid = lo + (hi - lo) / 2;
-    if (__uint_as_float(mid) * kBinScale >= float(b)) hi = mid;
-    else lo = mid + 1;
-  }
-  return lo;
+  return first_true(0u, kDead, [&](uint32_t key) { return __uint_as_float(key) * kBinScale >= float(b); });
 }
 
 // CTA-wide running sums, inclusive.
@@ -218,21 +229,53 @@ __device__ __forceinline__ void scan_pair(Shared& sh, uint32_t n, unsigned long 
   __syncthreads();
 }
 
-// Sorts n entries (a power of two from 32 on) in shared memory, rising.
-__device__ __forceinline__ void sort_entries(unsigned long long* e, int n) {
-  for (int size = 2; size <= n; size <<= 1) {
-    for (int stride = size >> 1; stride > 0; stride >>= 1) {
-      for (int p = threadIdx.x; p < n / 2; p += kThreads) {
-        const int i = ((p & ~(stride - 1)) << 1) | (p & (stride - 1)), j = i + stride;
-        const unsigned long long x = e[i], y = e[j];
-        if ((x > y) == ((i & size) == 0)) {
-          e[i] = y;
-          e[j] = x;
-        }
-      }
-      __syncthreads();
+// Sorts n entries (at most kList) from `from` to `to` (which may be the same), rising: `bin` is a rising
+// function of the key with values below kBins; entries find their bin's place, then their rank in the
+// bin by comparing.
+template <typename F>
+__device__ __forceinline__ void sort_entries(Shared& sh, const unsigned long long* from, unsigned long long* to, int n, F bin) {
+  constexpr int kPer = kList / kThreads;
+  const int tid = threadIdx.x;
+  unsigned long long e[kPer];
+  int b[kPer];
+  sh.bin_count[tid] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const int i = tid + j * kThreads;
+    b[j] = -1;
+    if (i < n) {
+      e[j] = from[i];
+      b[j] = bin(uint32_t(e[j] >> 32));
+      atomicAdd(&sh.bin_count[b[j]], 1u);
     }
   }
+  __syncthreads();
+  const uint32_t c = sh.bin_count[tid];
+  uint32_t cum;
+  unsigned long long none;
+  scan_pair(sh, c, 0ull, cum, none);
+  sh.bin_lo[tid] = cum - c;  // the bin's first place
+  sh.bin_hi[tid] = 0;        // of it taken
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kPer; ++j)
+    if (b[j] >= 0) to[sh.bin_lo[b[j]] + atomicAdd(&sh.bin_hi[b[j]], 1u)] = e[j];
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    if (b[j] >= 0) {
+      const uint32_t start = sh.bin_lo[b[j]], count = sh.bin_count[b[j]];
+      uint32_t rank = 0;
+      for (uint32_t x = 0; x < count; ++x) rank += to[start + x] < e[j] ? 1u : 0u;
+      b[j] = int(start + rank);
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kPer; ++j)
+    if (b[j] >= 0) to[b[j]] = e[j];
+  __syncthreads();
 }
 
 template <typename T, bool kResident>
@@ -411,15 +454,25 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
     else cluster.sync();  // everyone has read the bins
   }
 
-  // Entries with x in [low, high) (a high of NaN bounds nothing), into CTA 0's list in index order. Returns how many there are in the
-  // cluster; only where they fit (kList) is the list filled, and only in CTA 0.
-  auto collect = [&](float low, float high) -> uint32_t {
+  // Entries with x in [low, high) (all up to the maximum where `open`), into CTA 0's list in index order.
+  // Returns how many there are in the cluster; only where they fit (kList) is the list filled, and only in CTA 0.
+  auto collect = [&](float low, float high, bool open) -> uint32_t {
     uint32_t mine = 0;
-    for (int s = w0 + lane * VEC; s < w1; s += kStep) {
-      float f[VEC];
-      load(s, f);
+    auto in = [&](float x) { return x >= low && (open || x < high); };  // never a NaN
+    if (open) {
+      for (int g = w0 / VEC + lane; g < w1 / VEC; g += 32) {
+        float f[VEC];
+        granule(g, f);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) mine += f[j] >= low && !(f[j] >= high) ? 1u : 0u;
+        for (int j = 0; j < VEC; ++j) mine += f[j] >= low ? 1u : 0u;
+      }
+    } else {
+      for (int g = w0 / VEC + lane; g < w1 / VEC; g += 32) {
+        float f[VEC];
+        granule(g, f);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) mine += f[j] >= low && f[j] < high ? 1u : 0u;
+      }
     }
     mine = __reduce_add_sync(0xffffffffu, mine);
     if (lane == 0) sh.warp_count[warp] = mine;
@@ -435,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
         load(s0 + lane * VEC, f);
         uint32_t bits = 0;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) bits |= f[j] >= low && !(f[j] >= high) ? 1u << j : 0u;
+        for (int j = 0; j < VEC; ++j) bits |= in(f[j]) ? 1u << j : 0u;
         if (__ballot_sync(0xffffffffu, bits != 0) == 0) continue;
         const uint32_t incl = warp_scan(uint32_t(__popc(bits)), lane);
         uint32_t at = before + incl - __popc(bits);
@@ -470,28 +523,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
     cluster.sync();
     return n_all;
   };
-  // The smallest x whose entry has a key below `key` > 0 (up to the maximum, keys fall as x rises).
-  auto x_below = [&](uint32_t key) -> float {
-    uint32_t lo = ordered(kNegInf), hi = ordered(sc.m);  // the maximum's key is 0
-    while (lo < hi) {
-      const uint32_t mid = lo + (hi - lo) / 2;
-      if (key_of(sc.z(from_ordered(mid))) < key) hi = mid;
-      else lo = mid + 1;
-    }
-    return from_ordered(lo);
-  };
-  // CTA 0: the first n list entries sorted into `to`, padded to a power of two (returned).
-  auto sort_list = [&](unsigned long long* to, int n) -> int {
-    int np = 32;
-    while (np < n) np <<= 1;
-    for (int i = tid; i < np; i += kThreads) to[i] = i < n ? list[i] : ~0ull;
-    __syncthreads();
-    sort_entries(to, np);
-    return np;
+  // The smallest x whose key passes `pred` (up to the maximum, keys fall as x rises; the maximum's, 0, passes).
+  auto x_first = [&](auto pred) -> float {
+    return from_ordered(first_true(ordered(kNegInf), ordered(sc.m), [&](uint32_t o) { return pred(key_of(sc.z(from_ordered(o)))); }));
   };
   // CTA 0: draws from the list, which holds all that can be drawn, and writes the row's result.
   auto draw_from_list = [&](int n) {
-    sort_list(sorted, n);
+    sort_entries(sh, list, sorted, n, [](uint32_t key) { return min(int(__uint_as_float(key) * kBinScale), kBins - 1); });
     // falling z: the weights' running sums, kPer neighbours a thread
     unsigned long long w[kPer], sum = 0, run, none;
     uint32_t zero;
@@ -545,10 +583,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
       }
     }
   };
-  // entries up to and with x = m (which may be infinite: the upper bound is left out)
-  auto collect_below = [&](uint32_t key) { return collect(x_below(key), NAN); };
   auto list_up_to = [&](int bin) -> bool {  // true: the row is done
-    const uint32_t n = collect_below(bin_edge(bin + 1));
+    const float end = float(bin + 1);
+    const uint32_t n = collect(x_first([&](uint32_t key) { return __uint_as_float(key) * kBinScale < end; }), 0.f, true);
     if (n > uint32_t(kList)) return false;
     if (rank == 0) draw_from_list(int(n));  // from CTA 0's memory alone
     return true;
@@ -567,7 +604,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           const float z = sc.z(f[j]);
-          const int b = bin(z);
+          const int b = bin(f[j], z);
           if (b < 0) continue;
           atomicAdd(&sh.bin_count[b], 1u);
           if (!use_p) continue;
@@ -616,7 +653,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
         while ((hi - lo - 1) >> shift >= uint32_t(kBins)) ++shift;
         uint32_t n, cum_n;
         unsigned long long m, cum_m;
-        histogram([&](float z) {
+        histogram([&](float, float z) {
           const uint32_t key = key_of(z);
           return key >= lo && key < hi ? int((key - lo) >> shift) : -1;
         }, n, m, cum_n, cum_m);
@@ -632,14 +669,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
         cut_ties = uint32_t(ties);
         return below_m + w * ties;
       }
-      collect(x_below(hi), lo == 0 ? NAN : x_below(lo));
+      collect(x_first([&](uint32_t key) { return key < hi; }), lo == 0 ? 0.f : x_first([&](uint32_t key) { return key < lo; }),
+              lo == 0);
       if (rank == 0) {  // sorted in place: the part is still needed
-        int np = 32;
-        while (np < int(in_n)) np <<= 1;
-        for (int i = tid; i < np; i += kThreads)
-          if (i >= int(in_n)) list[i] = ~0ull;
-        __syncthreads();
-        sort_entries(list, np);
+        int shift = 0;
+        while ((hi - lo - 1) >> shift >= uint32_t(kBins)) ++shift;
+        sort_entries(sh, list, list, int(in_n), [&](uint32_t key) { return int((key - lo) >> shift); });
         unsigned long long w[kPer], sum = 0, run;
         uint32_t zero;
 #pragma unroll
@@ -676,16 +711,58 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
 
     uint32_t n, cum_n, in_n;
     unsigned long long m, cum_m;
-    histogram([&](float z) {
+    float reach = kNegInf;  // the histogram takes entries from here on
+    if (!use_k) {
+      // top-p alone: the row's mass, and a depth that holds the nucleus, so that the histogram's atomics are
+      // spent on few entries
+      constexpr int kDepths = 3;
+      const float depth[kDepths] = {4.f, 8.f, 13.f};
+      unsigned long long sum[kDepths + 1] = {0, 0, 0, 0};
+      for (int g = w0 / VEC + lane; g < w1 / VEC; g += 32) {
+        float f[VEC];
+        granule(g, f);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float z = sc.z(no_nan(f[j]));
+          const uint32_t w = weight(expf(z));
+          sum[kDepths] += w;
+#pragma unroll
+          for (int d = 0; d < kDepths; ++d) sum[d] += z >= -depth[d] ? w : 0u;
+        }
+      }
+#pragma unroll
+      for (int d = 0; d <= kDepths; ++d) sum[d] = warp_sum(sum[d]);
+      __syncthreads();
+      if (lane == 0) {
+#pragma unroll
+        for (int d = 0; d <= kDepths; ++d) sh.depth_mass[warp][d] = sum[d];
+      }
+      __syncthreads();
+      if (tid <= kDepths) {
+        unsigned long long all = 0;
+        for (int w = 0; w < kWarps; ++w) all += sh.depth_mass[w][tid];
+        sh.cta_depth_mass[tid] = all;
+      }
+      cluster.sync();
+#pragma unroll
+      for (int d = 0; d <= kDepths; ++d) sum[d] = warp_sum(of_lane([&](const Shared& o) { return o.cta_depth_mass[d]; }, 0ull));
+      total = sum[kDepths];
+      const unsigned long long need = mass_needed(top_p, total);
+#pragma unroll
+      for (int d = kDepths - 1; d >= 0; --d)
+        if (sum[d] >= need) reach = -depth[d];
+      if (reach > kNegInf) reach = x_first([&](uint32_t key) { return __uint_as_float(key) <= -reach; });
+    }
+    histogram([&](float x, float z) {
       const float b = bin_of(z);
-      return b < float(kBins) ? int(b) : -1;
+      return x >= reach && b < float(kBins) ? int(b) : -1;
     }, n, m, cum_n, cum_m);
     if (tid == kThreads - 1) {
       sh.found_n = cum_n;
       sh.found_m = cum_m;
     }
     __syncthreads();
-    total = sh.found_m;
+    if (use_k) total = sh.found_m;
     use_k = use_k && sh.found_n > uint32_t(k);  // entries past the bins have no weight
     if (use_k || use_p) {
       unsigned long long below_n = 0, below_m = 0;
@@ -707,12 +784,24 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
 
   // ---- walk the row: where this CTA's and this warp's ties begin, then the kept mass
   const bool limit_ties = cut_ties != 0xffffffffu;
+  // entries below this are not kept: most of a warp's steps hold none of the others
+  const float x_cut = x_first([&](uint32_t key) {
+    const float e = expf(z_of(key));
+    return key <= cut_key && !(e < min_p) && weight(e) != 0;
+  });
+  auto any_from = [&](const float* f) {
+    float most = f[0];
+#pragma unroll
+    for (int j = 1; j < VEC; ++j) most = fmaxf(most, f[j]);
+    return __any_sync(0xffffffffu, most >= x_cut);
+  };
   uint32_t tie0 = 0;
   if (limit_ties) {
     uint32_t mine = 0;
-    for (int s = w0 + lane * VEC; s < w1; s += kStep) {
+    for (int s0 = w0; s0 < w1; s0 += kStep) {
       float f[VEC];
-      load(s, f);
+      load(s0 + lane * VEC, f);
+      if (!any_from(f)) continue;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) mine += key_of(sc.z(f[j])) == cut_key ? 1u : 0u;
     }
@@ -734,6 +823,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
     float f[VEC];
     load(s, f);
     unsigned long long sum = 0;
+    if (!any_from(f)) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) w[j] = 0;
+      return 0;
+    }
     if (!limit_ties) {
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
