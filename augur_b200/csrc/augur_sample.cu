@@ -83,11 +83,11 @@ struct Shared {
   uint32_t warp_count[kWarps];
   unsigned long long warp_mass[kWarps];
   // histogram; masses in halves of 16 bits (a part has at most 65,536 entries), or whole where it has more
-  uint32_t bin_count[kBins], bin_lo[kBins], bin_hi[kBins];
+  uint32_t bin_count[kBins], bin_lo[kBins], bin_hi[kBins], bin_low[kBins], bin_high[kBins];
   unsigned long long depth_mass[kWarps][4], cta_depth_mass[4];  // within some depths of the maximum, and in all
   // results of a step, written by one thread; cut: by CTA 0 for the cluster
   uint32_t found, found_n;
-  unsigned long long found_m, found_bin_m;
+  unsigned long long found_m;
   uint32_t cut_key, cut_ties;
   unsigned long long cut_mass;
 };
@@ -229,25 +229,31 @@ __device__ __forceinline__ void scan_pair(Shared& sh, uint32_t n, unsigned long 
   __syncthreads();
 }
 
-// Sorts n entries (at most kList) from `from` to `to` (which may be the same), rising: `bin` is a rising
-// function of the key with values below kBins; entries find their bin's place, then their rank in the
-// bin by comparing.
+// Sorts n entries (at most kList) in place, rising: `bin` is a rising function of an entry with
+// values below kBins. Entries find their bin's place, then their rank in the bin by comparing; with
+// `by_high`, entries of equal high words may stay in any order, and a bin of one high word is left alone.
 template <typename F>
-__device__ __forceinline__ void sort_entries(Shared& sh, const unsigned long long* from, unsigned long long* to, int n, F bin) {
+__device__ __forceinline__ void sort_entries(Shared& sh, unsigned long long* list, int n, bool by_high, F bin) {
   constexpr int kPer = kList / kThreads;
   const int tid = threadIdx.x;
   unsigned long long e[kPer];
   int b[kPer];
   sh.bin_count[tid] = 0;
+  sh.bin_low[tid] = 0xffffffffu;
+  sh.bin_high[tid] = 0;
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
     const int i = tid + j * kThreads;
     b[j] = -1;
     if (i < n) {
-      e[j] = from[i];
-      b[j] = bin(uint32_t(e[j] >> 32));
+      e[j] = list[i];
+      b[j] = bin(e[j]);
       atomicAdd(&sh.bin_count[b[j]], 1u);
+      if (by_high) {
+        atomicMin(&sh.bin_low[b[j]], uint32_t(e[j] >> 32));
+        atomicMax(&sh.bin_high[b[j]], uint32_t(e[j] >> 32));
+      }
     }
   }
   __syncthreads();
@@ -258,23 +264,28 @@ __device__ __forceinline__ void sort_entries(Shared& sh, const unsigned long lon
   sh.bin_lo[tid] = cum - c;  // the bin's first place
   sh.bin_hi[tid] = 0;        // of it taken
   __syncthreads();
-#pragma unroll
-  for (int j = 0; j < kPer; ++j)
-    if (b[j] >= 0) to[sh.bin_lo[b[j]] + atomicAdd(&sh.bin_hi[b[j]], 1u)] = e[j];
-  __syncthreads();
+  uint32_t place[kPer];
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
     if (b[j] >= 0) {
-      const uint32_t start = sh.bin_lo[b[j]], count = sh.bin_count[b[j]];
-      uint32_t rank = 0;
-      for (uint32_t x = 0; x < count; ++x) rank += to[start + x] < e[j] ? 1u : 0u;
-      b[j] = int(start + rank);
+      place[j] = sh.bin_lo[b[j]] + atomicAdd(&sh.bin_hi[b[j]], 1u);
+      list[place[j]] = e[j];
     }
   }
   __syncthreads();
 #pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    if (b[j] < 0) continue;
+    const uint32_t start = sh.bin_lo[b[j]], count = sh.bin_count[b[j]];
+    if (by_high && sh.bin_low[b[j]] == sh.bin_high[b[j]]) continue;
+    uint32_t rank = 0;  // entries are unlike
+    for (uint32_t x = start; x < start + count; ++x) rank += list[x] < e[j] ? 1u : 0u;
+    place[j] = start + rank;
+  }
+  __syncthreads();
+#pragma unroll
   for (int j = 0; j < kPer; ++j)
-    if (b[j] >= 0) to[b[j]] = e[j];
+    if (b[j] >= 0) list[place[j]] = e[j];
   __syncthreads();
 }
 
@@ -397,11 +408,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
   // warp w owns slots [w0, w1), VEC consecutive ones a lane and step, so warps hold rising indices
   const int per = ((n_slots + kWarps - 1) / kWarps + kStep - 1) / kStep * kStep;
   const int w0 = min(warp * per, n_slots), w1 = min(w0 + per, n_slots);
-  auto load = [&](int s, float* f) {  // slots s .. s + VEC - 1 (whole granules); past the warp's: -inf
+  // Slots s .. s + VEC - 1 (whole granules); past the warp's: -inf. A NaN stays one: it lies in no bin and no key
+  // range, and its weight is 0 (a conversion to a whole number takes NaN to 0).
+  auto load = [&](int s, float* f) {
     if (s < w1) {
       granule(s / VEC, f);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) f[j] = no_nan(f[j]);
     } else {
 #pragma unroll
       for (int j = 0; j < VEC; ++j) f[j] = kNegInf;
@@ -454,50 +465,27 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
     else cluster.sync();  // everyone has read the bins
   }
 
-  // Entries with x in [low, high) (all up to the maximum where `open`), into CTA 0's list in index order.
-  // Returns how many there are in the cluster; only where they fit (kList) is the list filled, and only in CTA 0.
+  // Entries with x in [low, high) (all up to the maximum where `open`), into CTA 0's list in any order.
+  // Returns how many there are in the cluster, or some number above kList; only where they fit (kList) is the
+  // list filled, and only in CTA 0.
   auto collect = [&](float low, float high, bool open) -> uint32_t {
-    uint32_t mine = 0;
-    auto in = [&](float x) { return x >= low && (open || x < high); };  // never a NaN
-    if (open) {
-      for (int g = w0 / VEC + lane; g < w1 / VEC; g += 32) {
-        float f[VEC];
-        granule(g, f);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) mine += f[j] >= low ? 1u : 0u;
-      }
-    } else {
-      for (int g = w0 / VEC + lane; g < w1 / VEC; g += 32) {
-        float f[VEC];
-        granule(g, f);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) mine += f[j] >= low && f[j] < high ? 1u : 0u;
-      }
-    }
-    mine = __reduce_add_sync(0xffffffffu, mine);
-    if (lane == 0) sh.warp_count[warp] = mine;
+    if (tid == 0) sh.count = 0;
     __syncthreads();
-    uint32_t before = lane < kWarps ? sh.warp_count[lane] : 0;
-    const uint32_t upto = warp_scan(before, lane);
-    const uint32_t here_all = __shfl_sync(0xffffffffu, upto, kWarps - 1);
-    before = __shfl_sync(0xffffffffu, upto, warp) - mine;
-    if (tid == 0) sh.count = here_all;
-    if (mine != 0 && here_all <= uint32_t(kList)) {
-      for (int s0 = w0; s0 < w1; s0 += kStep) {
-        float f[VEC];
-        load(s0 + lane * VEC, f);
-        uint32_t bits = 0;
+    for (int g = tid; g < n_g; g += kThreads) {
+      float f[VEC];
+      granule(g, f);
+      uint32_t bits = 0;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) bits |= in(f[j]) ? 1u << j : 0u;
-        if (__ballot_sync(0xffffffffu, bits != 0) == 0) continue;
-        const uint32_t incl = warp_scan(uint32_t(__popc(bits)), lane);
-        uint32_t at = before + incl - __popc(bits);
+      for (int j = 0; j < VEC; ++j) bits |= f[j] >= low && (open || f[j] < high) ? 1u << j : 0u;  // never a NaN
+      if (bits == 0) continue;
+      if (*reinterpret_cast<volatile uint32_t*>(&sh.count) > uint32_t(kList)) break;  // too many: how many does not matter
+      uint32_t at = atomicAdd(&sh.count, uint32_t(__popc(bits)));
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          if (bits >> j & 1u)
-            list[at++] = (uint64_t(key_of(sc.z(f[j]))) << 32) | uint32_t(first + s0 + lane * VEC + j);
+      for (int j = 0; j < VEC; ++j) {
+        if (bits >> j & 1u) {
+          if (at < uint32_t(kList)) list[at] = (uint64_t(key_of(sc.z(f[j]))) << 32) | uint32_t(first + g * VEC + j);
+          ++at;
         }
-        before += __shfl_sync(0xffffffffu, incl, 31);
       }
     }
     cluster.sync();
@@ -505,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
     const uint32_t ends = warp_scan(theirs, lane);  // of the CTAs' entries, in the list
     const uint32_t n_all = __shfl_sync(0xffffffffu, ends, kMaxCluster - 1);
     if (n_all <= uint32_t(kList) && rank == 0) {
-      for (uint32_t i0 = here_all; i0 < n_all; i0 += kThreads) {
+      for (uint32_t i0 = __shfl_sync(0xffffffffu, theirs, 0); i0 < n_all; i0 += kThreads) {
         const uint32_t i = i0 + tid;
         int c = 0;
         uint32_t start = 0;
@@ -527,9 +515,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
   auto x_first = [&](auto pred) -> float {
     return from_ordered(first_true(ordered(kNegInf), ordered(sc.m), [&](uint32_t o) { return pred(key_of(sc.z(from_ordered(o)))); }));
   };
-  // CTA 0: draws from the list, which holds all that can be drawn, and writes the row's result.
-  auto draw_from_list = [&](int n) {
-    sort_entries(sh, list, sorted, n, [](uint32_t key) { return min(int(__uint_as_float(key) * kBinScale), kBins - 1); });
+  // CTA 0: draws from the list, which holds all that can be drawn (keys below `end`), and writes the row's result.
+  auto draw_from_list = [&](int n, uint32_t end) {
+    const float scale = kBins / __uint_as_float(end);
+    sort_entries(sh, list, n, false,
+                 [&](unsigned long long e) { return min(int(__uint_as_float(uint32_t(e >> 32)) * scale), kBins - 1); });
     // falling z: the weights' running sums, kPer neighbours a thread
     unsigned long long w[kPer], sum = 0, run, none;
     uint32_t zero;
@@ -538,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       const int i = tid * kPer + j;
-      e[j] = i < n_k ? expf(z_of(uint32_t(sorted[i] >> 32))) : 0.f;
+      e[j] = i < n_k ? expf(z_of(uint32_t(list[i] >> 32))) : 0.f;
       w[j] = weight(e[j]);
       sum += w[j];
     }
@@ -557,13 +547,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
     scan_pair(sh, kept, 0ull, kept, none);
     if (tid == kThreads - 1) sh.found = kept;
     __syncthreads();
-    const unsigned long long cut = sorted[sh.found - 1];  // the entry with z = 0 always stays
-    // rising index: the kept weights' running sum, and the first to pass the target
+    const int n_kept = int(sh.found);  // the first of the list: at least the entry with z = 0
+    // by rising index: the kept weights' running sum, and the first to pass the target
+    for (int i = tid; i < n_kept; i += kThreads) list[i] = (list[i] << 32) | (list[i] >> 32);
+    __syncthreads();
+    const float per_bin = float(kBins) / float(a.vocab);
+    sort_entries(sh, list, n_kept, false,
+                 [&](unsigned long long e) { return min(int(float(uint32_t(e >> 32)) * per_bin), kBins - 1); });
     sum = 0;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       const int i = tid * kPer + j;
-      w[j] = i < n && list[i] <= cut ? weight(expf(z_of(uint32_t(list[i] >> 32)))) : 0;
+      w[j] = i < n_kept ? weight(expf(z_of(uint32_t(list[i])))) : 0;
       sum += w[j];
     }
     scan_pair(sh, 0u, sum, zero, run);
@@ -576,8 +571,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
       for (int j = 0; j < kPer; ++j) {
         if (run <= target && target < run + w[j]) {
           const unsigned long long it = list[tid * kPer + j];
-          a.tokens[row] = int64_t(uint32_t(it));
-          if (a.logprobs) a.logprobs[row] = z_of(uint32_t(it >> 32)) - logf(float(double(whole) / double(kUnit)));
+          a.tokens[row] = int64_t(it >> 32);
+          if (a.logprobs) a.logprobs[row] = z_of(uint32_t(it)) - logf(float(double(whole) / double(kUnit)));
         }
         run += w[j];
       }
@@ -587,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
     const float end = float(bin + 1);
     const uint32_t n = collect(x_first([&](uint32_t key) { return __uint_as_float(key) * kBinScale < end; }), 0.f, true);
     if (n > uint32_t(kList)) return false;
-    if (rank == 0) draw_from_list(int(n));  // from CTA 0's memory alone
+    if (rank == 0) draw_from_list(int(n), bin_edge(bin + 1));  // from CTA 0's memory alone
     return true;
   };
   if (last_bin >= 0 && list_up_to(last_bin)) return;
@@ -595,26 +590,32 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
   uint32_t cut_key = kDead, cut_ties = 0xffffffffu;  // entries below the key stay, and of those at it the first ties
   if (use_k || use_p) {
     // One histogram over the cluster: this thread's bin, and the running sums up to and with it.
-    auto histogram = [&](auto bin, uint32_t& n, unsigned long long& m, uint32_t& cum_n, unsigned long long& cum_m) {
+    // Counts are kept where something is looked for by count, masses where something is by mass.
+    auto histogram = [&](bool counts, auto bin, uint32_t& n, unsigned long long& m, uint32_t& cum_n, unsigned long long& cum_m) {
       sh.bin_count[tid] = sh.bin_lo[tid] = sh.bin_hi[tid] = 0;
       __syncthreads();
       for (int s = w0 + lane * VEC; s < w1; s += kStep) {
         float f[VEC];
         load(s, f);
+        int b[VEC];
+        uint32_t w[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {  // without branches: the chains of the entries run beside one another
+          const float z = sc.z(f[j]);
+          b[j] = bin(f[j], z);
+          w[j] = use_p ? weight(expf(z)) : 0u;
+        }
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          const float z = sc.z(f[j]);
-          const int b = bin(f[j], z);
-          if (b < 0) continue;
-          atomicAdd(&sh.bin_count[b], 1u);
+          if (b[j] < 0) continue;
+          if (counts) atomicAdd(&sh.bin_count[b[j]], 1u);
           if (!use_p) continue;
-          const uint32_t w = weight(expf(z));
           if constexpr (kResident) {
-            atomicAdd(&sh.bin_lo[b], w & 0xffffu);
-            atomicAdd(&sh.bin_hi[b], w >> 16);
+            atomicAdd(&sh.bin_lo[b[j]], w[j] & 0xffffu);
+            if (w[j] >> 16) atomicAdd(&sh.bin_hi[b[j]], w[j] >> 16);
           } else {  // parts may be longer: carry by hand
-            const uint32_t old = atomicAdd(&sh.bin_lo[b], w);
-            if (old + w < old) atomicAdd(&sh.bin_hi[b], 1u);
+            const uint32_t old = atomicAdd(&sh.bin_lo[b[j]], w[j]);
+            if (old + w[j] < old) atomicAdd(&sh.bin_hi[b[j]], 1u);
           }
         }
       }
@@ -628,53 +629,52 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
     };
     // The bin whose running sum is the first to reach the goal; what lies before it, and in it.
     auto find = [&](bool by_count, unsigned long long goal, uint32_t n, unsigned long long m, uint32_t cum_n,
-                    unsigned long long cum_m, unsigned long long& below_n, unsigned long long& below_m, uint32_t& in_n) -> int {
+                    unsigned long long cum_m, unsigned long long& below_n, unsigned long long& below_m) -> int {
       const unsigned long long c0 = by_count ? below_n + cum_n - n : below_m + cum_m - m;
       const unsigned long long c1 = by_count ? below_n + cum_n : below_m + cum_m;
       __syncthreads();
       if (c0 < goal && goal <= c1) {
         sh.found = uint32_t(tid);
-        sh.found_n = n;
-        sh.found_m = below_n + cum_n - n;
-        sh.found_bin_m = below_m + cum_m - m;
+        sh.found_n = uint32_t(below_n + cum_n - n);
+        sh.found_m = below_m + cum_m - m;
       }
       __syncthreads();
-      in_n = sh.found_n;
-      below_n = sh.found_m;
-      below_m = sh.found_bin_m;
+      below_n = sh.found_n;
+      below_m = sh.found_m;
       return int(sh.found);
     };
-    // The exact cut within keys [lo, hi), which hold in_n entries behind below_n entries of mass below_m;
-    // leaves cut_key and cut_ties and returns the mass up to the cut.
+    // The exact cut within keys [lo, hi), behind below_n entries of mass below_m; leaves cut_key and
+    // cut_ties and returns the mass up to the cut.
     auto refine = [&](bool by_count, unsigned long long goal, uint32_t lo, uint32_t hi, unsigned long long below_n,
-                      unsigned long long below_m, uint32_t in_n) -> unsigned long long {
-      while (in_n > uint32_t(kList) && hi - lo > 1) {
+                      unsigned long long below_m) -> unsigned long long {
+      uint32_t in_n;
+      for (;;) {
+        in_n = collect(x_first([&](uint32_t key) { return key < hi; }),
+                       lo == 0 ? 0.f : x_first([&](uint32_t key) { return key < lo; }), lo == 0);
+        if (in_n <= uint32_t(kList) || hi - lo == 1) break;
         int shift = 0;
         while ((hi - lo - 1) >> shift >= uint32_t(kBins)) ++shift;
         uint32_t n, cum_n;
         unsigned long long m, cum_m;
-        histogram([&](float, float z) {
+        histogram(by_count, [&](float, float z) {
           const uint32_t key = key_of(z);
           return key >= lo && key < hi ? int((key - lo) >> shift) : -1;
         }, n, m, cum_n, cum_m);
-        const int b = find(by_count, goal, n, m, cum_n, cum_m, below_n, below_m, in_n);
+        const int b = find(by_count, goal, n, m, cum_n, cum_m, below_n, below_m);
         lo += uint32_t(b) << shift;
         hi = min(hi, lo + (1u << shift));
       }
       if (in_n > uint32_t(kList)) {  // one key
         const unsigned long long w = weight(expf(z_of(lo)));
-        unsigned long long ties = by_count ? goal - below_n : w != 0 ? (goal - below_m + w - 1) / w : 1;
-        ties = min(ties, (unsigned long long)in_n);
+        const unsigned long long ties = by_count ? goal - below_n : w != 0 ? (goal - below_m + w - 1) / w : 1;
         cut_key = lo;
         cut_ties = uint32_t(ties);
         return below_m + w * ties;
       }
-      collect(x_first([&](uint32_t key) { return key < hi; }), lo == 0 ? 0.f : x_first([&](uint32_t key) { return key < lo; }),
-              lo == 0);
-      if (rank == 0) {  // sorted in place: the part is still needed
+      if (rank == 0) {
         int shift = 0;
         while ((hi - lo - 1) >> shift >= uint32_t(kBins)) ++shift;
-        sort_entries(sh, list, list, int(in_n), [&](uint32_t key) { return int((key - lo) >> shift); });
+        sort_entries(sh, list, int(in_n), true, [&](unsigned long long e) { return int((uint32_t(e >> 32) - lo) >> shift); });
         unsigned long long w[kPer], sum = 0, run;
         uint32_t zero;
 #pragma unroll
@@ -692,7 +692,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
           run += w[j];
           if (here && i < int(in_n)) {
             const uint32_t key = uint32_t(list[i] >> 32);
-            int f = i;  // ties: how many entries of this key lie up to here
+            int f = i;  // ties: how many entries of this key lie up to here (the walk takes them by index)
             while (f > 0 && uint32_t(list[f - 1] >> 32) == key) --f;
             sh.cut_key = key;
             sh.cut_ties = uint32_t(i - f + 1);
@@ -709,7 +709,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
       return mass;
     };
 
-    uint32_t n, cum_n, in_n;
+    uint32_t n, cum_n;
     unsigned long long m, cum_m;
     float reach = kNegInf;  // the histogram takes entries from here on
     if (!use_k) {
@@ -723,7 +723,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
         granule(g, f);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          const float z = sc.z(no_nan(f[j]));
+          const float z = sc.z(f[j]);
           const uint32_t w = weight(expf(z));
           sum[kDepths] += w;
 #pragma unroll
@@ -753,7 +753,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
         if (sum[d] >= need) reach = -depth[d];
       if (reach > kNegInf) reach = x_first([&](uint32_t key) { return __uint_as_float(key) <= -reach; });
     }
-    histogram([&](float x, float z) {
+    histogram(use_k, [&](float x, float z) {
       const float b = bin_of(z);
       return x >= reach && b < float(kBins) ? int(b) : -1;
     }, n, m, cum_n, cum_m);
@@ -767,15 +767,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
     if (use_k || use_p) {
       unsigned long long below_n = 0, below_m = 0;
       const unsigned long long goal = use_k ? (unsigned long long)k : mass_needed(top_p, total);
-      const int b = find(use_k, goal, n, m, cum_n, cum_m, below_n, below_m, in_n);
-      if (below_n + in_n <= (unsigned long long)kList && list_up_to(b)) return;
-      const unsigned long long mass = refine(use_k, goal, bin_edge(b), bin_edge(b + 1), below_n, below_m, in_n);
+      const int b = find(use_k, goal, n, m, cum_n, cum_m, below_n, below_m);
+      if (below_n < (unsigned long long)kList && list_up_to(b)) return;
+      const unsigned long long mass = refine(use_k, goal, bin_edge(b), bin_edge(b + 1), below_n, below_m);
       if (use_k && use_p) {
         const uint32_t k_key = cut_key, k_ties = cut_ties;
         const unsigned long long need = mass_needed(top_p, mass);
         below_n = below_m = 0;
-        const int b2 = find(false, need, n, m, cum_n, cum_m, below_n, below_m, in_n);
-        refine(false, need, bin_edge(b2), bin_edge(b2 + 1), below_n, below_m, in_n);
+        const int b2 = find(false, need, n, m, cum_n, cum_m, below_n, below_m);
+        refine(false, need, bin_edge(b2), bin_edge(b2 + 1), below_n, below_m);
         // the nucleus lies within the top k: where both end at one key, the smaller part stays
         if (cut_key == k_key) cut_ties = min(cut_ties, k_ties);
       }
