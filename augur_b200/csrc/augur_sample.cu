@@ -54,6 +54,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kList = 2048;  // most entries CTA 0 sorts
 constexpr int kBins = kThreads;  // bins of a histogram, one a thread
 constexpr float kBinScale = kBins / 21.6f;  // linear bins of |z|: e^-21.6 has no weight any more
+constexpr int kDepths = 5;  // of the maximum at which top-p first looks
 constexpr int kMaxCluster = 8;
 constexpr float kNegInf = -INFINITY;
 constexpr float kUnit = 2147483648.f;  // 2^31
@@ -84,7 +85,7 @@ struct Shared {
   unsigned long long warp_mass[kWarps];
   // histogram; masses in halves of 16 bits (a part has at most 65,536 entries), or whole where it has more
   uint32_t bin_count[kBins], bin_lo[kBins], bin_hi[kBins], bin_low[kBins], bin_high[kBins];
-  unsigned long long depth_mass[kWarps][4], cta_depth_mass[4];  // within some depths of the maximum, and in all
+  unsigned long long depth_mass[kWarps][kDepths + 1], cta_depth_mass[kDepths + 1];  // within depths of the maximum, and in all
   // results of a step, written by one thread; cut: by CTA 0 for the cluster
   uint32_t found, found_n;
   unsigned long long found_m;
@@ -298,9 +299,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
   __shared__ Shared sh;
   // entries in question, (key, index), in index order; CTA 0's hold the cluster's
   unsigned long long* list = reinterpret_cast<unsigned long long*>(dyn);
-  // this CTA's part of the row, as stored; CTA 0's sorted copy of the list lies over it once it is no longer read
-  unsigned char* part = dyn + kList * 8;
-  unsigned long long* sorted = reinterpret_cast<unsigned long long*>(part);
+  unsigned char* part = dyn + kList * 8;  // this CTA's part of the row, as stored
 
   cg::cluster_group cluster = cg::this_cluster();
   const int C = int(cluster.num_blocks()), rank = int(cluster.block_rank());
@@ -357,6 +356,37 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
     else u = g >= in0 && g < in1 ? __ldg(reinterpret_cast<const uint4*>(part_base + int64_t(g) * 16)) : edge_granule(g);
     Logit<T>::unpack(u, f);
   };
+  // All granules of the part, a thread every kThreads-th (the ones it copied itself); several loads under way
+  auto each_granule = [&](auto use) {
+    constexpr int kBatch = kResident ? 2 : 8;
+    int g = tid;
+    if constexpr (!kResident) {
+      for (; g < in0; g += kThreads) {  // the first granule may lie in the row in part
+        float f[VEC];
+        granule(g, f);
+        use(g, f);
+      }
+    }
+    const int whole = kResident ? n_g : in1;
+    for (; g + (kBatch - 1) * kThreads < whole; g += kBatch * kThreads) {
+      uint4 u[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        u[i] = kResident ? *reinterpret_cast<const uint4*>(part + (g + i * kThreads) * 16)
+                         : __ldg(reinterpret_cast<const uint4*>(part_base + int64_t(g + i * kThreads) * 16));
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        float f[VEC];
+        Logit<T>::unpack(u[i], f);
+        use(g + i * kThreads, f);
+      }
+    }
+    for (; g < n_g; g += kThreads) {
+      float f[VEC];
+      granule(g, f);
+      use(g, f);
+    }
+  };
   const float temperature = a.temperature ? __ldg(a.temperature + row) : a.temperature_s;
   int k = a.top_k ? __ldg(a.top_k + row) : a.top_k_s;
   const float top_p = a.top_p ? __ldg(a.top_p + row) : a.top_p_s;
@@ -365,13 +395,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
   const float u = __ldg(a.uniform + row);
 
   float tmax = kNegInf;  // fmaxf passes NaN over
-#pragma unroll 4
-  for (int g = tid; g < n_g; g += kThreads) {  // the granules this thread copied itself
-    float f[VEC];
-    granule(g, f);
+  each_granule([&](int, const float* f) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) tmax = fmaxf(tmax, f[j]);
-  }
+  });
   {
     float m = tmax;
 #pragma unroll
@@ -471,14 +498,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
   auto collect = [&](float low, float high, bool open) -> uint32_t {
     if (tid == 0) sh.count = 0;
     __syncthreads();
-    for (int g = tid; g < n_g; g += kThreads) {
-      float f[VEC];
-      granule(g, f);
+    each_granule([&](int g, const float* f) {
       uint32_t bits = 0;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) bits |= f[j] >= low && (open || f[j] < high) ? 1u << j : 0u;  // never a NaN
-      if (bits == 0) continue;
-      if (*reinterpret_cast<volatile uint32_t*>(&sh.count) > uint32_t(kList)) break;  // too many: how many does not matter
+      // too many: how many does not matter
+      if (bits == 0 || *reinterpret_cast<volatile uint32_t*>(&sh.count) > uint32_t(kList)) return;
       uint32_t at = atomicAdd(&sh.count, uint32_t(__popc(bits)));
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
@@ -487,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
           ++at;
         }
       }
-    }
+    });
     cluster.sync();
     const uint32_t theirs = of_lane([](const Shared& o) { return o.count; }, 0u);
     const uint32_t ends = warp_scan(theirs, lane);  // of the CTAs' entries, in the list
@@ -594,9 +619,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
     auto histogram = [&](bool counts, auto bin, uint32_t& n, unsigned long long& m, uint32_t& cum_n, unsigned long long& cum_m) {
       sh.bin_count[tid] = sh.bin_lo[tid] = sh.bin_hi[tid] = 0;
       __syncthreads();
-      for (int s = w0 + lane * VEC; s < w1; s += kStep) {
-        float f[VEC];
-        load(s, f);
+      each_granule([&](int, const float* f) {
         int b[VEC];
         uint32_t w[VEC];
 #pragma unroll
@@ -618,7 +641,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
             if (old + w[j] < old) atomicAdd(&sh.bin_hi[b[j]], 1u);
           }
         }
-      }
+      });
       cluster.sync();
       n = cluster_sum([&](const Shared& o) { return o.bin_count[tid]; });
       m = cluster_sum([&](const Shared& o) {
@@ -711,16 +734,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
 
     uint32_t n, cum_n;
     unsigned long long m, cum_m;
-    float reach = kNegInf;  // the histogram takes entries from here on
+    float from = kNegInf, to = INFINITY;  // the histogram takes entries in [from, to)
+    unsigned long long above_m = 0;       // mass of those from `to` on
     if (!use_k) {
-      // top-p alone: the row's mass, and a depth that holds the nucleus, so that the histogram's atomics are
-      // spent on few entries
-      constexpr int kDepths = 3;
-      const float depth[kDepths] = {4.f, 8.f, 13.f};
-      unsigned long long sum[kDepths + 1] = {0, 0, 0, 0};
-      for (int g = w0 / VEC + lane; g < w1 / VEC; g += 32) {
-        float f[VEC];
-        granule(g, f);
+      // top-p alone: the row's mass, and between which depths the nucleus ends, so that the histogram's atomics
+      // are spent on few entries
+      const float depth[kDepths] = {3.f, 6.f, 9.f, 12.f, 15.f};
+      unsigned long long sum[kDepths + 1] = {0, 0, 0, 0, 0, 0};
+      each_granule([&](int, const float* f) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           const float z = sc.z(f[j]);
@@ -729,7 +750,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
 #pragma unroll
           for (int d = 0; d < kDepths; ++d) sum[d] += z >= -depth[d] ? w : 0u;
         }
-      }
+      });
 #pragma unroll
       for (int d = 0; d <= kDepths; ++d) sum[d] = warp_sum(sum[d]);
       __syncthreads();
@@ -748,14 +769,22 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
       for (int d = 0; d <= kDepths; ++d) sum[d] = warp_sum(of_lane([&](const Shared& o) { return o.cta_depth_mass[d]; }, 0ull));
       total = sum[kDepths];
       const unsigned long long need = mass_needed(top_p, total);
+      float end = 0.f, start = 0.f;  // depths
 #pragma unroll
-      for (int d = kDepths - 1; d >= 0; --d)
-        if (sum[d] >= need) reach = -depth[d];
-      if (reach > kNegInf) reach = x_first([&](uint32_t key) { return __uint_as_float(key) <= -reach; });
+      for (int d = kDepths - 1; d >= 0; --d) {
+        if (sum[d] >= need) end = depth[d];
+        else if (start == 0.f) {
+          start = depth[d];
+          above_m = sum[d];
+        }
+      }
+      // |z| in (start, end]: falling x
+      if (end > 0.f) from = x_first([&](uint32_t key) { return __uint_as_float(key) <= end; });
+      if (start > 0.f) to = x_first([&](uint32_t key) { return __uint_as_float(key) <= start; });
     }
     histogram(use_k, [&](float x, float z) {
       const float b = bin_of(z);
-      return x >= reach && b < float(kBins) ? int(b) : -1;
+      return x >= from && (x < to || to == INFINITY) && b < float(kBins) ? int(b) : -1;
     }, n, m, cum_n, cum_m);
     if (tid == kThreads - 1) {
       sh.found_n = cum_n;
@@ -765,10 +794,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
     if (use_k) total = sh.found_m;
     use_k = use_k && sh.found_n > uint32_t(k);  // entries past the bins have no weight
     if (use_k || use_p) {
-      unsigned long long below_n = 0, below_m = 0;
+      unsigned long long below_n = 0, below_m = above_m;
       const unsigned long long goal = use_k ? (unsigned long long)k : mass_needed(top_p, total);
       const int b = find(use_k, goal, n, m, cum_n, cum_m, below_n, below_m);
-      if (below_n < (unsigned long long)kList && list_up_to(b)) return;
+      // with counts it is known whether the list will hold them; without, a nucleus that ends this side of e^-6 is tried
+      if ((use_k ? below_n < (unsigned long long)kList : b < int(9.f * kBinScale)) && list_up_to(b)) return;
       const unsigned long long mass = refine(use_k, goal, bin_edge(b), bin_edge(b + 1), below_n, below_m);
       if (use_k && use_p) {
         const uint32_t k_key = cut_key, k_ties = cut_ties;
@@ -981,22 +1011,22 @@ AUGUR_KV_EXPORT int augur_kv_sample(const void* logits, int64_t row_stride, int3
   a.min_p_s = min_p_all;
   a.tokens = tokens;
   a.logprobs = logprobs;
-  // CTAs per row: as many as keep the GPU's resident CTAs (two an SM) busy, at
-  // least enough for two parts to fit an SM's shared memory, and parts of at
-  // least 2,048 entries
+  // CTAs per row: as many as the GPU holds at once (two an SM), at least 4 (a row whose nucleus is wide takes
+  // long, and with fewer CTAs a batch waits for it: 256 rows of 151,936 float32 logits with mixed settings take 205 us
+  // with 2, 167 with 4, 183 with 8), with parts of at least 2,048 entries. Parts stay in shared memory where two
+  // CTAs' fit an SM's; else every pass reads them again, from L2 for the most part.
   const int vec = 16 / es;
-  constexpr size_t kMost = 200 * 1024;  // of the 227 KB a CTA may have
-  auto bytes = [&](int c) {  // the list, and the part or (CTA 0, if larger) the sorted list over it
+  constexpr size_t kMost = 100 * 1024;  // of the 227 KB an SM's CTAs may have
+  auto bytes = [&](int c) {  // the list and the part
     const int64_t granules = ((int64_t(vocab) + vec - 1) / vec + 1 + c - 1) / c;
-    const size_t part = size_t(granules) * 16;
-    return size_t(kList) * 8 + (part > size_t(kList) * 8 ? part : size_t(kList) * 8);
+    return size_t(kList) * 8 + size_t(granules) * 16;
   };
   const int64_t slots = int64_t(augur_kv_dev::sm_count()) * 2;
   int c = 1;
-  while (c < kMaxCluster && (bytes(c) > kMost / 2 || (int64_t(rows) * c * 2 <= slots * 2 && vocab / (c * 2) >= 2048))) c *= 2;
+  while (c < kMaxCluster && vocab / (c * 2) >= 2048 && (c < 4 || int64_t(rows) * c * 2 <= slots)) c *= 2;
   // masses are added in halves of 16 bits: a part has at most 65,536 entries
   const bool resident = bytes(c) <= kMost && (vocab + 2 * vec) / c + vec <= 65536;
-  const size_t smem = resident ? bytes(c) : size_t(kList) * 16;
+  const size_t smem = resident ? bytes(c) : size_t(kList) * 8;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == AUGUR_KV_F32)
     return resident ? launch<float, true>(a, rows, c, smem, st) : launch<float, false>(a, rows, c, smem, st);
