@@ -14,9 +14,10 @@
 // Bound by HBM: every row is read and written once, 2 (heads + 2 kv heads)
 // head_dim elements a token. A CTA takes a few tokens: it computes their
 // head_dim / 2 angles once for all heads (sin and cos in shared memory: no
-// table of positions, so none to grow or to read), with its first pieces of q,
-// k and v already on their way, and then turns pieces of 16 bytes of a row's
-// first half together with the matching 16 bytes of the second.
+// table of positions, so none to grow or to read) and where their slots lie,
+// with its first pieces of q, k and v already on their way, and then turns
+// pieces of 16 bytes of a row's first half together with the matching 16 bytes of
+// the second, kBatch pieces of a thread under way at a time.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -51,99 +52,137 @@ struct AxesArgs {
   int32_t n_axes, hq, hkv, half;
   int32_t pieces;        // of a row's half
   int32_t token_pieces;  // (hq + 2 hkv) * pieces
+  uint32_t piece_mul, token_mul;  // 2^32 / pieces and 2^32 / token_pieces, rounded up
   int32_t tokens_per_cta;
   int64_t n_tokens;
   int32_t* status;
 };
 
 constexpr int kThreads = 256;
+constexpr int kBatch = 3;  // pieces of a thread under way (32 bytes each)
+constexpr int kCtas = 4;   // resident per SM
 
-template <typename T, int VEC>
-struct alignas(VEC * sizeof(T)) Vec {
-  T v[VEC];
+// A piece: 16 bytes (four words of one float, or of two 16-bit values), or one element.
+template <typename T, int VEC> struct Piece;
+template <typename T> __device__ __forceinline__ float2 two(uint32_t w);
+template <> __device__ __forceinline__ float2 two<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
+template <> __device__ __forceinline__ float2 two<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <typename T> __device__ __forceinline__ uint32_t word(float x, float y);
+template <> __device__ __forceinline__ uint32_t word<__half>(float x, float y) {
+  const __half2 v = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <> __device__ __forceinline__ uint32_t word<__nv_bfloat16>(float x, float y) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// One product rounded, then a fused multiply-add, spelled out so that every piece width gives the same bits.
+__device__ __forceinline__ void turn_pair(float& p, float& q, float c, float s) {
+  const float x = __fmaf_rn(p, c, -__fmul_rn(q, s));
+  q = __fmaf_rn(q, c, __fmul_rn(p, s));
+  p = x;
+}
+template <typename T> struct Piece<T, 8> {  // two 16-bit values a word
+  uint4 v;
+  static __device__ __forceinline__ void turned(Piece& x, Piece& y, const float2* cs) {
+    uint32_t* a = &x.v.x;
+    uint32_t* b = &y.v.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 f = *reinterpret_cast<const float4*>(cs + 2 * i);  // cos, sin of two frequencies
+      float2 p = two<T>(a[i]), q = two<T>(b[i]);
+      turn_pair(p.x, q.x, f.x, f.y);
+      turn_pair(p.y, q.y, f.z, f.w);
+      a[i] = word<T>(p.x, p.y);
+      b[i] = word<T>(q.x, q.y);
+    }
+  }
+};
+template <> struct Piece<float, 4> {
+  float4 v;
+  static __device__ __forceinline__ void turned(Piece& x, Piece& y, const float2* cs) {
+    turn_pair(x.v.x, y.v.x, cs[0].x, cs[0].y);
+    turn_pair(x.v.y, y.v.y, cs[1].x, cs[1].y);
+    turn_pair(x.v.z, y.v.z, cs[2].x, cs[2].y);
+    turn_pair(x.v.w, y.v.w, cs[3].x, cs[3].y);
+  }
 };
 __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <typename T> __device__ __forceinline__ T from_f(float x);
-template <> __device__ __forceinline__ float from_f<float>(float x) { return x; }
-template <> __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+__device__ __forceinline__ void from_f(float& y, float x) { y = x; }
+__device__ __forceinline__ void from_f(__half& y, float x) { y = __float2half_rn(x); }
+__device__ __forceinline__ void from_f(__nv_bfloat16& y, float x) { y = __float2bfloat16_rn(x); }
+template <typename T> struct Piece<T, 1> {
+  T v;
+  static __device__ __forceinline__ void turned(Piece& x, Piece& y, const float2* cs) {
+    float p = to_f(x.v), q = to_f(y.v);
+    turn_pair(p, q, cs->x, cs->y);
+    from_f(x.v, p);
+    from_f(y.v, q);
+  }
+};
 
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads) rope_axes_kernel(AxesArgs a) {
-  extern __shared__ float2 turn[];  // [token of the CTA][frequency]: cos, sin
-  using V = Vec<T, VEC>;
+__global__ void __launch_bounds__(kThreads, kCtas) rope_axes_kernel(AxesArgs a) {
+  extern __shared__ __align__(16) float2 turn[];  // [token of the CTA][frequency]: cos, sin; then each token's place in the pool
+  using V = Piece<T, VEC>;
+  int64_t* place = reinterpret_cast<int64_t*>(turn + a.tokens_per_cta * a.half);
   const int64_t t0 = int64_t(blockIdx.x) * a.tokens_per_cta;
   const int n = int(min(int64_t(a.tokens_per_cta), a.n_tokens - t0));
   const int work = n * a.token_pieces;
   const int64_t half_bytes = int64_t(a.half) * int64_t(sizeof(T));
 
   struct Task {
-    const char* src;
-    char* dst;  // null: nothing to write
-    int t, c;   // the CTA's token; first frequency, or -1 for a v row
+    int t, h, c;  // the CTA's token; head of q, then of k, then of v; piece
   };
   auto task = [&](int p) -> Task {
     Task w;
-    w.t = p / a.token_pieces;
+    w.t = int(__umulhi(uint32_t(p), a.token_mul));
     const int r = p - w.t * a.token_pieces;
-    int h = r / a.pieces;
-    const int c = r - h * a.pieces;
-    const int64_t token = t0 + w.t, off = int64_t(c) * int64_t(sizeof(V));
-    w.c = c * VEC;
-    if (h < a.hq) {
-      w.src = a.q + token * a.q_stride[0] + int64_t(h) * a.q_stride[1] + off;
-      w.dst = a.q_out + token * a.q_out_stride[0] + int64_t(h) * a.q_out_stride[1] + off;
-      return w;
-    }
-    h -= a.hq;
-    const bool is_v = h >= a.hkv;
-    if (is_v) {
-      h -= a.hkv;
-      w.c = -1;
-    }
-    w.src = is_v ? a.v + token * a.v_stride[0] + int64_t(h) * a.v_stride[1] + off
-                 : a.k + token * a.k_stride[0] + int64_t(h) * a.k_stride[1] + off;
-    const int64_t slot = __ldg(a.slots + token * a.slot_stride);
-    w.dst = nullptr;
-    if (slot >= a.num_slots) {
-      record_status(a.status, AUGUR_KV_EBOUNDS);
-    } else if (slot >= 0) {
-      const int64_t block = slot / a.block_size;
-      w.dst = (is_v ? a.v_pool : a.k_pool) + block * a.pool_stride[0] + int64_t(h) * a.pool_stride[1] +
-              (slot - block * a.block_size) * a.pool_stride[2] + off;
-    }
+    w.h = a.pieces == 1 ? r : int(__umulhi(uint32_t(r), a.piece_mul));
+    w.c = r - w.h * a.pieces;
     return w;
   };
   auto load = [&](const Task& w, V& x, V& y) {
-    x = *reinterpret_cast<const V*>(w.src);
-    y = *reinterpret_cast<const V*>(w.src + half_bytes);
+    const int64_t token = t0 + w.t, off = int64_t(w.c) * int64_t(sizeof(V));
+    const char* src = w.h < a.hq ? a.q + token * a.q_stride[0] + int64_t(w.h) * a.q_stride[1]
+                      : w.h < a.hq + a.hkv ? a.k + token * a.k_stride[0] + int64_t(w.h - a.hq) * a.k_stride[1]
+                                           : a.v + token * a.v_stride[0] + int64_t(w.h - a.hq - a.hkv) * a.v_stride[1];
+    x = *reinterpret_cast<const V*>(src + off);
+    y = *reinterpret_cast<const V*>(src + off + half_bytes);
   };
   auto finish = [&](const Task& w, V& x, V& y) {
-    if (w.dst == nullptr) return;
-    if (w.c >= 0) {
-      const float2* cs = turn + w.t * a.half + w.c;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float2 f = cs[j];
-        const float p = to_f(x.v[j]), q = to_f(y.v[j]);
-        x.v[j] = from_f<T>(p * f.x - q * f.y);
-        y.v[j] = from_f<T>(q * f.x + p * f.y);
-      }
+    const int64_t off = int64_t(w.c) * int64_t(sizeof(V));
+    char* dst;
+    if (w.h < a.hq) {
+      dst = a.q_out + (t0 + w.t) * a.q_out_stride[0] + int64_t(w.h) * a.q_out_stride[1];
+    } else {
+      const int64_t at = place[w.t];
+      if (at < 0) return;
+      const int h = w.h - a.hq;
+      dst = h < a.hkv ? a.k_pool + at + int64_t(h) * a.pool_stride[1] : a.v_pool + at + int64_t(h - a.hkv) * a.pool_stride[1];
     }
-    *reinterpret_cast<V*>(w.dst) = x;
-    *reinterpret_cast<V*>(w.dst + half_bytes) = y;
+    if (w.h < a.hq + a.hkv) V::turned(x, y, turn + w.t * a.half + w.c * VEC);
+    *reinterpret_cast<V*>(dst + off) = x;
+    *reinterpret_cast<V*>(dst + off + half_bytes) = y;
   };
 
-  // the first piece is on its way while the angles are computed
-  Task w0;
-  V x0, y0;
-  const bool any = int(threadIdx.x) < work;
-  if (any) {
-    w0 = task(threadIdx.x);
-    load(w0, x0, y0);
-  }
+  // the first pieces are on their way while the angles are computed
+  Task w[kBatch];
+  V x[kBatch], y[kBatch];
+  auto fetch = [&](int p) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (p + i * kThreads < work) {
+        w[i] = task(p + i * kThreads);
+        load(w[i], x[i], y[i]);
+      }
+    }
+  };
+  fetch(threadIdx.x);
   for (int i = threadIdx.x; i < n * a.half; i += kThreads) {
     const int t = i / a.half, j = i - t * a.half;
     const int axis = __ldg(a.axis + j);
@@ -155,20 +194,25 @@ __global__ void __launch_bounds__(kThreads) rope_axes_kernel(AxesArgs a) {
       record_status(a.status, AUGUR_KV_EBOUNDS);
     turn[i] = make_float2(c, s);
   }
-  __syncthreads();
-  if (any) finish(w0, x0, y0);
-  for (int p = threadIdx.x + kThreads; p < work; p += 2 * kThreads) {
-    const bool two = p + kThreads < work;
-    Task w1;
-    V x1, y1;
-    w0 = task(p);
-    load(w0, x0, y0);
-    if (two) {
-      w1 = task(p + kThreads);
-      load(w1, x1, y1);
+  for (int t = threadIdx.x; t < n; t += kThreads) {
+    const int64_t slot = __ldg(a.slots + (t0 + t) * a.slot_stride);
+    int64_t at = -1;
+    if (slot >= a.num_slots) {
+      record_status(a.status, AUGUR_KV_EBOUNDS);
+    } else if (slot >= 0) {
+      const int64_t block = slot / a.block_size;
+      at = block * a.pool_stride[0] + (slot - block * a.block_size) * a.pool_stride[2];
     }
-    finish(w0, x0, y0);
-    if (two) finish(w1, x1, y1);
+    place[t] = at;
+  }
+  __syncthreads();
+  for (int p = threadIdx.x;;) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      if (p + i * kThreads < work) finish(w[i], x[i], y[i]);
+    p += kBatch * kThreads;
+    if (p >= work) break;
+    fetch(p);
   }
 }
 
@@ -176,12 +220,26 @@ template <typename T, int VEC>
 int launch(AxesArgs a, cudaStream_t st) {
   a.pieces = a.half / VEC;
   a.token_pieces = (a.hq + 2 * a.hkv) * a.pieces;
-  // tokens per CTA: as many as leave two resident waves of CTAs, at most 8
-  const int64_t want = a.n_tokens / (int64_t(augur_kv_dev::sm_count()) * 16);
-  a.tokens_per_cta = int32_t(want < 1 ? 1 : want > 8 ? 8 : want);
+  // tokens per CTA: one wave of resident CTAs where that makes at most 16, so that the angles are ready early and
+  // the memory of 16 tokens' angles stays small
+  const int64_t ctas = int64_t(augur_kv_dev::sm_count()) * kCtas;
+  const int64_t want = (a.n_tokens + ctas - 1) / ctas;
+  a.tokens_per_cta = int32_t(want > 16 ? 16 : want);
+  // p / d = p * ceil(2^32 / d) / 2^32 exactly while p * d < 2^32 (p is below tokens_per_cta * token_pieces)
+  if (uint64_t(a.token_pieces) * uint64_t(a.token_pieces) * 16u >= (uint64_t(1) << 32))
+    return augur_kv_dev::fail(AUGUR_KV_EINVAL, "rope_axes_scatter: rows of too many heads");
+  a.token_mul = uint32_t(((uint64_t(1) << 32) + uint32_t(a.token_pieces) - 1) / uint32_t(a.token_pieces));
+  a.piece_mul = uint32_t(((uint64_t(1) << 32) + uint32_t(a.pieces) - 1) / uint32_t(a.pieces));  // (unused for one piece)
   const int64_t grid = (a.n_tokens + a.tokens_per_cta - 1) / a.tokens_per_cta;
   if (grid > 0x7fffffff) return augur_kv_dev::fail(AUGUR_KV_EINVAL, "rope_axes_scatter: too many tokens");
-  rope_axes_kernel<T, VEC><<<unsigned(grid), kThreads, size_t(a.tokens_per_cta) * size_t(a.half) * sizeof(float2), st>>>(a);
+  const size_t smem = size_t(a.tokens_per_cta) * (size_t(a.half) * sizeof(float2) + sizeof(int64_t));
+  if (smem > 48 * 1024) {  // head_dim above 700
+    a.tokens_per_cta = 4;
+    const int64_t g = (a.n_tokens + 3) / 4;
+    rope_axes_kernel<T, VEC><<<unsigned(g), kThreads, 4 * (size_t(a.half) * sizeof(float2) + sizeof(int64_t)), st>>>(a);
+  } else {
+    rope_axes_kernel<T, VEC><<<unsigned(grid), kThreads, smem, st>>>(a);
+  }
   return augur_kv_dev::check_launch("rope_axes_kernel");
 }
 
