@@ -735,7 +735,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
     uint32_t n, cum_n;
     unsigned long long m, cum_m;
     float from = kNegInf, to = INFINITY;  // the histogram takes entries in [from, to)
-    unsigned long long above_m = 0;       // mass of those from `to` on
+    unsigned long long above_m = 0;       // mass of those from `to` on, and the first key past theirs
+    uint32_t above_key = 0;
     if (!use_k) {
       // top-p alone: the row's mass, and between which depths the nucleus ends, so that the histogram's atomics
       // are spent on few entries
@@ -780,7 +781,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
       }
       // |z| in (start, end]: falling x
       if (end > 0.f) from = x_first([&](uint32_t key) { return __uint_as_float(key) <= end; });
-      if (start > 0.f) to = x_first([&](uint32_t key) { return __uint_as_float(key) <= start; });
+      if (start > 0.f) {
+        to = x_first([&](uint32_t key) { return __uint_as_float(key) <= start; });
+        above_key = __float_as_uint(start) + 1;
+      }
     }
     histogram(use_k, [&](float x, float z) {
       const float b = bin_of(z);
@@ -799,7 +803,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
       const int b = find(use_k, goal, n, m, cum_n, cum_m, below_n, below_m);
       // with counts it is known whether the list will hold them; without, a nucleus that ends this side of e^-6 is tried
       if ((use_k ? below_n < (unsigned long long)kList : b < int(9.f * kBinScale)) && list_up_to(b)) return;
-      const unsigned long long mass = refine(use_k, goal, bin_edge(b), bin_edge(b + 1), below_n, below_m);
+      // a bin that holds the depth `start` begins, for the search, behind it
+      const unsigned long long mass = refine(use_k, goal, max(bin_edge(b), above_key), bin_edge(b + 1), below_n, below_m);
       if (use_k && use_p) {
         const uint32_t k_key = cut_key, k_ties = cut_ties;
         const unsigned long long need = mass_needed(top_p, mass);

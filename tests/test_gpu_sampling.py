@@ -75,7 +75,9 @@ def whole_number_rows(logits, uniform, temperature, top_k, top_p, min_p):
     total = run[:, -1:]
     target = torch.minimum((uniform.double().unsqueeze(1) * total.double()).floor().long().clamp(min=0), total - 1)
     token = (run <= target).sum(1).clamp(max=vocab - 1)
-    return torch.where(most[:, 0] == -_INF, -1, token)
+    logprob = z.gather(1, token.unsqueeze(1))[:, 0].double() - (total[:, 0].double() * 2.0 ** -31).log()
+    nothing = most[:, 0] == -_INF
+    return torch.where(nothing, -1, token), torch.where(nothing, -_INF, logprob)
 
 
 def check(logits, uniform, temperature, top_k, top_p, min_p, sure=0.75):
@@ -87,7 +89,12 @@ def check(logits, uniform, temperature, top_k, top_p, min_p, sure=0.75):
     tokens, logprobs = sample_tokens(logits, uniform, temperature, top_k, top_p, min_p)
     assert tokens.dtype == torch.int64 and logprobs.dtype == torch.float32 and tokens.shape == logprobs.shape == (rows,)
     per_row = [full(temperature, torch.float32), full(top_k, torch.int32), full(top_p, torch.float32), full(min_p, torch.float32)]
-    assert torch.equal(tokens, whole_number_rows(logits, uniform, *per_row))
+    whole_tokens, whole_logprobs = whole_number_rows(logits, uniform, *per_row)
+    assert torch.equal(tokens, whole_tokens)
+    # the same kept sum, its logarithm and one subtraction in float32: 2^-22 of each, and of the sum's rounding
+    some = torch.isfinite(whole_logprobs)
+    assert torch.equal(torch.isfinite(logprobs), some)
+    assert ((logprobs.double() - whole_logprobs).abs()[some] <= 2.0 ** -21 * (1 + 25 + whole_logprobs.abs()[some])).all()
     settings = list(zip(uniform.tolist(), *(v.tolist() for v in per_row)))
     agree, vocab = 0, logits.shape[1]
     share = 1e-5 + vocab * 2.0 ** -31
@@ -260,3 +267,37 @@ def test_refusals(cuda):
         sample_tokens(x[:, :0], u)
     tokens, logprobs = sample_tokens(x[:0], u[:0])
     assert tokens.shape == logprobs.shape == (0,)
+
+
+@pytest.mark.parametrize("vocab", [3001, 40013, 151936])
+@pytest.mark.parametrize("depth", [1.0, 3.0, 6.0, 9.0, 12.0, 15.0])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_nucleus_ends_close_to_a_depth(cuda, vocab, depth, dtype):
+    """Entries crowded around one depth below the maximum, a nucleus that ends at every place among them."""
+    rows = 24
+    g = torch.Generator(device=cuda).manual_seed(int(depth))
+    x = -depth + 0.2 * (torch.rand(rows, vocab, generator=g, device=cuda) - 0.5)
+    x[:, 77] = 0.0
+    x = x.to(dtype)
+    top_p = torch.linspace(0.02, 0.999, rows, device=cuda)
+    settings = (torch.rand(rows, generator=g, device=cuda), torch.ones(rows, device=cuda),
+                torch.zeros(rows, dtype=torch.int32, device=cuda), top_p, torch.zeros(rows, device=cuda))
+    tokens, logprobs = sample_tokens(x, settings[0], top_p=top_p)
+    want, want_logprobs = whole_number_rows(x, *settings)
+    assert torch.equal(tokens, want)
+    assert ((logprobs.double() - want_logprobs).abs() <= 2.0 ** -21 * (1 + 25 + want_logprobs.abs())).all()
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_wide_nuclei(cuda, seed):
+    """Many rows of top-p alone: the kept sum is the definition's to the last unit."""
+    rows, vocab = 96, 32003
+    x, u = make(cuda, rows, vocab, torch.float16 if seed % 2 else torch.float32, seed=100 + seed)
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    top_p = torch.tensor([0.7, 0.8, 0.9, 0.95, 0.99], device=cuda)[torch.randint(0, 5, (rows,), generator=g, device=cuda)]
+    t = 0.8 + 0.6 * torch.rand(rows, generator=g, device=cuda)
+    tokens, logprobs = sample_tokens(x, u, temperature=t, top_p=top_p)
+    zero = torch.zeros(rows, device=cuda)
+    want, want_logprobs = whole_number_rows(x, u, t, zero.int(), top_p, zero)
+    assert torch.equal(tokens, want)
+    assert ((logprobs.double() - want_logprobs).abs() <= 2.0 ** -21 * (1 + 25 + want_logprobs.abs())).all()
