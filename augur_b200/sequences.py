@@ -17,6 +17,8 @@ allocator, plus the batched kernels here:
 - decode_step: shared, partially filled last blocks are copied before they
   are appended to (one launch for the batch), then every table grows by one
   position (DecodeStep, or DecodeGraphStep.update for a captured step);
+- shared_prefix_step: the same, for a step that reads the blocks which
+  several sequences hold once for all of them (paged_shared_prefix_attention);
 - release: a finished sequence's blocks go back to the pool once no other
   sequence and no prefix-cache entry holds them.
 
@@ -31,8 +33,11 @@ from collections.abc import Sequence
 from dataclasses import dataclass
 
 import numpy as np
+import torch
+from torch import Tensor
 
-from .batched import cow_partial_blocks
+from .attention import SharedPrefixTables
+from .batched import cow_partial_blocks, decode_slot_mapping
 from .decode import DecodeGraphStep, DecodeStep
 from .paged_kv_cache import PagedKVCache, PagedPrefixCache, SequenceBlockTable, slots_for_positions
 
@@ -137,6 +142,19 @@ class PagedSequences:
         copy-on-write launch here is followed by the step's uploads, so it has finished
         before the first layer's launch)."""
         return DecodeStep(self.cache, self._prepare_append(seq_ids), early_reads=early_reads)
+
+    def shared_prefix_step(self, seq_ids: Sequence[int], n_q_heads: int) -> tuple[Tensor, SharedPrefixTables]:
+        """The next decode step of these sequences for paged_shared_prefix_attention: shared partial
+        last blocks are copied and each table grows by one position. Returns the new tokens'
+        pool slots (int64 on the device; write their keys and values there first, with
+        write_paged_kv_batch or a RoPE form of it) and the plan that all layers share."""
+        tables = self._prepare_append(seq_ids)
+        slots = decode_slot_mapping(tables, self.cache.allocator)  # seq_len += 1 for every table
+        device = self.cache.keys.device
+        on_device = torch.from_numpy(slots)
+        if device.type == "cuda" and slots.size:
+            on_device = on_device.pin_memory().to(device, non_blocking=True)
+        return on_device, SharedPrefixTables(self.cache, tables, n_q_heads)
 
     def update_graph_step(self, step: DecodeGraphStep, seq_ids: Sequence[int]) -> None:
         """decode_step for a captured step: copy shared partial blocks, then step.update."""

@@ -148,3 +148,88 @@ def test_decode_layer_rejects_bad_arguments_without_touching_the_device():
         assert b"outside [0, 24)" in lib.augur_kv_last_error()
     assert lib.augur_kv_decode_layer(ctypes.byref(args), 0, None, None, None, None, None) == _lib.EINVAL
     assert b"null pool" in lib.augur_kv_last_error()
+
+
+@pytest.mark.parametrize("struct,mirror", [("augur_kv_shared_prefix_args", _lib.SharedPrefixArgs),
+                                           ("augur_kv_rope_axes_args", _lib.RopeAxesArgs)])
+def test_args_layouts_match_header(tmp_path, struct, mirror):
+    """The ctypes mirrors have the C structs' sizes and field offsets."""
+    import shutil
+    import subprocess
+
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if cc is None:
+        pytest.skip("no host C compiler")
+    fields = [name for name, _ in mirror._fields_]
+    lines = ['#include <stddef.h>', '#include <stdio.h>', '#include "augur_kv.h"', "int main(void) {",
+             f'  printf("size %zu\\n", sizeof({struct}));']
+    lines += [f'  printf("{f} %zu\\n", offsetof({struct}, {f}));' for f in fields]
+    src = tmp_path / "layout.c"
+    src.write_text("\n".join([*lines, "  return 0;", "}"]) + "\n")
+    exe = tmp_path / "layout"
+    subprocess.run([cc, "-I", os.path.dirname(HEADER), str(src), "-o", str(exe)], check=True)
+    out = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout
+    got = dict(line.split() for line in out.splitlines())
+    assert int(got["size"]) == ctypes.sizeof(mirror)
+    for f in fields:
+        assert int(got[f]) == getattr(mirror, f).offset, f
+
+
+def test_shared_prefix_attention_rejects_bad_arguments_without_touching_the_device():
+    lib = _lib.load()
+    fake = ctypes.c_void_p(16)
+    call = lib.augur_kv_shared_prefix_attention
+    assert call(None, 0, fake, fake, None) == _lib.EINVAL and b"null args" in lib.augur_kv_last_error()
+    args = _lib.SharedPrefixArgs()
+    args.n_layers, args.dtype = 3, _lib.BF16
+    for layer in (-1, 3):
+        assert call(ctypes.byref(args), layer, fake, fake, None) == _lib.EINVAL
+        assert b"outside [0, 3)" in lib.augur_kv_last_error()
+    assert call(ctypes.byref(args), 0, None, None, None) == _lib.OK  # no sequence: nothing is looked at
+    args.batch = 2
+    assert call(ctypes.byref(args), 0, fake, fake, None) == _lib.EINVAL and b"null pointer" in lib.augur_kv_last_error()
+    for f in ("k_pool", "v_pool", "block_tables", "seq_lens", "shared_lens", "ref_starts"):
+        setattr(args, f, 16)
+    args.n_q_heads, args.n_kv_heads, args.head_dim, args.block_size, args.num_blocks, args.max_blocks = 7, 2, 64, 16, 4, 4
+    assert call(ctypes.byref(args), 0, fake, fake, None) == _lib.EINVAL and b"bad sizes" in lib.augur_kv_last_error()
+    args.n_q_heads, args.n_items = 14, 1
+    assert call(ctypes.byref(args), 0, fake, fake, None) == _lib.EINVAL and b"its arrays" in lib.augur_kv_last_error()
+    args.n_items, args.flags = 0, 99
+    assert call(ctypes.byref(args), 0, fake, fake, None) == _lib.EINVAL and b"flags" in lib.augur_kv_last_error()
+    args.flags, args.head_dim = _lib.ATTN_AUTO, 257
+    assert call(ctypes.byref(args), 0, fake, fake, None) == _lib.EINVAL and b"at most" in lib.augur_kv_last_error()
+    cnt, scr = ctypes.c_int64(-1), ctypes.c_int64(-1)
+    sizes = lib.augur_kv_shared_prefix_workspace
+    assert sizes(4, 2, 13, 2, 64, 10, ctypes.byref(cnt), ctypes.byref(scr)) == _lib.EINVAL
+    assert sizes(4, 2, 14, 2, 64, 10, ctypes.byref(cnt), ctypes.byref(scr)) == _lib.OK
+    assert cnt.value >= 0 and scr.value >= 4 * 128 * 66 * 4
+
+
+def test_rope_axes_and_sample_reject_bad_arguments_without_touching_the_device():
+    lib = _lib.load()
+    fake = ctypes.c_void_p(16)
+    call = lib.augur_kv_rope_axes_scatter
+    assert call(None, 0, fake, fake, fake, fake, fake, fake, None) == _lib.EINVAL
+    args = _lib.RopeAxesArgs()
+    args.n_layers, args.dtype = 2, _lib.F16
+    assert call(ctypes.byref(args), 2, fake, fake, fake, fake, fake, fake, None) == _lib.EINVAL
+    assert b"outside [0, 2)" in lib.augur_kv_last_error()
+    assert call(ctypes.byref(args), 0, None, None, None, None, None, None, None) == _lib.OK  # no token
+    args.n_tokens = 5
+    assert call(ctypes.byref(args), 0, None, fake, fake, fake, fake, fake, None) == _lib.EINVAL
+    for f in ("k_pool", "v_pool", "inv_freq", "axis_of_frequency"):
+        setattr(args, f, 16)
+    args.n_q_heads = args.n_kv_heads = args.block_size = args.num_blocks = args.n_axes = 1
+    args.head_dim = 7
+    assert call(ctypes.byref(args), 0, fake, fake, fake, fake, fake, fake, None) == _lib.EINVAL
+    assert b"even" in lib.augur_kv_last_error()
+
+    def sample(rows, vocab, dtype, logits=fake):
+        return lib.augur_kv_sample(logits, vocab, rows, vocab, dtype, fake, None, 1.0, None, 0, None, 1.0, None, 0.0, fake, None, None)
+
+    assert sample(1, 10, 9) == _lib.EINVAL and b"dtype" in lib.augur_kv_last_error()
+    assert sample(-1, 10, _lib.F32) == _lib.EINVAL and sample(1, 0, _lib.F32) == _lib.EINVAL
+    assert sample(1, (1 << 21) + 1, _lib.F32) == _lib.EINVAL and b"bad sizes" in lib.augur_kv_last_error()
+    assert sample(0, 10, _lib.F32, None) == _lib.OK
+    assert sample(1, 10, _lib.F32, None) == _lib.EINVAL and b"null pointer" in lib.augur_kv_last_error()
+    assert sample(1, 10, _lib.F32, ctypes.c_void_p(18)) == _lib.EINVAL and b"aligned" in lib.augur_kv_last_error()
