@@ -403,19 +403,19 @@ def _shared_runs(rows: np.ndarray, full: np.ndarray, min_saved: int) -> tuple[li
     return runs, covered
 
 
-def _ranges(tiles: Sequence[int], units: Sequence[int], steps: Sequence[float], ctas: int, least: int) -> list[int]:
+def _ranges(tiles: Sequence[int], units: Sequence[int], steps: Sequence[float], ctas: int) -> list[int]:
     """Into how many key ranges each run's tiles are cut: tiles[i] key tiles, each range an item
     for each of units[i] (row tiles x KV heads), steps[i] of a CTA's steps a tile.
 
     An item costs its steps and a start and an end worth about _ITEM_STEPS more. With c items'
     cost a CTA: one wave takes its longest item; several take their average and half an item.
-    The range length that this makes cheapest is taken, `least` tiles or more."""
+    The range length that this makes cheapest is taken, a step or more."""
     if not tiles:
         return []
     best, longest = None, max(tiles)
-    lengths = sorted({max(least, -(-longest // n)) for n in (*range(1, 33), 40, 48, 64, 80, 96, 112, 128, ctas)}, reverse=True)
+    lengths = sorted({-(-longest // n) for n in (*range(1, 33), 40, 48, 64, 80, 96, 112, 128, ctas)}, reverse=True)
     for per in lengths:
-        ranges = [-(-t // per) for t in tiles]
+        ranges = [-(-t // max(per, 2 if s < 1 else 1)) for t, s in zip(tiles, steps)]
         items = sum(n * u for n, u in zip(ranges, units))
         most = max(-(-t // n) * s for t, n, s in zip(tiles, ranges, steps)) + _ITEM_STEPS
         total = items * _ITEM_STEPS + sum(t * u * s for t, u, s in zip(tiles, units, steps))
@@ -470,7 +470,7 @@ class SharedPrefixTables:
         # a tensor-core item of one row tile works on two key tiles at a time; the float32 kernel is slower a tile
         wide = cache.keys.dtype != torch.float32
         ranges = _ranges(tiles, [-(-rt // 2) * Hkv for rt in row_tiles],
-                         [(0.5 if rt == 1 else 1.0) if wide else 8.0 for rt in row_tiles], ctas, 2 if wide else 1)
+                         [(0.5 if rt == 1 else 1.0) if wide else 8.0 for rt in row_tiles], ctas)
         items: list[tuple[int, ...]] = []
         refs: list[list[tuple[int, ...]]] = [[] for _ in range(B)]
         member0 = block0 = slab = 0
