@@ -439,7 +439,7 @@ class SharedPrefixTables:
                  seq_lens: Sequence[int] | None = None, stream: torch.cuda.Stream | None = None,
                  min_saved_bytes: int | None = None) -> None:
         """stream: the stream the copy is ordered on (the current one by default); launches on
-        another stream wait for it. min_saved_bytes: how much reading (bytes of one layer) the
+        another stream wait for it (a captured graph's replays have to be ordered behind it). min_saved_bytes: how much reading (bytes of one layer) the
         runs must spare to be taken apart; where they spare less, each sequence reads them
         itself, which is then faster (None: the measured threshold)."""
         L, NB, Hkv, bs, D = cache.keys.shape
@@ -517,14 +517,14 @@ class SharedPrefixTables:
         if device.type == "cuda":
             self.uploaded = torch.cuda.Event()
             self.uploaded.record(stream if stream is not None else torch.cuda.current_stream(device))
-        self._fast: tuple | None = None
+        self._ready: tuple | None = None  # an argument block, and the layouts and stream it is for
 
     def _prepare(self, q: Tensor, out: Tensor, cache: PagedKVCache, st: torch.cuda.Stream, flags: int) -> _lib.SharedPrefixArgs:
         """The argument block of a call with q and out laid out like these ([batch, heads, head_dim])."""
         lib = _lib.load()
         L, NB, Hkv, bs, D = cache.keys.shape
         Hq = self.n_q_heads
-        if self.uploaded is not None:
+        if self.uploaded is not None and not torch.cuda.is_current_stream_capturing():
             st.wait_event(self.uploaded)
         cnt, scr = _shared_workspace(lib, q.device, st, (self.n_slabs, self.batch, Hq, Hkv, D, self.max_own_len))
         d, a = self._dev, _lib.SharedPrefixArgs()
@@ -543,7 +543,7 @@ class SharedPrefixTables:
         a.scratch, a.scratch_bytes = scr.data_ptr(), scr.numel()
         a.counters, a.counters_bytes = cnt.data_ptr(), cnt.numel() * 4
         a.status = _ops.status_word(q.device).data_ptr()
-        a._keep = (cnt, scr, cache)  # what the block points into stays alive with it
+        a._keep = (cnt, scr)  # the block points into them
         return a
 
 
@@ -567,16 +567,22 @@ def _shared_workspace(lib, device: torch.device, st: torch.cuda.Stream, sizes: t
     _lib.check(lib.augur_kv_shared_prefix_workspace(*sizes, ctypes.byref(need_c), ctypes.byref(need_s)),
                "augur_kv_shared_prefix_workspace")
     key = (device.index, st.cuda_stream)
-    cnt, scr = _shared_workspaces.get(key, (None, None))
+    capturing = torch.cuda.is_current_stream_capturing()  # a graph owns what it uses: a pair of its own
+    cnt, scr = (None, None) if capturing else _shared_workspaces.get(key, (None, None))
     if cnt is None or cnt.numel() * 4 < need_c.value or scr.numel() < need_s.value:
         with torch.cuda.stream(st):
             if cnt is None or cnt.numel() * 4 < need_c.value:
                 cnt = torch.zeros(max(1, need_c.value // 4), dtype=torch.int32, device=device)
             if scr is None or scr.numel() < need_s.value:
                 scr = torch.empty(max(64, need_s.value), dtype=torch.uint8, device=device)
-        if not torch.cuda.is_current_stream_capturing():  # a graph owns what its capture allocates
+        if not capturing:
             _shared_workspaces[key] = (cnt, scr)
     return cnt, scr
+
+
+def _shared_layout(q: Tensor, keys: Tensor, values: Tensor) -> tuple:
+    return (q.shape, q.stride(), q.dtype, q.get_device(), keys.shape, keys.stride(), keys.dtype, keys.get_device(),
+            values.shape, values.stride(), values.dtype, values.get_device())
 
 
 def paged_shared_prefix_attention(
@@ -602,18 +608,19 @@ def paged_shared_prefix_attention(
     is rounded once, so results differ from paged_decode_attention's, which rounds scores and
     probabilities where the reference does, within that rounding.
     """
-    fast = tables._fast if type(tables) is SharedPrefixTables else None
-    if (fast is not None and out is None and stream is None and kernel == "auto" and fast[0] is cache
-            and q.shape == fast[1] and q.stride() == fast[2] and q.dtype is fast[3] and q.get_device() == fast[4]
-            and cache.keys.data_ptr() == fast[5] and 0 <= layer_idx < fast[6]
-            and _ops.current_device() == fast[4]):
-        st_raw = _ops.current_raw_stream(fast[4])
-        if st_raw == fast[7]:
+    # the layers of a step: tensors laid out as the last call's were need no checks again
+    ready = tables._ready if type(tables) is SharedPrefixTables else None
+    if ready is not None and out is None and stream is None and kernel == "auto":
+        layout, index, n_layers, st_raw, a, at, fn, launches = ready
+        if (_shared_layout(q, cache.keys, cache.values) == layout and 0 <= layer_idx < n_layers
+                and _ops.current_device() == index and _ops.current_raw_stream(index) == st_raw
+                and not torch.cuda.is_current_stream_capturing()):
             res = torch.empty_like(q, memory_format=torch.contiguous_format)
-            code = fast[9](fast[8], layer_idx, q.data_ptr(), res.data_ptr(), st_raw)
+            a.k_pool, a.v_pool = cache.keys.data_ptr(), cache.values.data_ptr()
+            code = fn(at, layer_idx, q.data_ptr(), res.data_ptr(), st_raw)
             if code != 0:
                 _lib.check(code, "augur_kv_shared_prefix_attention")
-            _ops.launch_count += fast[10]
+            _ops.launch_count += launches
             return res
     if kernel not in ("auto", "tcgen05", "generic"):
         raise ValueError("kernel must be 'auto', 'tcgen05' or 'generic'")
@@ -661,9 +668,9 @@ def paged_shared_prefix_attention(
                    "augur_kv_shared_prefix_attention")
     launches = 1 + (plan.n_items > 0)
     _ops.launch_count += launches
-    _ops.keep_until_done(st, rows, res, *plan._dev.values(), *a._keep[:2])
+    _ops.keep_until_done(st, rows, res, *plan._dev.values(), *a._keep)
     if (rows is q3 and out is None and stream is None and kernel == "auto"
             and not torch.cuda.is_current_stream_capturing()):
-        plan._fast = (cache, q.shape, q.stride(), q.dtype, q.get_device(), cache.keys.data_ptr(), L, st.cuda_stream,
-                      ctypes.addressof(a), fn, launches, a)
+        plan._ready = (_shared_layout(q, cache.keys, cache.values), q.get_device(), L, st.cuda_stream, a, ctypes.addressof(a),
+                       fn, launches)
     return res

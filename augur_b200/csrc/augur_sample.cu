@@ -147,8 +147,6 @@ template <> struct Logit<__half> {
   }
 };
 
-__device__ __forceinline__ float no_nan(float x) { return x == x ? x : kNegInf; }  // a NaN is never drawn
-
 // floats as unsigned integers of the same order
 __device__ __forceinline__ uint32_t ordered(float x) {
   const uint32_t b = __float_as_uint(x);
@@ -964,7 +962,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a) {
             const int i = first + s0 + lane * VEC + j;
             a.tokens[row] = i;
             if (a.logprobs) {
-              const float z = sc.z(no_nan(Logit<T>::one(base + int64_t(i) * int64_t(sizeof(T)))));
+              const float z = sc.z(Logit<T>::one(base + int64_t(i) * int64_t(sizeof(T))));
               a.logprobs[row] = z - logf(float(double(whole) / double(kUnit)));
             }
           }

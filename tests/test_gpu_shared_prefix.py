@@ -208,6 +208,34 @@ def test_captured_in_a_graph_and_repeatable(cuda):
     case.check(out)
 
 
+def test_a_graph_has_scratch_of_its_own(cuda):
+    case = Case(cuda, torch.bfloat16, 14, 2, 64, 16, _BATCHES["long answers"], seed=6)
+    plan = SharedPrefixTables(case.pool, case.tables, 14)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):  # its first use: nothing is there from an eager call
+        out = paged_shared_prefix_attention(case.q, case.pool, case.layer, plan)
+    other = Case(cuda, torch.bfloat16, 14, 2, 64, 16, _BATCHES["long answers"], seed=7)
+    for _ in range(3):
+        graph.replay()
+        with torch.cuda.stream(side):
+            side.wait_stream(torch.cuda.current_stream())
+            got = paged_shared_prefix_attention(other.q, other.pool, other.layer, other.tables)
+    torch.cuda.synchronize()
+    case.check(out)
+    other.check(got)
+
+
+def test_values_replaced_between_layers(cuda):
+    case = Case(cuda, torch.bfloat16, 14, 2, 64, 16, _BATCHES["long answers"], seed=8)
+    plan = SharedPrefixTables(case.pool, case.tables, 14)
+    first = paged_shared_prefix_attention(case.q, case.pool, case.layer, plan)
+    case.pool.values = case.pool.values * 2  # exact in the type: twice the output
+    again = paged_shared_prefix_attention(case.q, case.pool, case.layer, plan)
+    assert torch.equal(again, first * 2)
+
+
 def test_agrees_with_paged_decode_attention(cuda):
     case = Case(cuda, torch.bfloat16, 14, 2, 64, 16, forks(32, 1024, 16, lambda i: 1 + 3 * i))
     got = paged_shared_prefix_attention(case.q, case.pool, case.layer, case.tables)
