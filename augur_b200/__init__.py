@@ -10,8 +10,9 @@ error messages):
 plus batched all-layer entry points in augur_b200.batched and sequence
 sharding / peer push in augur_b200.sharding and augur_b200.peer, and the
 cache's consumers that read the pool in place in augur_b200.attention
-(decode and prefill attention) and augur_b200.decode. Every byte of cache
-data the device moves goes through libaugur_kv.so (include/augur_kv.h);
+(decode, prefill and shared-prefix decode attention) and augur_b200.decode,
+rotary positions in augur_b200.rope and token sampling in
+augur_b200.sampling. Every byte of cache data the device moves goes through libaugur_kv.so (include/augur_kv.h);
 there is no CPU fallback.
 """
 

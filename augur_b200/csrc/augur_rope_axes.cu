@@ -17,7 +17,11 @@
 // table of positions, so none to grow or to read) and where their slots lie,
 // with its first pieces of q, k and v already on their way, and then turns
 // pieces of 16 bytes of a row's first half together with the matching 16 bytes of
-// the second, kBatch pieces of a thread under way at a time.
+// the second, kBatch pieces of a thread under way at a time. Measured: 40,001
+// tokens of 32 / 8 heads of 128 in fp16 (984 MB): 172 us, 5.7 TB/s; 8,191 of 14 / 2
+// heads of 64 in bf16 (38 MB): 8.4 us, where half is the start of a launch; 48: 2.9 us.
+// (A slot and angles looked up by each piece took 197 and 16.2 us: the latency of
+// two dependent loads, and a sine and a cosine for every head.)
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -443,6 +443,9 @@ __device__ __forceinline__ void generic_attend(const Args& a, float* sq, int n, 
   l += __shfl_xor_sync(0xffffffffu, l, 2);
 }
 
+// A work item on CUDA cores: up to 64 of its rows at a time go over the item's keys, 32 of them in
+// shared memory. Bound by shared-memory reads: each K and V value in it serves 64 rows, where
+// own_generic_kernel would fetch it again for every sequence.
 template <typename T>
 __global__ void __launch_bounds__(kGThreads) shared_generic_kernel(Args a) {
   extern __shared__ __align__(16) float gsm[];
@@ -510,7 +513,8 @@ __device__ __forceinline__ bool last_to_arrive(const Args& a, int unit) {
 // memory; a warp takes query heads w, w + 8, ..: for the scores its lanes are the
 // keys, for P V the dims (kDims = head_dim / 32 of them a lane, rounded up to 2, 4 or 8).
 // The next 32 keys' rows are on their way to registers meanwhile. Bound by the
-// latency of those loads with few heads, by shared-memory reads with many.
+// latency of those loads with few heads, by shared-memory reads with many
+// (24 float32 sequences of 333 to 1,060 tokens, 14 / 2 heads of 64: 15.6 us).
 template <typename T, int kDims>
 __global__ void __launch_bounds__(kGThreads) own_generic_kernel(Args a) {
   extern __shared__ __align__(16) float gsm[];
@@ -651,7 +655,10 @@ __global__ void __launch_bounds__(kGThreads) own_generic_kernel(Args a) {
 // which also cover each other's starts and joins. The CTA joins
 // the warps, the run's slabs and (for long own parts) the other CTAs' parts,
 // whose last arrival writes the output (it joins them in their order, so the
-// result does not depend on the order of arrival). Bound by HBM: K and V rows are read once.
+// result does not depend on the order of arrival). Bound by HBM: K and V rows
+// are read once. Measured: 216 answers of up to 700 tokens, 32 / 8 heads of 128 (323 MB):
+// 67 us beside the shared launch, 4.9 TB/s; 8 of 500 tokens, 14 / 2 heads of 64: 7.9 us, all
+// latency (launch, lengths, block ids, rows, join).
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -911,7 +918,10 @@ __global__ void __launch_bounds__(kOwnThreads, OwnCfg<D>::kCtas) own_mma_kernel(
 // products 1,024 (head_dim 64) or 2,048 (128); it takes about 3,500, in which each
 // group spends 2,000 on its softmax and 1,400 waiting for its next S. (A
 // quarter or a half of the exponentials on the FMA pipes changed nothing, nor
-// did rows that lie in L2.) With few rows it is bound by HBM.
+// did rows that lie in L2, nor S in halves of 64 keys that take turns, whose products
+// are slower by as much as the waits were shorter.) 64 questions over 98,304
+// tokens, 32 / 8 heads of 128 in bf16: 101 us, 1.02 PFLOP/s and 4.0 TB/s; tensor and
+// exponential pipes are each busy 57 % of it. With few rows it is bound by HBM.
 //
 // Every wait is bounded (2 s of %globaltimer); on expiry the CTA records
 // AUGUR_KV_ETIMEOUT, drains its copies and products, frees its tensor memory and returns.
