@@ -467,10 +467,16 @@ class SharedPrefixTables:
         ctas = _sm_count(device)
         row_tiles = [-(-m.size * groups // _TILE_ROWS) for m, _, _ in runs]
         tiles = [-(-(end - start) * bs // _TILE_KEYS) for _, start, end in runs]
-        # a tensor-core item of one row tile works on two key tiles at a time; the float32 kernel is slower a tile
-        wide = cache.keys.dtype != torch.float32
-        ranges = _ranges(tiles, [-(-rt // 2) * Hkv for rt in row_tiles],
-                         [(0.5 if rt == 1 else 1.0) if wide else 8.0 for rt in row_tiles], ctas)
+        if cache.keys.dtype != torch.float32:
+            # an item of one row tile works on two key tiles at a time
+            ranges = _ranges(tiles, [-(-rt // 2) * Hkv for rt in row_tiles], [0.5 if rt == 1 else 1.0 for rt in row_tiles], ctas)
+        else:
+            # CTAs of 32 rows, two an SM; groups of four rows share their eight warps, which take 8 keys at a time (4 with
+            # wide heads), about 1.1 us each
+            rows_of = [m.size * groups for m, _, _ in runs]
+            warps = [1 if n > 16 else 2 if n > 8 else 4 if n > 4 else 8 for n in rows_of]  # on the keys of a row
+            ranges = _ranges(tiles, [-(-n // 32) * Hkv for n in rows_of],
+                             [0.6 * _TILE_KEYS / (8 if D <= 64 else 4) / w for w in warps], 2 * ctas)
         items: list[tuple[int, ...]] = []
         refs: list[list[tuple[int, ...]]] = [[] for _ in range(B)]
         member0 = block0 = slab = 0

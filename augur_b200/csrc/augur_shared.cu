@@ -71,7 +71,8 @@ struct Args {
   float scale;  // log2(e) / sqrt(head_dim)
   char* out;
   int64_t out_stride_b, out_stride_h;
-  int32_t out_wide;  // output rows are aligned to four values
+  int32_t out_wide;   // output rows are aligned to four values
+  int32_t rows_wide;  // query and pool rows are
   const Item* items;
   int32_t n_items;
   const int32_t* members;
@@ -348,142 +349,297 @@ __host__ __device__ constexpr int join_bytes(int groups) { return groups * (kJoi
 // CUDA cores: any type and shape, float32 throughout
 // ---------------------------------------------------------------------------
 
-constexpr int kGRows = 64;   // rows at a time: four threads each
-constexpr int kGKeys = 32;   // keys at a time
-constexpr int kGThreads = kGRows * 4;
+// Two float32 operations at a time.
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+constexpr int kGWarps = 8;
+constexpr int kGThreads = kGWarps * 32;
+constexpr int kGMaxRows = 64;  // of a CTA
+constexpr int kGKeys = 32;     // parts of a sequence are cut at multiples of these
 constexpr int kGMaxDim = 256;
 
-// Shared memory of the generic kernels, in floats: q [64][pitch], k and v [32][pitch], p [64][33].
+// What the generic kernels work with: kLanes lanes hold a key's row, kEach dims a lane; a warp keeps kRows
+// query rows in registers.
+template <int kEach_, int kLanes_, int kRows_> struct Shape {
+  static constexpr int kEach = kEach_, kLanes = kLanes_, kRows = kRows_;
+};
 __host__ __device__ constexpr int generic_pitch(int D) { return ((D + 3) & ~3) + 4; }
-__host__ __device__ constexpr int generic_floats(int D) {
-  return (kGRows + 2 * kGKeys) * generic_pitch(D) + kGRows * (kGKeys + 1);
+
+// Dims d0 .. of a row; past head_dim (and without a row): zero
+template <typename T, int kEach> struct alignas(kEach * sizeof(T) < 16 ? kEach * sizeof(T) : 16) Dims {
+  T v[kEach];
+};
+template <typename T, int kEach>
+__device__ __forceinline__ void load_dims(Dims<T, kEach>& x, const char* row, int d0, int D, bool wide) {
+  if (wide) {  // every row aligned, head_dim a multiple of four: a group of four lies in the row or past it
+    constexpr int kVec = sizeof(T) == 4 ? 4 : kEach < 8 ? kEach : 4;
+    using V = Dims<T, kVec>;
+#pragma unroll
+    for (int c = 0; c < kEach / kVec; ++c) {
+      V y;
+      if (row != nullptr && d0 + c * kVec < D) {
+        y = *reinterpret_cast<const V*>(reinterpret_cast<const T*>(row) + d0 + c * kVec);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) y.v[i] = Elem<T>::from_f(0.f);
+      }
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) x.v[c * kVec + i] = y.v[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      x.v[i] = row != nullptr && d0 + i < D ? reinterpret_cast<const T*>(row)[d0 + i] : Elem<T>::from_f(0.f);
+  }
 }
 
-// Attention of up to 64 rows (already in sq) over n keys; key_off(j) is key j's byte offset in the
-// pool (-1: skipped). Thread tid works for row tid / 4 and dims 4 (4 i + tid % 4) ..: leaves m, l and o.
-template <typename T, typename F>
-__device__ __forceinline__ void generic_attend(const Args& a, float* sq, int n, F key_off, float& m, float& l,
-                                               float (&o)[kGMaxDim / 4]) {
-  const int D = a.head_dim, P = generic_pitch(D), tid = threadIdx.x, r = tid >> 2, part = tid & 3;
-  float* sk = sq + kGRows * P;
-  float* sv = sk + kGKeys * P;
-  float* sp = sv + kGKeys * P;
-  m = kNegInf;
-  l = 0.f;
+// A warp attends to 4 x (32 / kLanes) keys of every `stride` from `first` on, with `n_rows` (at most kRows) query rows. A
+// score's sum over the lanes starts with two exchanges of halves, after which lane i is left with key i % 4's alone: fewer
+// exchanges, and an exponential for every fourth lane's key. The next keys' rows are fetched into the registers of these as
+// they fall free. key_off(j): key j's byte offset in the pool, or -1.
+// row_of(i): query row i. Leaves the parts' (m, l, O) in shared memory at row0 + i.
+template <typename T, typename S, typename Row, typename Key>
+__device__ __forceinline__ void warp_attend(const Args& a, Row row_of, int n_rows, int first, int last, int stride, Key key_off,
+                                            float* out_ml, float* out_o, int pitch) {
+  constexpr int kEach = S::kEach, kLanes = S::kLanes, kRows = S::kRows, kSubs = 32 / kLanes;
+  const int lane = threadIdx.x & 31, sub = lane / kLanes, d0 = lane % kLanes * kEach, D = a.head_dim;
+  uint64_t q[kRows][kEach / 2], o[kRows][kEach / 2];
+  float m[kRows], l[kRows];
 #pragma unroll
-  for (int i = 0; i < kGMaxDim / 4; ++i) o[i] = 0.f;
-  for (int k0 = 0; k0 < n; k0 += kGKeys) {
-    __syncthreads();
-    for (int i = tid >> 5; i < kGKeys; i += kGThreads / 32) {  // a warp per key
-      const int64_t off = k0 + i < n ? key_off(k0 + i) : -1;
-      for (int d = tid & 31; d < D; d += 32) {
-        sk[i * P + d] = off >= 0 ? Elem<T>::to_f(reinterpret_cast<const T*>(a.k + off)[d]) : 0.f;
-        sv[i * P + d] = off >= 0 ? Elem<T>::to_f(reinterpret_cast<const T*>(a.v + off)[d]) : 0.f;
-      }
-      if ((tid & 31) == 0) sp[i * (kGKeys + 1) + kGKeys] = off >= 0 ? 0.f : kNegInf;  // the mask, beside p
+  for (int r = 0; r < kRows; ++r) {
+    Dims<T, kEach> x;
+    load_dims<T, kEach>(x, r < n_rows ? row_of(r) : nullptr, d0, D, a.rows_wide);
+#pragma unroll
+    for (int c = 0; c < kEach / 2; ++c) {
+      q[r][c] = pack2(Elem<T>::to_f(x.v[2 * c]) * a.scale, Elem<T>::to_f(x.v[2 * c + 1]) * a.scale);
+      o[r][c] = 0;
     }
-    __syncthreads();
-    float s[kGKeys / 4];
+    m[r] = kNegInf;
+    l[r] = 0.f;
+  }
+  // Lane i finds the row of key i of the next kAhead steps: a block id and a division for 32 keys at a time.
+  constexpr int kStep = 4 * kSubs, kAhead = 32 / kStep;
+  auto find = [&](int k) -> int64_t {
+    const int key = k + lane / kStep * stride + lane % kStep;
+    return key < last ? key_off(key) : -1;
+  };
+  int64_t off[4], found = -1, found_next = -1;
+  auto offsets = [&](int t, int k) {  // of step t, the one that begins at key k
+    if (t % kAhead == 0) {
+      found = found_next;
+      found_next = find(k + kAhead * stride);
+    }
 #pragma unroll
-    for (int j = 0; j < kGKeys / 4; ++j) s[j] = 0.f;
-    if ((D & 3) == 0) {
-      for (int d = 0; d < D; d += 4) {
-        const float4 x = *reinterpret_cast<const float4*>(sq + r * P + d);
+    for (int u = 0; u < 4; ++u) off[u] = __shfl_sync(0xffffffffu, found, t % kAhead * kStep + u * kSubs + sub);
+  };
+  Dims<T, kEach> kx[4], vx[4];
+  auto fetch = [&](Dims<T, kEach>(&x)[4], const char* pool) {
 #pragma unroll
-        for (int j = 0; j < kGKeys / 4; ++j) {
-          const float4 y = *reinterpret_cast<const float4*>(sk + (j * 4 + part) * P + d);
-          s[j] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, s[j]))));
-        }
+    for (int u = 0; u < 4; ++u) load_dims<T, kEach>(x[u], off[u] >= 0 ? pool + off[u] : nullptr, d0, D, a.rows_wide);
+  };
+  const bool b0 = lane & 1, b1 = lane & 2;
+  auto mine_of = [&] { return (b1 ? (b0 ? off[3] : off[2]) : (b0 ? off[1] : off[0])) >= 0; };
+  bool mine = false;
+  if (first < last) {
+    found_next = find(first);
+    offsets(0, first);
+    fetch(kx, a.k);
+    fetch(vx, a.v);
+    mine = mine_of();
+    offsets(1, first + stride);
+  }
+  int t = 2;
+  for (int k = first; k < last; k += stride, ++t) {
+    float p[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      if (r >= n_rows) break;
+      float s[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        uint64_t t = 0;
+#pragma unroll
+        for (int c = 0; c < kEach / 2; ++c)
+          t = fma2(q[r][c], pack2(Elem<T>::to_f(kx[u].v[2 * c]), Elem<T>::to_f(kx[u].v[2 * c + 1])), t);
+        float x, y;
+        unpack2(t, x, y);
+        s[u] = x + y;
       }
-    } else {
-      for (int d = 0; d < D; ++d) {
-        const float x = sq[r * P + d];
+      const float s01 = (b0 ? s[1] : s[0]) + __shfl_xor_sync(0xffffffffu, b0 ? s[0] : s[1], 1);
+      const float s23 = (b0 ? s[3] : s[2]) + __shfl_xor_sync(0xffffffffu, b0 ? s[2] : s[3], 1);
+      float x = (b1 ? s23 : s01) + __shfl_xor_sync(0xffffffffu, b1 ? s01 : s23, 2);
 #pragma unroll
-        for (int j = 0; j < kGKeys / 4; ++j) s[j] = fmaf(x, sk[(j * 4 + part) * P + d], s[j]);
+      for (int w = 4; w < kLanes; w *= 2) x += __shfl_xor_sync(0xffffffffu, x, w);
+      p[r] = mine ? x : kNegInf;
+    }
+    fetch(kx, a.k);  // the next keys, while the sums are taken
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      if (r >= n_rows) break;
+      float mx = fmaxf(p[r], __shfl_xor_sync(0xffffffffu, p[r], 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float mn = fmaxf(m[r], mx), alpha = m[r] == kNegInf ? 0.f : ex2(m[r] - mn);
+      const uint64_t alpha2 = pack2(alpha, alpha);
+      m[r] = mn;
+      const float x = p[r];
+      p[r] = mn == kNegInf && x == x ? 0.f : ex2(x - mn);
+      l[r] = fmaf(l[r], alpha, p[r]);
+#pragma unroll
+      for (int c = 0; c < kEach / 2; ++c) o[r][c] = fma2(o[r][c], alpha2, 0);
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      if (r >= n_rows) break;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float pu = __shfl_sync(0xffffffffu, p[r], (lane & ~3) | u);
+        const uint64_t p2 = pack2(pu, pu);
+#pragma unroll
+        for (int c = 0; c < kEach / 2; ++c)
+          o[r][c] = fma2(p2, pack2(Elem<T>::to_f(vx[u].v[2 * c]), Elem<T>::to_f(vx[u].v[2 * c + 1])), o[r][c]);
       }
     }
-    float mx = kNegInf;
+    fetch(vx, a.v);  // while the next scores are
+    mine = mine_of();
+    offsets(t, k + 2 * stride);
+  }
 #pragma unroll
-    for (int j = 0; j < kGKeys / 4; ++j) {
-      s[j] = s[j] * a.scale + sp[(j * 4 + part) * (kGKeys + 1) + kGKeys];
-      mx = fmaxf(mx, s[j]);
-    }
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    const float mn = fmaxf(m, mx);
-    const float alpha = mn == kNegInf ? 1.f : ex2(m - mn);
-    m = mn;
-    l *= alpha;
-    __syncwarp();
+  for (int r = 0; r < kRows; ++r) {
+    if (r >= n_rows) break;
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    float v[kEach];
 #pragma unroll
-    for (int j = 0; j < kGKeys / 4; ++j) {
-      const float p = mn == kNegInf ? 0.f : ex2(s[j] - mn);
-      l += p;
-      sp[r * (kGKeys + 1) + j * 4 + part] = p;
-    }
-    __syncwarp();
+    for (int c = 0; c < kEach / 2; ++c) unpack2(o[r][c], v[2 * c], v[2 * c + 1]);
+    if constexpr (kSubs == 2) {
+      const float other = __shfl_xor_sync(0xffffffffu, m[r], 16), mn = fmaxf(m[r], other);
+      const float f = m[r] == kNegInf ? 0.f : ex2(m[r] - mn);
+      l[r] = l[r] == 0.f ? 0.f : l[r] * f;  // a NaN stays
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 16);
 #pragma unroll
-    for (int i = 0; i < kGMaxDim / 4; ++i) o[i] *= alpha;
-    for (int j = 0; j < kGKeys; ++j) {
-      const float p = sp[r * (kGKeys + 1) + j];
-#pragma unroll
-      for (int i = 0; i < kGMaxDim / 16; ++i) {
-        const int d = 16 * i + 4 * part;
-        if (d < D) {  // of the last four, those past D lie in the row's padding and are not stored
-          const float4 y = *reinterpret_cast<const float4*>(sv + j * P + d);
-          o[4 * i] = fmaf(p, y.x, o[4 * i]);
-          o[4 * i + 1] = fmaf(p, y.y, o[4 * i + 1]);
-          o[4 * i + 2] = fmaf(p, y.z, o[4 * i + 2]);
-          o[4 * i + 3] = fmaf(p, y.w, o[4 * i + 3]);
-        }
+      for (int c = 0; c < kEach; ++c) {
+        v[c] *= f;
+        v[c] += __shfl_xor_sync(0xffffffffu, v[c], 16);
       }
+      m[r] = mn;
+    }
+    if (lane == 0) {
+      out_ml[2 * r] = m[r];
+      out_ml[2 * r + 1] = l[r];
+    }
+    if (sub == 0) {
+#pragma unroll
+      for (int c = 0; c < kEach; ++c)
+        if (d0 + c < a.quads * 4) out_o[r * pitch + d0 + c] = v[c];
     }
   }
-  l += __shfl_xor_sync(0xffffffffu, l, 1);
-  l += __shfl_xor_sync(0xffffffffu, l, 2);
 }
 
-// A work item on CUDA cores: up to 64 of its rows at a time go over the item's keys, 32 of them in
-// shared memory. Bound by shared-memory reads: each K and V value in it serves 64 rows, where
-// own_generic_kernel would fetch it again for every sequence.
-template <typename T>
-__global__ void __launch_bounds__(kGThreads) shared_generic_kernel(Args a) {
+// How a CTA's warps share `rows` query rows and their keys: row groups of kRows, and as many warps on each
+// group's keys as there are to spare.
+struct Split {
+  int groups, key_warps;
+  __device__ __forceinline__ Split(int rows, int each) {
+    groups = (rows + each - 1) / each;
+    const int g = groups <= 1 ? 1 : groups <= 2 ? 2 : groups <= 4 ? 4 : kGWarps;
+    key_warps = kGWarps / g;
+  }
+};
+// The `rows` rows' parts, [key_warps][rows], in shared memory, of keys [first, last). All threads call it.
+template <typename T, typename S, typename Row, typename Key>
+__device__ __forceinline__ void cta_attend(const Args& a, Row row_of, int rows, Split sp, int first, int last, Key key_off,
+                                           float* ml, float* o, int pitch) {
+  constexpr int kStep = 4 * (32 / S::kLanes);  // keys of a warp's step
+  const int warp = threadIdx.x >> 5, part = warp % sp.key_warps;
+  for (int g = warp / sp.key_warps; g < sp.groups; g += kGWarps / sp.key_warps) {
+    const int r0 = g * S::kRows, at = part * rows + r0;
+    warp_attend<T, S>(a, [&](int r) { return row_of(r0 + r); }, min(S::kRows, rows - r0), first + part * kStep, last,
+                      sp.key_warps * kStep, key_off, ml + 2 * at, o + at * pitch, pitch);
+  }
+  __syncthreads();
+}
+// Joins the parts of row r: its reference and sum, and the parts' factors.
+__device__ __forceinline__ float2 part_factors(const float* ml, int rows, int parts, int r, float (&f)[kGWarps]) {
+  float m = kNegInf, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < kGWarps; ++i)
+    if (i < parts) m = fmaxf(m, ml[2 * (i * rows + r)]);
+#pragma unroll
+  for (int i = 0; i < kGWarps; ++i) {
+    f[i] = 0.f;
+    if (i < parts) {
+      const float x = ml[2 * (i * rows + r)], y = ml[2 * (i * rows + r) + 1];
+      f[i] = x == kNegInf ? 0.f : ex2(x - m);
+      l += y == 0.f ? 0.f : x == kNegInf ? y : y * f[i];
+    }
+  }
+  return make_float2(m, l);
+}
+__device__ __forceinline__ float4 join_quad(const float* o, int pitch, int rows, int parts, int r, int quad, const float (&f)[kGWarps]) {
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < kGWarps; ++i) {
+    if (i >= parts) break;
+    const float4 y = *reinterpret_cast<const float4*>(o + (i * rows + r) * pitch + 4 * quad);
+    x.x = fmaf(f[i], y.x, x.x);
+    x.y = fmaf(f[i], y.y, x.y);
+    x.z = fmaf(f[i], y.z, x.z);
+    x.w = fmaf(f[i], y.w, x.w);
+  }
+  return x;
+}
+
+// A work item on CUDA cores: a CTA takes 32 of its rows (16 above head_dim 128), each warp up to 4 (2) of them. K and V
+// rows go from global memory straight to the registers of the warps that need them (L1 and L2 serve the others), so there
+// is neither a tile to fill for few rows nor a barrier. Bound by instruction issue and the latency of a step (about 1.1 us:
+// exchanges, rows on their way), which is why a warp keeps four rows, not eight: two CTAs are resident then. Measured,
+// float32, a layer: 9 prompts of 392 to 1,248 tokens x 3, 16 heads of 64, 33 us; 2 prompts of up to 9,963 x 6, 32 / 8
+// heads of 128, 177 us. (Tiles of 32 keys in shared memory for 64 rows took 303 and 434 us.)
+template <typename T, typename S>
+__global__ void __launch_bounds__(kGThreads, S::kEach == 4 ? 2 : 1) shared_generic_kernel(Args a) {
   extern __shared__ __align__(16) float gsm[];
   launch_dependents();
   Item it;
   if (!read_item(a, blockIdx.x, it)) return;
-  const int D = a.head_dim, P = generic_pitch(D), tid = threadIdx.x, r = tid >> 2, part = tid & 3;
-  const int rows = min(it.slab1 >= 0 ? 2 * kSlabRows : kSlabRows, it.n_rows - it.row0);
-  const int r0 = int(blockIdx.y) * kGRows;
-  if (r0 < rows) {
-    for (int i = tid >> 5; i < kGRows; i += kGThreads / 32) {
-      const char* src = r0 + i < rows ? query_row(a, it, it.row0 + r0 + i) : nullptr;
-      for (int d = tid & 31; d < D; d += 32)
-        gsm[i * P + d] = src != nullptr ? Elem<T>::to_f(reinterpret_cast<const T*>(src)[d]) : 0.f;
+  constexpr int kCtaRows = kGWarps * S::kRows;
+  const int P = generic_pitch(a.head_dim), tid = threadIdx.x;
+  const int r0 = int(blockIdx.y) * kCtaRows;
+  const int rows = min(min(it.slab1 >= 0 ? 2 * kSlabRows : kSlabRows, it.n_rows - it.row0) - r0, kCtaRows);
+  if (rows <= 0) return;
+  float* ml = gsm + kCtaRows * P;
+  auto key_off = [&](int pos) -> int64_t {
+    const int lb = pos / a.block_size;
+    const int blk = __ldg(a.run_blocks + it.block0 + lb);
+    if (blk < 0 || blk >= a.num_blocks) {
+      record_status(a.status, AUGUR_KV_EBOUNDS);
+      return -1;
     }
-    auto key_off = [&](int j) -> int64_t {
-      const int pos = it.key0 + j, lb = pos / a.block_size;
-      const int blk = __ldg(a.run_blocks + it.block0 + lb);
-      if (blk < 0 || blk >= a.num_blocks) {
-        record_status(a.status, AUGUR_KV_EBOUNDS);
-        return -1;
-      }
-      return int64_t(blk) * a.blk_stride + int64_t(it.kv_head) * a.head_stride +
-             int64_t(pos - lb * a.block_size) * a.row_stride;
-    };
-    float m, l, o[kGMaxDim / 4];
-    generic_attend<T>(a, gsm, it.key1 - it.key0, key_off, m, l, o);
-    const int row = r0 + r;
-    if (row < rows) {
-      const int64_t at = int64_t(row < kSlabRows ? it.slab0 : it.slab1) * kSlabRows + (row & (kSlabRows - 1));
-      if (part == 0) *reinterpret_cast<float2*>(a.slab_ml + at * 2) = make_float2(m, l);
-      const int64_t quad = (at / kSlabRows) * a.quads * kSlabRows + at % kSlabRows;
-#pragma unroll
-      for (int i = 0; i < kGMaxDim / 16; ++i)
-        if (4 * i + part < a.quads)
-          *reinterpret_cast<float4*>(a.slab_o + (quad + int64_t(4 * i + part) * kSlabRows) * 4) =
-              make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-    }
+    return int64_t(blk) * a.blk_stride + int64_t(it.kv_head) * a.head_stride + int64_t(pos - lb * a.block_size) * a.row_stride;
+  };
+  const Split sp(rows, S::kRows);
+  cta_attend<T, S>(a, [&](int r) { return query_row(a, it, it.row0 + r0 + r); }, rows, sp, it.key0, it.key1, key_off, ml, gsm, P);
+  for (int i = tid; i < rows * a.quads; i += kGThreads) {  // rows fastest, as the slabs lie
+    const int quad = i / rows, r = i - quad * rows, row = r0 + r;
+    float f[kGWarps];
+    const float2 x = part_factors(ml, rows, sp.key_warps, r, f);
+    const int64_t at = int64_t(row < kSlabRows ? it.slab0 : it.slab1) * kSlabRows + (row & (kSlabRows - 1));
+    if (quad == 0) *reinterpret_cast<float2*>(a.slab_ml + at * 2) = x;
+    const int64_t to = (at / kSlabRows) * a.quads * kSlabRows + at % kSlabRows + int64_t(quad) * kSlabRows;
+    *reinterpret_cast<float4*>(a.slab_o + to * 4) = join_quad(gsm, P, rows, sp.key_warps, r, quad, f);
   }
 }
 
@@ -509,136 +665,44 @@ __device__ __forceinline__ bool last_to_arrive(const Args& a, int unit) {
   return is_last != 0;
 }
 
-// A sequence's own keys on CUDA cores. Eight warps share 32 keys in shared
-// memory; a warp takes query heads w, w + 8, ..: for the scores its lanes are the
-// keys, for P V the dims (kDims = head_dim / 32 of them a lane, rounded up to 2, 4 or 8).
-// The next 32 keys' rows are on their way to registers meanwhile. Bound by the
-// latency of those loads with few heads, by shared-memory reads with many
-// (24 float32 sequences of 333 to 1,060 tokens, 14 / 2 heads of 64: 15.6 us).
-template <typename T, int kDims>
-__global__ void __launch_bounds__(kGThreads) own_generic_kernel(Args a) {
+// A sequence's own keys on CUDA cores, the query heads of the group as the rows. With few heads all warps share the
+// keys (a head of its own per KV head: eight warps, 64 keys a step of all). Bound by HBM and the latency of rows with a
+// head or two, by instruction issue with more. Measured, float32: 24 sequences of 333 to 1,060 tokens, 14 / 2 heads of 64:
+// 15.8 us; 724 of up to 436 own tokens, 16 heads of 64 (1.6 GB): 437 us (797 with a warp per head and 32 keys at a time).
+template <typename T, typename S>
+__global__ void __launch_bounds__(kGThreads, S::kEach == 4 ? 2 : 1) own_generic_kernel(Args a) {
   extern __shared__ __align__(16) float gsm[];
-  constexpr int kHeads = kDims == 8 ? 4 : 8;  // of a warp: heads x dims at most 8,192
   const int unit = blockIdx.x / a.n_split, part = blockIdx.x - unit * a.n_split;
   const int b = unit / a.hkv, hk = unit - b * a.hkv;
-  const int D = a.head_dim, P = generic_pitch(D), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.groups;
-  float* sk = gsm + kGRows * P;
-  float* sv = sk + kGKeys * P;
-  float* ml = gsm + generic_floats(D);  // [64][2]; the queries' place takes the output rows
+  const int P = generic_pitch(a.head_dim), tid = threadIdx.x, G = a.groups;
+  const Split sp(G, S::kRows);
+  const int all = sp.key_warps * G;  // rows of parts
+  float* ml = gsm + all * P;
   int first, last;
   own_range(a, b, first, last);
   part_range(a, part, kGKeys, first, last);
-  for (int i = warp; i < G; i += 8) {
-    const char* src = a.q + int64_t(b) * a.q_stride_b + int64_t(hk * G + i) * a.q_stride_h;
-    for (int d = lane; d < a.quads * 4; d += 32) gsm[i * P + d] = d < D ? Elem<T>::to_f(reinterpret_cast<const T*>(src)[d]) : 0.f;
-  }
-  float m[kHeads], l[kHeads], o[kHeads][kDims];
-#pragma unroll
-  for (int h = 0; h < kHeads; ++h) {
-    m[h] = kNegInf;
-    l[h] = 0.f;
-#pragma unroll
-    for (int c = 0; c < kDims; ++c) o[h][c] = 0.f;
-  }
-  constexpr int kKeys = kGKeys / 8;  // a warp fetches four keys' rows
-  T kr[kKeys][kDims], vr[kKeys][kDims];
-  bool there[kKeys];
-  auto fetch = [&](int k0) {
-    const int key = k0 + warp * kKeys + lane;
-    const int64_t mine = lane < kKeys && key < last ? own_row(a, b, hk, key) : -1;
-#pragma unroll
-    for (int i = 0; i < kKeys; ++i) {
-      const int64_t off = __shfl_sync(0xffffffffu, mine, i);
-      there[i] = off >= 0;
-#pragma unroll
-      for (int c = 0; c < kDims; ++c) {
-        const int d = min(c * 32 + lane, D - 1);  // in the row even where it is not used
-        kr[i][c] = reinterpret_cast<const T*>(a.k + max(off, int64_t(0)))[d];
-        vr[i][c] = reinterpret_cast<const T*>(a.v + max(off, int64_t(0)))[d];
-      }
-    }
-  };
-  if (first < last) fetch(first);
-  for (int k0 = first; k0 < last; k0 += kGKeys) {
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kKeys; ++i) {
-      const int key = warp * kKeys + i;
-#pragma unroll
-      for (int c = 0; c < kDims; ++c) {
-        const int d = c * 32 + lane;
-        const bool in = there[i] && d < D;
-        if (d < a.quads * 4) {
-          sk[key * P + d] = in ? Elem<T>::to_f(kr[i][c]) : 0.f;
-          sv[key * P + d] = in ? Elem<T>::to_f(vr[i][c]) : 0.f;
-        }
-      }
-    }
-    if (k0 + kGKeys < last) fetch(k0 + kGKeys);
-    __syncthreads();
-#pragma unroll
-    for (int h = 0; h < kHeads; ++h) {
-      const int head = warp + 8 * h;
-      if (head >= G) break;
-      float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
-      for (int d = 0; d < a.quads * 4; d += 4) {
-        const float4 x = *reinterpret_cast<const float4*>(gsm + head * P + d);
-        const float4 y = *reinterpret_cast<const float4*>(sk + lane * P + d);
-        s0 = fmaf(x.x, y.x, s0);
-        s1 = fmaf(x.y, y.y, s1);
-        s2 = fmaf(x.z, y.z, s2);
-        s3 = fmaf(x.w, y.w, s3);
-      }
-      const float s = k0 + lane < last ? ((s0 + s1) + (s2 + s3)) * a.scale : kNegInf;
-      float mn = s;
-#pragma unroll
-      for (int x = 16; x > 0; x >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, x));
-      mn = fmaxf(mn, m[h]);
-      const float alpha = mn == kNegInf ? 1.f : ex2(m[h] - mn);
-      const float p = mn == kNegInf ? 0.f : ex2(s - mn);
-      m[h] = mn;
-      l[h] = l[h] * alpha + p;
-#pragma unroll
-      for (int c = 0; c < kDims; ++c) o[h][c] *= alpha;
-#pragma unroll 8
-      for (int j = 0; j < kGKeys; ++j) {
-        const float pj = __shfl_sync(0xffffffffu, p, j);
-#pragma unroll
-        for (int c = 0; c < kDims; ++c)
-          o[h][c] = fmaf(pj, sv[j * P + min(c * 32 + lane, D - 1)], o[h][c]);
-      }
-    }
-  }
-  __syncthreads();
-#pragma unroll
-  for (int h = 0; h < kHeads; ++h) {
-    const int head = warp + 8 * h;
-    if (head >= G) break;
-    float sum = l[h];
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-    if (lane == 0) {
-      ml[2 * head] = m[h];
-      ml[2 * head + 1] = sum;
-    }
-#pragma unroll
-    for (int c = 0; c < kDims; ++c)
-      if (c * 32 + lane < a.quads * 4) gsm[head * P + c * 32 + lane] = o[h][c];
-  }
-  __syncthreads();
+  const char* q = a.q + int64_t(b) * a.q_stride_b + int64_t(hk * G) * a.q_stride_h;
+  cta_attend<T, S>(a, [&](int r) { return q + int64_t(r) * a.q_stride_h; }, G, sp, first, last,
+                   [&](int key) { return own_row(a, b, hk, key); }, ml, gsm, P);
+  float* join = ml + ((2 * all + 3) & ~3);
   if (a.n_split == 1) {
     wait_prerequisites();  // the shared launch's slabs
-    join_rows<T>(a, b, hk, 1, ml, gsm, kGRows, P, ml + 2 * kGRows);
+    join_rows<T>(a, b, hk, sp.key_warps, ml, gsm, G, P, join);
     return;
   }
   const int width = 4 * a.quads;
   const int64_t base = (int64_t(unit) * a.n_split + part) * G;
-  for (int i = tid; i < G * width; i += kGThreads) a.split_o[base * width + i] = gsm[i / width * P + i % width];
-  for (int i = tid; i < 2 * G; i += kGThreads) a.split_ml[base * 2 + i] = ml[i];
+  for (int i = tid; i < G * a.quads; i += kGThreads) {
+    const int r = i / a.quads, quad = i - r * a.quads;
+    float f[kGWarps];
+    const float2 x = part_factors(ml, G, sp.key_warps, r, f);
+    if (quad == 0) *reinterpret_cast<float2*>(a.split_ml + (base + r) * 2) = x;
+    *reinterpret_cast<float4*>(a.split_o + (base + r) * width + 4 * quad) = join_quad(gsm, P, G, sp.key_warps, r, quad, f);
+  }
   if (!last_to_arrive(a, unit)) return;
   wait_prerequisites();
   const int64_t unit0 = int64_t(unit) * a.n_split * G;
-  join_rows<T>(a, b, hk, a.n_split, a.split_ml + unit0 * 2, a.split_o + unit0 * width, G, width, ml + 2 * kGRows);
+  join_rows<T>(a, b, hk, a.n_split, a.split_ml + unit0 * 2, a.split_o + unit0 * width, G, width, join);
 }
 
 // ---------------------------------------------------------------------------
@@ -1055,23 +1119,6 @@ __device__ __forceinline__ void tmem_wait_ld32(uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Two float32 operations at a time.
-__device__ __forceinline__ uint64_t pack2(float x, float y) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 // A value that is the same in all lanes, in a form the compiler knows to be.
 __device__ __forceinline__ int warp_uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 // True in one lane of a converged warp.
@@ -1571,26 +1618,37 @@ int run_tensor(const Args& a, cudaStream_t st) {
   return a.groups <= 8 ? own(own_mma_kernel<T, D, 1>, 8, done1) : own(own_mma_kernel<T, D, 2>, 16, done2);
 }
 
-template <typename T>
+template <typename T, typename S>
+int launch_shared_generic(const Args& a, cudaStream_t st) {
+  static int done[augur_kv_dev::kMaxDevices] = {0};
+  constexpr int kCtaRows = kGWarps * S::kRows;
+  const int smem = kCtaRows * (generic_pitch(a.head_dim) + 2) * 4;
+  const int rc = allow_smem(reinterpret_cast<const void*>(shared_generic_kernel<T, S>), smem, done, "shared_generic_kernel");
+  if (rc != AUGUR_KV_OK) return rc;
+  shared_generic_kernel<T, S><<<dim3(unsigned(a.n_items), 2 * kSlabRows / kCtaRows), kGThreads, size_t(smem), st>>>(a);
+  return augur_kv_dev::check_launch("shared_generic_kernel");
+}
+template <typename T, typename S, typename O>
 int run_generic(const Args& a, cudaStream_t st) {
-  const int shared = generic_floats(a.head_dim) * 4;
-  const int smem = shared + 2 * kGRows * 4 + join_bytes(a.groups);
-  static int done_s[augur_kv_dev::kMaxDevices] = {0}, done_o[3][augur_kv_dev::kMaxDevices] = {{0}};
+  static int done[augur_kv_dev::kMaxDevices] = {0};
+  const int pitch = generic_pitch(a.head_dim);
   if (a.n_items > 0) {
-    const int rc = allow_smem(reinterpret_cast<const void*>(shared_generic_kernel<T>), shared, done_s, "shared_generic_kernel");
+    const int rc = launch_shared_generic<T, S>(a, st);
     if (rc != AUGUR_KV_OK) return rc;
-    shared_generic_kernel<T><<<dim3(unsigned(a.n_items), 2 * kSlabRows / kGRows), kGThreads, size_t(shared), st>>>(a);
-    const int lc = augur_kv_dev::check_launch("shared_generic_kernel");
-    if (lc != AUGUR_KV_OK) return lc;
   }
-  auto own = [&](auto kernel, int (&done)[augur_kv_dev::kMaxDevices]) {
-    const int rc = allow_smem(reinterpret_cast<const void*>(kernel), smem, done, "own_generic_kernel");
-    if (rc != AUGUR_KV_OK) return rc;
-    return launch_own(kernel, a, a.batch * a.hkv * a.n_split, kGThreads, size_t(smem), a.n_items > 0, st, "own_generic_kernel");
-  };
-  if (a.head_dim <= 64) return own(own_generic_kernel<T, 2>, done_o[0]);
-  if (a.head_dim <= 128) return own(own_generic_kernel<T, 4>, done_o[1]);
-  return own(own_generic_kernel<T, 8>, done_o[2]);
+  // rows of parts: at most a row for each warp's each, or the heads where these are more
+  const int rows = a.groups > kGWarps * O::kRows ? a.groups : kGWarps * O::kRows;
+  const int smem = rows * (pitch + 2) * 4 + 16 + join_bytes(a.groups);
+  const int rc = allow_smem(reinterpret_cast<const void*>(own_generic_kernel<T, O>), smem, done, "own_generic_kernel");
+  if (rc != AUGUR_KV_OK) return rc;
+  return launch_own(own_generic_kernel<T, O>, a, a.batch * a.hkv * a.n_split, kGThreads, size_t(smem), a.n_items > 0, st,
+                    "own_generic_kernel");
+}
+template <typename T>
+int pick_generic(const Args& a, cudaStream_t st) {
+  if (a.head_dim <= 64) return run_generic<T, Shape<4, 16, 4>, Shape<4, 16, 2>>(a, st);
+  if (a.head_dim <= 128) return run_generic<T, Shape<4, 32, 4>, Shape<4, 32, 2>>(a, st);
+  return run_generic<T, Shape<8, 32, 2>, Shape<8, 32, 2>>(a, st);
 }
 
 // Parts of a sequence's own keys: enough CTAs for the GPU, and at least `least` keys a part
@@ -1652,10 +1710,10 @@ AUGUR_KV_EXPORT int augur_kv_shared_prefix_attention(const augur_kv_shared_prefi
   Args a;
   memset(&a, 0, sizeof(a));
   a.groups = p->n_q_heads / p->n_kv_heads;
-  if (a.groups > kGRows || p->head_dim > kGMaxDim || a.groups * ((p->head_dim + 3) / 4) > 8 * kGThreads)
+  if (a.groups > kGMaxRows || p->head_dim > kGMaxDim || a.groups * ((p->head_dim + 3) / 4) > 8 * kGThreads)
     return fail(AUGUR_KV_EINVAL,
                 "shared_prefix_attention: at most %d query heads per KV head, head_dim %d, and %d values of both together",
-                kGRows, kGMaxDim, 32 * kGThreads);
+                kGMaxRows, kGMaxDim, 32 * kGThreads);
   const int64_t ls = p->pool_strides[0] * es;
   a.q = static_cast<const char*>(q);
   a.q_stride_b = p->q_strides[0] * es;
@@ -1681,6 +1739,10 @@ AUGUR_KV_EXPORT int augur_kv_shared_prefix_attention(const augur_kv_shared_prefi
   a.out_stride_b = p->out_strides[0] * es;
   a.out_stride_h = p->out_strides[1] * es;
   a.quads = (p->head_dim + 3) / 4;
+  a.rows_wide = p->head_dim % 4 == 0 &&
+                ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
+                  uintptr_t(a.q_stride_b) | uintptr_t(a.q_stride_h) | uintptr_t(a.blk_stride) | uintptr_t(a.head_stride) |
+                  uintptr_t(a.row_stride)) & uintptr_t(4 * es - 1)) == 0;
   a.out_wide = p->head_dim % 4 == 0 && ((reinterpret_cast<uintptr_t>(out) | uintptr_t(a.out_stride_b) | uintptr_t(a.out_stride_h)) & uintptr_t(4 * es - 1)) == 0;
   a.items = reinterpret_cast<const Item*>(p->items);
   a.n_items = p->n_items;
@@ -1740,7 +1802,7 @@ AUGUR_KV_EXPORT int augur_kv_shared_prefix_attention(const augur_kv_shared_prefi
       return p->head_dim == 64 ? run_tensor<__nv_bfloat16, 64>(a, st) : run_tensor<__nv_bfloat16, 128>(a, st);
     return p->head_dim == 64 ? run_tensor<__half, 64>(a, st) : run_tensor<__half, 128>(a, st);
   }
-  if (p->dtype == AUGUR_KV_F32) return run_generic<float>(a, st);
-  if (p->dtype == AUGUR_KV_F16) return run_generic<__half>(a, st);
-  return run_generic<__nv_bfloat16>(a, st);
+  if (p->dtype == AUGUR_KV_F32) return pick_generic<float>(a, st);
+  if (p->dtype == AUGUR_KV_F16) return pick_generic<__half>(a, st);
+  return pick_generic<__nv_bfloat16>(a, st);
 }
