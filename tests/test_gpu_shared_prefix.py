@@ -132,6 +132,20 @@ _BATCHES = {
 }
 
 
+@pytest.mark.parametrize("n", [2, 3, 5, 9, 17, 33, 70])  # rows of a run: all divisions of a CTA's warps into rows and keys
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim", [
+    (torch.float32, 2, 2, 64), (torch.float32, 6, 2, 128), (torch.float32, 4, 4, 256), (torch.bfloat16, 3, 1, 100), (torch.float16, 5, 1, 30)])
+def test_rows_and_keys_divided_among_warps(cuda, n, dtype, heads, kv_heads, dim):
+    case = Case(cuda, dtype, heads, kv_heads, dim, 8, forks(n, 777, 8, lambda i: 1 + 13 * (i % 11)), seed=n)
+    case.check(paged_shared_prefix_attention(case.q, case.pool, case.layer, case.tables, kernel="generic"))
+
+
+@pytest.mark.parametrize("heads", [1, 9, 24, 33, 64])  # of one KV head: one warp's, and more than all warps take at once
+def test_many_heads_of_one_kv_head(cuda, heads):
+    case = Case(cuda, torch.float32, heads, 1, 64, 16, forks(4, 333, 16, lambda i: 1 + 100 * i), seed=heads)
+    case.check(paged_shared_prefix_attention(case.q, case.pool, case.layer, case.tables))
+
+
 @pytest.mark.parametrize("kernel", ["tcgen05", "generic"])
 @pytest.mark.parametrize("name", _BATCHES)
 @pytest.mark.parametrize("heads,kv_heads,dim", [(14, 2, 64), (8, 2, 128)])
