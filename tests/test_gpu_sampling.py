@@ -301,3 +301,31 @@ def test_wide_nuclei(cuda, seed):
     want, want_logprobs = whole_number_rows(x, u, t, zero.int(), top_p, zero)
     assert torch.equal(tokens, want)
     assert ((logprobs.double() - want_logprobs).abs() <= 2.0 ** -21 * (1 + 25 + want_logprobs.abs())).all()
+
+
+@pytest.mark.parametrize("temperature", [0.03, 1.0, 40.0])
+@pytest.mark.parametrize("move", ["maximum 0", "cut near 0", "far up", "far down", "tiny", "huge"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_limits_anywhere_among_the_floats(cuda, move, temperature, dtype):
+    g = torch.Generator(device=cuda).manual_seed(17)
+    rows, vocab = 12, 20011
+    x = torch.randn(rows, vocab, generator=g, device=cuda) * 2.0 * temperature
+    if move == "maximum 0":
+        x = x - x.amax(1, keepdim=True)
+    elif move == "cut near 0":  # where the floats are densest
+        x = x - x.topk(400, dim=1).values[:, -1:]
+    elif move in ("far up", "far down"):
+        x = x + (1e5 if move == "far up" else -1e5) * temperature
+    elif move in ("tiny", "huge"):
+        scale = 1e-30 if move == "tiny" else 1e30
+        x, temperature = x * scale, temperature * scale
+    logits = x.to(dtype)
+    uniform = torch.rand(rows, generator=g, device=cuda)
+    for k, p, m in ((50, 1.0, 0.0), (0, 0.9, 0.0), (3000, 0.7, 0.0), (0, 1.0, 0.05), (0, 0.97, 0.001)):
+        per_row = (torch.full((rows,), v, dtype=d, device=cuda)
+                   for v, d in ((temperature, torch.float32), (k, torch.int32), (p, torch.float32), (m, torch.float32)))
+        tokens, logprobs = sample_tokens(logits, uniform, temperature, k, p, m)
+        want, want_logprobs = whole_number_rows(logits, uniform, *per_row)
+        assert torch.equal(tokens, want), (k, p, m)
+        # as in check: float32 roundings of z, of the kept sum's logarithm and of their difference
+        assert ((logprobs.double() - want_logprobs).abs() <= 2.0 ** -21 * (26 + want_logprobs.abs())).all()
